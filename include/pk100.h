@@ -629,6 +629,121 @@ int pk100_mel_frontend(void* stream, const pk100_frontend_weights* weights, cons
                        int utterances, long long sample_stride, const int* sample_counts, float* mel,
                        int frame_cap, int* valid_frames);
 
+/* ------------------------------------------------------------------------
+ * Operators of a language-model layer in serving, for hosts that run a decoder-only model behind the encoder
+ * (no reference counterpart).  Activations are fp16 or bf16, weights of the products as above; statistics,
+ * softmax and sums are fp32. */
+enum { PK100_TYPE_F16 = 0, PK100_TYPE_BF16 = 1 };
+
+/* Bits that the operators below set in their device status word (OR-ed, never cleared). */
+enum {
+    PK100_STATUS_PLAN = 16,    /* pk100_paged_plan refused the step */
+    PK100_STATUS_PAGE = 32     /* a page id, slot or length pointed outside the cache */
+};
+
+/* Residual addition and root-mean-square norm:
+ *   s = round(input + residual)  (residual == NULL: s = input), written to residual_out when given (may alias
+ *       either input);
+ *   y = s * rsqrt(mean(s^2) + eps) * gamma, in fp32 from the rounded s;
+ *   output in `mode`: PK100_LN_F16 = round(y) in the input's type; PK100_LN_E4M3_FIXED = E4M3(y * inv_scale);
+ *   PK100_LN_E4M3_ROW = E4M3(y / c), c = max|y| / 448; PK100_LN_S8_ROW = rne(y / c), c = max|y| / 127, c -> scales
+ *   (0 -> 1): the operands of pk100_gemm kinds E4M3 and S8.  A row with a NaN or an infinity takes its maximum over
+ *   what is a number; NaN becomes INT8 0 or E4M3 NaN.
+ * Leading dimensions are in elements of their array; any width up to 32768, any alignment of the elements (rows
+ * whose pointers and strides are multiples of 16 bytes, 8 for 8-bit outputs, are the fast ones). */
+typedef struct pk100_rms_norm_args {
+    int type;                                     /* PK100_TYPE_* of input, residual, gamma and PK100_LN_F16 output */
+    int mode;                                     /* PK100_LN_F16, _E4M3_FIXED, _E4M3_ROW or _S8_ROW */
+    int rows, width;
+    const void* input;    long long ld_in;
+    const void* residual; long long ld_res;       /* NULL: no addition */
+    void* residual_out;   long long ld_res_out;   /* NULL: s is not kept */
+    const void* gamma;                            /* [width] */
+    float eps, inv_scale;
+    void* output;         long long ld_out;
+    float* scales;                                /* fp32 [rows], the per-row modes */
+} pk100_rms_norm_args;
+
+int pk100_add_rms_norm(void* stream, const pk100_rms_norm_args* args);
+
+/* PK100_KIND_F16_W4G128 for 1 to 16 rows (single tokens of a few requests), where the product is bound by the
+ * weights' bytes and pk100_gemm's tiles are mostly padding: the same arguments, weights W = f16(code * scale) and
+ * epilogue algebra, fp32 sums (in another order than pk100_gemm's).  Any n; k % 128 == 0; a and b 16-byte
+ * aligned, lda % 8 == 0; out and residual of any leading dimension; PK100_EPI_LINEAR; out_type PK100_OUT_F16 or
+ * _F32.  More than 16 rows: PK100_ERR_LIMIT.  tau, keep_*, stats_out, status and max_ctas are not read. */
+int pk100_gemv_w4g128(void* stream, const pk100_gemm_args* args);
+
+/* One step's bookkeeping of a paged key-value cache, from the request lengths alone:
+ *   starts[r] = sum of new_tokens before r (starts[requests] = all of them), lengths[r] = cached[r] + new_tokens[r];
+ *   request r takes ceil(lengths[r] / page_size) - ceil(cached[r] / page_size) pages from the front of free_pages,
+ *   in request order, into its row of block_table behind those it has; *used = pages taken;
+ *   token t of request r, i-th new one: positions[t] = cached[r] + i,
+ *   slots[t] = block_table[r][positions[t] / page_size] * page_size + positions[t] % page_size.
+ * Rows t >= starts[requests] get slot and position -1.  Where the step does not fit (a negative length, more new
+ * tokens than `tokens`, more pages than *free_count or max_pages) nothing is taken: PK100_STATUS_PLAN is set in
+ * *status, starts and *used are 0, lengths = cached, every slot and position -1, block_table as it was.  At most
+ * PK100_PLAN_MAX_REQUESTS requests (PK100_ERR_LIMIT).  Outputs overlap no input (lengths == cached is refused). */
+#define PK100_PLAN_MAX_REQUESTS 4096
+typedef struct pk100_paged_plan_args {
+    int requests, tokens, page_size, max_pages;
+    const int* cached;                            /* [requests] */
+    const int* new_tokens;                        /* [requests] */
+    const int* free_pages; const int* free_count; /* page ids (NULL: none); device count of them */
+    int* block_table;                             /* [requests, max_pages], rows beyond a request's pages are not read */
+    int* starts;                                  /* [requests + 1] */
+    int* lengths;                                 /* [requests] */
+    int* positions;                               /* [tokens] */
+    long long* slots;                             /* [tokens] */
+    int* used;                                    /* [1] */
+    int* status;                                  /* may be NULL */
+} pk100_paged_plan_args;
+
+int pk100_paged_plan(void* stream, const pk100_paged_plan_args* args);
+
+/* Attention of new tokens over a paged key-value cache.  Request r owns rows [starts[r], starts[r + 1]) of query and
+ * out; its keys are the first lengths[r] positions of its pages, the new tokens' own among them, and its i-th new
+ * token stands at position p = lengths[r] - new + i:
+ *   out = softmax_j(scale * q . k_j) . v_j over the positions j < lengths[r], j <= p when causal, j > p - window when
+ *   window > 0;  lse (fp32 [tokens, heads], may be NULL) = log sum_j exp(scale * q . k_j).
+ * A row that sees nothing gets zeros and lse -infinity.  Rows behind starts[requests] are not touched.
+ * Query head h reads key-value head h / (heads / kv_heads).  head_dim 64 or 128; page_size 16, 32, 64, 128 or 256.
+ * Element (page, token, head, d) of both caches is at page * page_stride + token * token_stride + head * head_stride
+ * + d (elements; strides multiples of 8, pointers 16-byte aligned); heads of a token of query, key, value and out are
+ * head_dim apart, tokens ld_* apart (multiples of 8).
+ * key != NULL: key and value [tokens, kv_heads, head_dim] are written to slots first (negative slots are skipped,
+ * two tokens never share one); the caches are not written otherwise.
+ * What is behind lengths[r] in a page, and pages behind it, may hold anything, infinities and NaN included; keys and
+ * values in front of it are multiplied by zero weights too, so a value that is not finite reaches the rows of its
+ * request that do not see it.  A page id outside [0, pages) reads as zeros, a slot outside the cache is not
+ * written, a length beyond max_pages pages is cut; each sets PK100_STATUS_PAGE.  Bit 0: a bounded wait expired.
+ * max_new: no request has more new tokens than this (<= 0: not known).  It chooses kernels, no result but rounding
+ * depends on it; requests beyond it are attended all the same.
+ * workspace: >= pk100_paged_attention_workspace_bytes(args) bytes, 256-byte aligned, used by the call until it has
+ * completed; calls that may overlap on the GPU need one each. */
+typedef struct pk100_paged_attention_args {
+    int type;                                     /* PK100_TYPE_* of every activation and of the caches */
+    int tokens, requests, heads, kv_heads, head_dim, pages, page_size, max_pages;
+    const void* query;    long long ld_query;
+    const void* key;      long long ld_key;
+    const void* value;    long long ld_value;
+    const long long* slots;                       /* [tokens], with key */
+    void* key_cache;      void* value_cache;
+    long long page_stride, token_stride, head_stride;
+    const int* starts;                            /* [requests + 1] */
+    const int* lengths;                           /* [requests] */
+    const int* block_table;                       /* [requests, max_pages] */
+    int causal, window, max_new;
+    float scale;
+    void* out;            long long ld_out;
+    float* lse;
+    void* workspace;      long long workspace_bytes;
+    int* status;                                  /* may be NULL */
+} pk100_paged_attention_args;
+
+/* Depends on tokens, requests, heads, kv_heads, head_dim and max_pages * page_size alone; 0 where the arguments are refused. */
+long long pk100_paged_attention_workspace_bytes(const pk100_paged_attention_args* args);
+int pk100_paged_attention(void* stream, const pk100_paged_attention_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -269,6 +269,17 @@ int pk100_tensor_map_2d(void* map, const void* base, int elem_bytes, unsigned lo
     return make_map(static_cast<CUtensorMap*>(map), base, elem_bytes, rows, cols, ld, box_rows, swizzle_bytes);
 }
 
+int pk100_tensor_map_4d(void* map, const void* base, const unsigned long long (&dims)[4], const unsigned long long (&strides)[3],
+                        const unsigned (&box)[4]) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) return PK100_ERR_DRIVER;
+    const cuuint64_t extents[4] = {dims[0], dims[1], dims[2], dims[3]}, steps[3] = {strides[0], strides[1], strides[2]};
+    const cuuint32_t boxes[4] = {box[0], box[1], box[2], box[3]}, ones[4] = {1, 1, 1, 1};
+    return fn(static_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), extents, steps, boxes, ones,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? PK100_OK : PK100_ERR_DRIVER;
+}
+
 int pk100_cta_budget() { return pk100::shared_budget(); }
 
 bool pk100_dependent_launch_enabled() { return pk100::g_dependent_launch.load(std::memory_order_relaxed) != 0; }

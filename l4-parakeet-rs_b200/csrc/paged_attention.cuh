@@ -1,0 +1,56 @@
+// Shared by the kernels of attention over a paged cache: parameters, geometry of a request, tensor-map loads.
+#pragma once
+
+#include <cuda.h>
+
+#include "element16.cuh"
+#include "pk100_internal.h"
+#include "ptx_sm100.cuh"
+
+namespace pk100 {
+
+struct PagedParams {
+    const void* query; long long ld_query;
+    void* out; long long ld_out;
+    float* lse;
+    const int* starts; const int* lengths; const int* table;
+    int tokens, requests, heads, kv_heads, group;      // group: query heads of a key-value head
+    int pages, page_shift, max_pages, causal, window;  // window: 0 or up to 2^30
+    float scale_log2;                                  // scale * log2(e)
+    int few_rows;                                      // requests of up to this many (token, head) rows belong to the few-row kernel
+    int* status;
+};
+
+constexpr float kLn2 = 0.6931471805599453f;
+
+// A request as the kernels see it: whatever the arrays hold, no row lies outside the batch, no key outside the table.
+struct PagedRequest {
+    int row0, n, len;
+    bool cut;
+    __device__ __forceinline__ PagedRequest(const PagedParams& p, int r) {
+        const int first = p.starts[r], end = p.starts[r + 1], length = p.lengths[r];
+        row0 = min(max(first, 0), p.tokens);
+        n = max(min(end, p.tokens) - row0, 0);
+        const int capacity = p.max_pages << p.page_shift;
+        len = min(max(length, 0), capacity);
+        cut = length != len || first < 0 || end > p.tokens;
+    }
+    // keys that the i-th new token sees: [lo, hi)
+    __device__ __forceinline__ int hi(const PagedParams& p, int i) const { return p.causal ? max(min(len - n + i + 1, len), 0) : len; }
+    __device__ __forceinline__ int lo(const PagedParams& p, int i) const { return p.window > 0 ? max(len - n + i - p.window + 1, 0) : 0; }
+};
+
+// 4-D tiled load (feature, token in page, head, page); the feature coordinate is a multiple of 64 here.
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int32_t c0, int32_t c1, int32_t c2, int32_t c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+}  // namespace pk100

@@ -128,3 +128,8 @@ int pk100_cta_budget();
 // (gemm_host.cu).  `map` points to a CUtensorMap.
 int pk100_tensor_map_2d(void* map, const void* base, int elem_bytes, unsigned long long rows,
                         unsigned long long cols, unsigned long long ld, int box_rows, int swizzle_bytes);
+
+// 4-D TMA descriptor of 16-bit elements (dims innermost first, strides of dims 1..3 in bytes), 128-byte swizzle, zeros
+// outside the tensor; not cached here.
+int pk100_tensor_map_4d(void* map, const void* base, const unsigned long long (&dims)[4], const unsigned long long (&strides)[3],
+                        const unsigned (&box)[4]);

@@ -1,0 +1,222 @@
+// Residual addition + root-mean-square norm with the output encodings of the 8-bit products.
+#include <cuda_fp8.h>
+
+#include "element16.cuh"
+#include "pk100_internal.h"
+#include "ptx_sm100.cuh"
+
+namespace pk100 {
+
+struct RmsNormParams {
+    int rows, width, threads;         // threads: of a row
+    const void* input;    long long ld_in;
+    const void* residual; long long ld_res;
+    void* residual_out;   long long ld_res_out;
+    const void* gamma;
+    float eps, inv_scale;
+    void* output;         long long ld_out;
+    float* scales;
+    bool vec_in, vec_res, vec_res_out, vec_gamma, vec_out;      // 16-byte (8-bit output: 8-byte) rows
+};
+
+__device__ __forceinline__ void store_codes(uint8_t* row, int column, int width, bool vec, uint2 v) {
+    if (vec) {
+        if (column < width) *reinterpret_cast<uint2*>(row + column) = v;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (column + i < width) row[column + i] = static_cast<uint8_t>((i < 4 ? v.x : v.y) >> (8 * (i % 4)));
+}
+
+// A row belongs to a warp (8 rows a block) or to a whole block; every thread keeps Chunks x 8 of its elements, so
+// the row is read once.  Mean square and max |s * gamma| leave in ONE reduction: max |y| = rstd * max |s * gamma|.
+// Sums are fp32 in a fixed order.  The codes are formed from the fp32 y: rounding it to 16 bits first would cost
+// bf16 rows a bit of their 7-bit codes.  Bound by HBM for many rows, by the latency of load, reduction and store
+// for a few.
+template <typename T, int Mode, int Chunks>
+__global__ void __launch_bounds__(1024)
+add_rms_norm_kernel(const RmsNormParams p) {
+    __shared__ float part_sum[32], part_max[32];
+    grid_dependents_launch();
+    grid_dependency_wait();
+    const int per_block = blockDim.x / p.threads;
+    const int row = blockIdx.x * per_block + threadIdx.x / p.threads, t = threadIdx.x % p.threads;
+    if (row >= p.rows) return;                          // (whole warps; blocks of one row have none)
+    const T* in = static_cast<const T*>(p.input) + row * p.ld_in;
+    const T* gamma = static_cast<const T*>(p.gamma);
+    uint4 s[Chunks], g[Chunks];
+#pragma unroll
+    for (int c = 0; c < Chunks; ++c) s[c] = load8(in, (c * p.threads + t) * 8, p.width, p.vec_in);
+    if (p.residual != nullptr) {
+        const T* res = static_cast<const T*>(p.residual) + row * p.ld_res;
+        uint4 r[Chunks];
+#pragma unroll
+        for (int c = 0; c < Chunks; ++c) r[c] = load8(res, (c * p.threads + t) * 8, p.width, p.vec_res);
+#pragma unroll
+        for (int c = 0; c < Chunks; ++c) {
+            uint32_t* a = reinterpret_cast<uint32_t*>(&s[c]);
+            const uint32_t* b = reinterpret_cast<const uint32_t*>(&r[c]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 x = floats_of(a[i], T()), y = floats_of(b[i], T());
+                a[i] = packed_of(x.x + y.x, x.y + y.y, T());
+            }
+        }
+    }
+    if (p.residual_out != nullptr) {
+        T* o = static_cast<T*>(p.residual_out) + row * p.ld_res_out;
+#pragma unroll
+        for (int c = 0; c < Chunks; ++c) store8(o, (c * p.threads + t) * 8, p.width, p.vec_res_out, s[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < Chunks; ++c) g[c] = load8(gamma, (c * p.threads + t) * 8, p.width, p.vec_gamma);
+    constexpr bool kRowScale = Mode == PK100_LN_E4M3_ROW || Mode == PK100_LN_S8_ROW;
+    float sum = 0.0f, top = 0.0f;
+#pragma unroll
+    for (int c = 0; c < Chunks; ++c) {
+        const uint32_t* a = reinterpret_cast<const uint32_t*>(&s[c]);
+        const uint32_t* b = reinterpret_cast<const uint32_t*>(&g[c]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 x = floats_of(a[i], T());
+            sum = fmaf(x.x, x.x, sum);
+            sum = fmaf(x.y, x.y, sum);
+            if constexpr (kRowScale) {
+                const float2 y = floats_of(b[i], T());
+                const float u = fabsf(x.x * y.x), v = fabsf(x.y * y.y);
+                if (u < INFINITY) top = fmaxf(top, u);              // what is a number
+                if (v < INFINITY) top = fmaxf(top, v);
+            }
+        }
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off /= 2) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if constexpr (kRowScale) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    }
+    if (p.threads > 32) {                               // the block is one row
+        const int warps = p.threads / 32, warp = t / 32, lane = t % 32;
+        if (lane == 0) {
+            part_sum[warp] = sum;
+            part_max[warp] = top;
+        }
+        __syncthreads();
+        sum = lane < warps ? part_sum[lane] : 0.0f;
+        top = kRowScale && lane < warps ? part_max[lane] : 0.0f;
+#pragma unroll
+        for (int off = 16; off > 0; off /= 2) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            if constexpr (kRowScale) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        }
+    }
+    const float rstd = rsqrtf(sum / p.width + p.eps);
+    float scale = 1.0f, inverse = p.inv_scale;
+    if constexpr (kRowScale) {
+        const float peak = top * rstd;
+        if (peak > 0.0f && peak < INFINITY) scale = __fdiv_rn(peak, Mode == PK100_LN_E4M3_ROW ? 448.0f : 127.0f);
+        inverse = __frcp_rn(scale);
+        if (t == 0) p.scales[row] = scale;
+    }
+#pragma unroll
+    for (int c = 0; c < Chunks; ++c) {
+        const int column = (c * p.threads + t) * 8;
+        const uint32_t* a = reinterpret_cast<const uint32_t*>(&s[c]);
+        const uint32_t* b = reinterpret_cast<const uint32_t*>(&g[c]);
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 x = floats_of(a[i], T()), w = floats_of(b[i], T());
+            y[2 * i] = x.x * rstd * w.x;
+            y[2 * i + 1] = x.y * rstd * w.y;
+        }
+        if constexpr (Mode == PK100_LN_F16) {
+            T* o = static_cast<T*>(p.output) + row * p.ld_out;
+            store8(o, column, p.width, p.vec_out, make_uint4(packed_of(y[0], y[1], T()), packed_of(y[2], y[3], T()),
+                                                             packed_of(y[4], y[5], T()), packed_of(y[6], y[7], T())));
+        } else {
+            uint32_t w[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                // a scale below the smallest normal number has no finite reciprocal: divide
+                const float lo = inverse < INFINITY ? y[2 * i] * inverse : y[2 * i] / scale;
+                const float hi = inverse < INFINITY ? y[2 * i + 1] * inverse : y[2 * i + 1] / scale;
+                if constexpr (Mode == PK100_LN_S8_ROW) {
+                    const int u = max(-127, min(127, __float2int_rn(lo))), v = max(-127, min(127, __float2int_rn(hi)));
+                    w[i / 2] |= static_cast<uint32_t>((u & 255) | ((v & 255) << 8)) << (16 * (i % 2));
+                } else {
+                    w[i / 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3))
+                                << (16 * (i % 2));
+                }
+            }
+            store_codes(static_cast<uint8_t*>(p.output) + row * p.ld_out, column, p.width, p.vec_out, make_uint2(w[0], w[1]));
+        }
+    }
+}
+
+template <typename T, int Mode>
+static void launch_rms_norm(const RmsNormParams& p, int chunks, int blocks, int block, cudaStream_t stream) {
+    if (chunks == 1) pk100_launch_chained(add_rms_norm_kernel<T, Mode, 1>, dim3(blocks), dim3(block), 0, stream, p);
+    else if (chunks == 2) pk100_launch_chained(add_rms_norm_kernel<T, Mode, 2>, dim3(blocks), dim3(block), 0, stream, p);
+    else pk100_launch_chained(add_rms_norm_kernel<T, Mode, 4>, dim3(blocks), dim3(block), 0, stream, p);
+}
+
+template <typename T>
+static void launch_rms_norm(const RmsNormParams& p, int mode, int chunks, int blocks, int block, cudaStream_t stream) {
+    if (mode == PK100_LN_F16) launch_rms_norm<T, PK100_LN_F16>(p, chunks, blocks, block, stream);
+    else if (mode == PK100_LN_E4M3_FIXED) launch_rms_norm<T, PK100_LN_E4M3_FIXED>(p, chunks, blocks, block, stream);
+    else if (mode == PK100_LN_E4M3_ROW) launch_rms_norm<T, PK100_LN_E4M3_ROW>(p, chunks, blocks, block, stream);
+    else launch_rms_norm<T, PK100_LN_S8_ROW>(p, chunks, blocks, block, stream);
+}
+
+}  // namespace pk100
+
+using namespace pk100;
+
+extern "C" int pk100_add_rms_norm(void* stream, const pk100_rms_norm_args* a) {
+    if (a == nullptr) return PK100_ERR_NULL;
+    if (a->type != PK100_TYPE_F16 && a->type != PK100_TYPE_BF16) return PK100_ERR_UNSUPPORTED;
+    if (a->mode < PK100_LN_F16 || a->mode > PK100_LN_S8_ROW) return PK100_ERR_UNSUPPORTED;
+    if (a->rows < 0 || a->width <= 0) return PK100_ERR_SHAPE;
+    if (a->width > 32768) return PK100_ERR_LIMIT;
+    if (a->rows == 0) return PK100_OK;
+    const bool row_scale = a->mode == PK100_LN_E4M3_ROW || a->mode == PK100_LN_S8_ROW;
+    if (a->input == nullptr || a->gamma == nullptr || a->output == nullptr || (row_scale && a->scales == nullptr)) return PK100_ERR_NULL;
+    const long long least = a->rows > 1 ? a->width : 0;             // (a single row has no distance)
+    if (a->ld_in < least || a->ld_out < least || (a->residual != nullptr && a->ld_res < least) ||
+        (a->residual_out != nullptr && a->ld_res_out < least))
+        return PK100_ERR_SHAPE;
+    auto odd = [](const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 1u) != 0; };
+    if (odd(a->input) || odd(a->gamma) || odd(a->residual) || odd(a->residual_out) || (a->mode == PK100_LN_F16 && odd(a->output)) ||
+        (reinterpret_cast<uintptr_t>(a->scales) & 3u))
+        return PK100_ERR_ALIGN;
+    // rows of 8 elements at a time: whole chunks, and every row starts on their boundary
+    auto vec = [&](const void* ptr, long long ld, unsigned bytes) {
+        return a->width % 8 == 0 && (reinterpret_cast<uintptr_t>(ptr) % bytes) == 0 && (a->rows == 1 || ld % 8 == 0);
+    };
+    RmsNormParams p{};
+    p.rows = a->rows; p.width = a->width;
+    p.input = a->input; p.ld_in = a->ld_in;
+    p.residual = a->residual; p.ld_res = a->ld_res;
+    p.residual_out = a->residual_out; p.ld_res_out = a->ld_res_out;
+    p.gamma = a->gamma; p.eps = a->eps; p.inv_scale = a->inv_scale;
+    p.output = a->output; p.ld_out = a->ld_out; p.scales = a->scales;
+    p.vec_in = vec(a->input, a->ld_in, 16);
+    p.vec_res = vec(a->residual, a->ld_res, 16);
+    p.vec_res_out = vec(a->residual_out, a->ld_res_out, 16);
+    p.vec_gamma = vec(a->gamma, 8, 16);
+    p.vec_out = vec(a->output, a->ld_out, a->mode == PK100_LN_F16 ? 16 : 8);
+    // Few rows: one chunk a thread, the shortest chain.  Many: two chunks in flight a thread.  A row that 32
+    // threads hold goes to a warp, without the exchange through shared memory.
+    const int need = (a->width + 7) / 8;
+    const bool many = a->rows > 4 * pk100_sm_count();
+    int chunks = many ? 2 : 1;
+    if (need <= 32) chunks = 1;
+    while (chunks < 4 && (need + chunks - 1) / chunks > 1024) chunks *= 2;
+    p.threads = ((need + chunks - 1) / chunks + 31) / 32 * 32;
+    const int block = p.threads == 32 ? 256 : p.threads;
+    const int blocks = (a->rows + block / p.threads - 1) / (block / p.threads);
+    if (a->type == PK100_TYPE_F16) launch_rms_norm<__half>(p, a->mode, chunks, blocks, block, static_cast<cudaStream_t>(stream));
+    else launch_rms_norm<__nv_bfloat16>(p, a->mode, chunks, blocks, block, static_cast<cudaStream_t>(stream));
+    return pk100_launch_status();
+}

@@ -34,6 +34,36 @@ class GemmArgs(C.Structure):
     ]
 
 
+class RmsNormArgs(C.Structure):
+    """Mirror of `pk100_rms_norm_args`."""
+    _fields_ = [
+        ("type", i32), ("mode", i32), ("rows", i32), ("width", i32),
+        ("input", vp), ("ld_in", i64), ("residual", vp), ("ld_res", i64), ("residual_out", vp), ("ld_res_out", i64),
+        ("gamma", vp), ("eps", f32), ("inv_scale", f32), ("output", vp), ("ld_out", i64), ("scales", vp),
+    ]
+
+
+class PagedPlanArgs(C.Structure):
+    """Mirror of `pk100_paged_plan_args`."""
+    _fields_ = [
+        ("requests", i32), ("tokens", i32), ("page_size", i32), ("max_pages", i32),
+        ("cached", vp), ("new_tokens", vp), ("free_pages", vp), ("free_count", vp), ("block_table", vp), ("starts", vp),
+        ("lengths", vp), ("positions", vp), ("slots", vp), ("used", vp), ("status", vp),
+    ]
+
+
+class PagedAttentionArgs(C.Structure):
+    """Mirror of `pk100_paged_attention_args`."""
+    _fields_ = [
+        ("type", i32), ("tokens", i32), ("requests", i32), ("heads", i32), ("kv_heads", i32), ("head_dim", i32), ("pages", i32),
+        ("page_size", i32), ("max_pages", i32),
+        ("query", vp), ("ld_query", i64), ("key", vp), ("ld_key", i64), ("value", vp), ("ld_value", i64), ("slots", vp),
+        ("key_cache", vp), ("value_cache", vp), ("page_stride", i64), ("token_stride", i64), ("head_stride", i64),
+        ("starts", vp), ("lengths", vp), ("block_table", vp), ("causal", i32), ("window", i32), ("max_new", i32), ("scale", f32),
+        ("out", vp), ("ld_out", i64), ("lse", vp), ("workspace", vp), ("workspace_bytes", i64), ("status", vp),
+    ]
+
+
 # name -> argument types (every function returns int)
 SIGNATURES = {
     "pk100_gemm": [vp, C.POINTER(GemmArgs)],
@@ -96,6 +126,11 @@ SIGNATURES = {
     "pk100_subsampling_fp8_workspace_bytes": None,
     "pk100_run_subsampling_fp8": None,
     "pk100_launch_count": None,
+    "pk100_add_rms_norm": [vp, C.POINTER(RmsNormArgs)],
+    "pk100_gemv_w4g128": [vp, C.POINTER(GemmArgs)],
+    "pk100_paged_plan": [vp, C.POINTER(PagedPlanArgs)],
+    "pk100_paged_attention": [vp, C.POINTER(PagedAttentionArgs)],
+    "pk100_paged_attention_workspace_bytes": [C.POINTER(PagedAttentionArgs)],
 }
 
 for _name, _argtypes in SIGNATURES.items():
@@ -105,6 +140,7 @@ for _name, _argtypes in SIGNATURES.items():
     _fn.restype = i32
 lib.pk100_launch_count.restype = i64
 lib.pk100_launch_count.argtypes = []
+lib.pk100_paged_attention_workspace_bytes.restype = i64
 lib.pk100_set_gemm_cta_pairs.restype = None
 lib.pk100_set_gemm_cta_pairs.argtypes = [i32]
 lib.pk100_set_gemm_cta_cap.restype = None
@@ -128,6 +164,9 @@ ACT_NONE, ACT_SILU, ACT_RELU = 0, 1, 2
 EPI_LINEAR, EPI_GLU, EPI_SPARSE_OUT = 0, 1, 2
 LN_F16, LN_E4M3_FIXED, LN_E4M3_ROW, LN_S8_ROW, LN_S4_ROW = 0, 1, 2, 3, 4
 PACK_E4M3, PACK_S8, PACK_S4_ROW, PACK_S4_G128 = 0, 1, 2, 3
+TYPE_F16, TYPE_BF16 = 0, 1
+STATUS_PLAN, STATUS_PAGE = 16, 32
+PLAN_MAX_REQUESTS = 4096
 
 
 class Pk100Error(RuntimeError):

@@ -5,7 +5,10 @@ inside libpk100.so.  Tensors must be CUDA and contiguous where stated.
 """
 from __future__ import annotations
 
+import functools
+import math
 import struct
+from collections import namedtuple
 
 import torch
 
@@ -16,10 +19,19 @@ EPS = 1e-5
 
 # The arguments of a GEMM as bytes (native sizes and alignment): filling the structure field by field took half of
 # the host time of a launch.
-_GEMM_ARGS = struct.Struct("@" + "".join({L.i32: "i", L.f32: "f", L.vp: "P"}[t] for _, t in L.GemmArgs._fields_) + "0P")
-assert _GEMM_ARGS.size == L.C.sizeof(L.GemmArgs)
-_gemm = L.lib["pk100_gemm"]                      # (a function object of its own, with bytes as its argument)
-_gemm.argtypes, _gemm.restype = [L.vp, L.C.c_char_p], L.i32
+def _packer(args):
+    packer = struct.Struct("@" + "".join({L.i32: "i", L.f32: "f", L.vp: "P", L.i64: "q"}[t] for _, t in args._fields_) + "0P")
+    assert packer.size == L.C.sizeof(args)
+    return packer
+
+
+def _taking_bytes(name):
+    function = L.lib[name]                       # (a function object of its own, with bytes as its argument)
+    function.argtypes, function.restype = [L.vp, L.C.c_char_p], L.i32
+    return function
+
+
+_GEMM_ARGS, _gemm = _packer(L.GemmArgs), _taking_bytes("pk100_gemm")
 
 
 def _ptr(t):
@@ -252,4 +264,209 @@ def local_attention_simple(q, k, v, pos, bias_u, bias_v, seg_stride=None, valid_
 def pack_position_heads(p):
     out = torch.empty((8, 272, 128), device=p.device, dtype=torch.float16)
     L.check(L.lib.pk100_pack_position_heads(_stream(), _ptr(p), _ptr(out)), "pk100_pack_position_heads")
+    return out
+
+
+# ---- operators of a language-model layer in serving
+_RMS_NORM_ARGS, _add_rms_norm = _packer(L.RmsNormArgs), _taking_bytes("pk100_add_rms_norm")
+_PAGED_PLAN_ARGS, _paged_plan = _packer(L.PagedPlanArgs), _taking_bytes("pk100_paged_plan")
+_PAGED_ATTENTION_ARGS, _paged_attention = _packer(L.PagedAttentionArgs), _taking_bytes("pk100_paged_attention")
+_gemv_w4g128 = _taking_bytes("pk100_gemv_w4g128")
+_TYPES = {torch.float16: L.TYPE_F16, torch.bfloat16: L.TYPE_BF16}
+
+
+def _type(t):
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"expected torch.float16 or torch.bfloat16, got {t.dtype}")
+    return code
+
+
+def _here(*tensors):
+    """The operators launch on the current device's stream: what they are given has to lie there."""
+    device = torch.cuda.current_device() if tensors[0].is_cuda else -1
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != device):
+            raise L.Pk100Error("libpk100 operates on tensors of the current CUDA device only (there is no CPU path)")
+
+
+def _shaped(name, t, shape, dtype, inner=1):
+    """t has this shape and type; its last `inner` dimensions lie one behind the other."""
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    step = 1
+    for d in range(1, inner + 1):
+        if t.shape[-d] > 1 and t.stride(-d) != step and t.numel() > 0:
+            raise ValueError(f"{name}: the last {inner} dimension(s) have to be contiguous")
+        step *= t.shape[-d]
+    return t
+
+
+def _distance(t):
+    """Elements between the rows (a single row's stride may be anything)."""
+    return 0 if t is None else t.stride(0) if t.shape[0] > 1 else t[0].numel() if t.shape[0] else 0
+
+
+def _out_dtype(mode, dtype):
+    return {L.LN_F16: dtype, L.LN_E4M3_FIXED: torch.uint8, L.LN_E4M3_ROW: torch.uint8, L.LN_S8_ROW: torch.int8}[mode]
+
+
+def add_rms_norm(x, gamma, residual=None, mode=L.LN_F16, inv_scale=0.0, eps=EPS, out=None, residual_out=None, scales=None):
+    """(out, scales, s): s = x + residual, out = the RMS norm of s in `mode`; see `pk100_add_rms_norm`.
+
+    x, residual [rows, width] fp16 or bf16, rows any distance apart.  s is kept in residual_out (one of the inputs, or
+    a new tensor when a residual is given) and is x itself without a residual.  scales is None for the modes without them."""
+    kind = _type(x)
+    if x.dim() != 2:
+        raise ValueError(f"x: expected [rows, width], got {tuple(x.shape)}")
+    rows, width = x.shape
+    if mode not in (L.LN_F16, L.LN_E4M3_FIXED, L.LN_E4M3_ROW, L.LN_S8_ROW):
+        raise ValueError(f"add_rms_norm has no output mode {mode}")
+    row_scales = mode in (L.LN_E4M3_ROW, L.LN_S8_ROW)
+    if out is None:
+        out = torch.empty((rows, width), device=x.device, dtype=_out_dtype(mode, x.dtype))
+    if residual_out is None and residual is not None:
+        residual_out = torch.empty((rows, width), device=x.device, dtype=x.dtype)
+    if scales is None and row_scales:
+        scales = torch.empty(rows, device=x.device, dtype=torch.float32)
+    _here(x, gamma, residual, out, residual_out, scales)
+    _shaped("x", x, x.shape, x.dtype)
+    _shaped("gamma", gamma, (width,), x.dtype)
+    _shaped("out", out, x.shape, _out_dtype(mode, x.dtype))
+    if residual is not None:
+        _shaped("residual", residual, x.shape, x.dtype)
+    if residual_out is not None:
+        _shaped("residual_out", residual_out, x.shape, x.dtype)
+    if row_scales:
+        _shaped("scales", scales, (rows,), torch.float32)
+    args = _RMS_NORM_ARGS.pack(
+        kind, mode, rows, width, x.data_ptr(), x.stride(0), _ptr(residual), 0 if residual is None else residual.stride(0),
+        _ptr(residual_out), 0 if residual_out is None else residual_out.stride(0), gamma.data_ptr(), eps, inv_scale,
+        out.data_ptr(), out.stride(0), _ptr(scales) if row_scales else 0)
+    L.check(_add_rms_norm(_stream(), args), "pk100_add_rms_norm")
+    return out, scales if row_scales else None, x if residual_out is None else residual_out
+
+
+def gemv_w4g128(a, codes, group_scales, *, out=None, row_scales=None, row_scale=1.0, col_scales=None, bias=None, act=L.ACT_NONE,
+                residual=None, alpha=1.0, valid_rows=0, out_type=L.OUT_F16):
+    """D = epilogue(A . W^T) for up to 16 rows, W from `pack_weight_rows(PACK_S4_G128)`; see `pk100_gemv_w4g128`."""
+    m, k = a.shape
+    n = codes.shape[0]
+    dtype = torch.float32 if out_type == L.OUT_F32 else torch.float16
+    if out is None:
+        out = torch.empty((m, n), device=a.device, dtype=dtype)
+    _here(a, codes, group_scales, out, row_scales, col_scales, bias, residual)
+    _shaped("a", a, (m, k), torch.float16)
+    _shaped("codes", codes, (n, k // 2), torch.uint8, 2)
+    _shaped("group_scales", group_scales, (k // 128, n), torch.float16, 2)
+    _shaped("out", out, (m, n), dtype)
+    for name, t, shape in (("row_scales", row_scales, (m,)), ("col_scales", col_scales, (n,)), ("bias", bias, (n,))):
+        if t is not None:
+            _shaped(name, t, shape, torch.float32)
+    if residual is not None:
+        _shaped("residual", residual, (m, n), torch.float16)
+    args = _GEMM_ARGS.pack(
+        L.KIND_F16_W4G128, L.EPI_LINEAR, m, n, k, a.data_ptr(), _distance(a), codes.data_ptr(), k // 2, _ptr(row_scales), row_scale,
+        _ptr(col_scales), _ptr(bias), act, _ptr(residual), _distance(residual), alpha, valid_rows,
+        out.data_ptr(), _distance(out), out_type, 1.0, 0.0, 0, 0, 0, 0, 0, group_scales.data_ptr())
+    L.check(_gemv_w4g128(_stream(), args), "pk100_gemv_w4g128")
+    return out
+
+
+PagedPlan = namedtuple("PagedPlan", "starts lengths positions slots used")
+
+
+def paged_plan(cached, new_tokens, block_table, free_pages, free_count, *, tokens, page_size, status=None, out=None):
+    """One step's bookkeeping of a paged cache; see `pk100_paged_plan`.
+
+    cached, new_tokens [requests], block_table [requests, max_pages] (its new pages are written), free_pages [any],
+    free_count [1], all int32.  `tokens` rows of positions (int32) and slots (int64) are returned in a PagedPlan with
+    starts [requests + 1], lengths [requests] and used [1]; `out`: such a tuple to write to."""
+    requests, max_pages = block_table.shape
+    if out is None:
+        new = functools.partial(torch.empty, device=block_table.device)
+        words = new(2 * requests + 2 + tokens, dtype=torch.int32)
+        out = PagedPlan(*words[:2 * requests + 1].split([requests + 1, requests]), words[2 * requests + 1:-1],
+                        new(tokens, dtype=torch.int64), words[-1:])
+    _here(block_table, cached, new_tokens, free_pages, free_count, status, *out)
+    i32 = torch.int32
+    _shaped("block_table", block_table, (requests, max_pages), i32, 2)
+    for name, t, shape, dtype in (("cached", cached, (requests,), i32), ("new_tokens", new_tokens, (requests,), i32),
+                                  ("free_pages", free_pages, (free_pages.numel(),), i32), ("free_count", free_count, (1,), i32),
+                                  ("starts", out.starts, (requests + 1,), i32), ("lengths", out.lengths, (requests,), i32),
+                                  ("positions", out.positions, (tokens,), i32), ("slots", out.slots, (tokens,), torch.int64),
+                                  ("used", out.used, (1,), i32)):
+        _shaped(name, t, shape, dtype)
+    args = _PAGED_PLAN_ARGS.pack(
+        requests, tokens, page_size, max_pages, cached.data_ptr(), new_tokens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
+        block_table.data_ptr(), out.starts.data_ptr(), out.lengths.data_ptr(), out.positions.data_ptr(), out.slots.data_ptr(),
+        out.used.data_ptr(), _ptr(status))
+    L.check(_paged_plan(_stream(), args), "pk100_paged_plan")
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_workspace(device, tokens, requests, heads, kv_heads, head_dim, page_size, max_pages, pages):
+    args = L.PagedAttentionArgs(tokens=tokens, requests=requests, heads=heads, kv_heads=kv_heads, head_dim=head_dim, pages=pages,
+                                page_size=page_size, max_pages=max_pages)
+    return L.lib.pk100_paged_attention_workspace_bytes(args)
+
+
+def paged_attention_workspace(query, key_cache, block_table):
+    """Bytes that `paged_attention` needs for these tensors on the current device."""
+    return _paged_workspace(torch.cuda.current_device(), query.shape[0], block_table.shape[0], query.shape[1], key_cache.shape[2],
+                            query.shape[2], key_cache.shape[1], block_table.shape[1], key_cache.shape[0])
+
+
+def paged_attention(query, key_cache, value_cache, block_table, starts, lengths, *, key=None, value=None, slots=None, causal=True,
+                    window=0, scale=None, max_new=0, out=None, lse=None, workspace=None, status=None):
+    """Attention of new tokens over a paged cache; see `pk100_paged_attention`.
+
+    query [tokens, heads, head_dim] fp16 or bf16 (tokens any distance apart), caches [pages, page_size, kv_heads, head_dim]
+    with any strides of the first three dimensions (the same ones in both), block_table [requests, max_pages], starts
+    [requests + 1] and lengths [requests] int32.  key, value [tokens, kv_heads, head_dim] with slots [tokens] int64 are
+    written to the cache first.  scale: 1 / sqrt(head_dim) by default.  workspace (uint8): allocated for the call where
+    it is not given; one that is given is not used by another call at the same time."""
+    kind, dtype = _type(query), query.dtype
+    tokens, heads, head_dim = query.shape
+    pages, page_size, kv_heads, _ = key_cache.shape
+    requests, max_pages = block_table.shape
+    if out is None:
+        out = torch.empty((tokens, heads, head_dim), device=query.device, dtype=dtype)
+    _here(query, key_cache, value_cache, block_table, starts, lengths, key, value, slots, out, lse, workspace, status)
+    _shaped("query", query, (tokens, heads, head_dim), dtype, 2)
+    _shaped("out", out, (tokens, heads, head_dim), dtype, 2)
+    _shaped("key_cache", key_cache, (pages, page_size, kv_heads, head_dim), dtype)
+    _shaped("value_cache", value_cache, (pages, page_size, kv_heads, head_dim), dtype)
+    if key_cache.stride() != value_cache.stride():
+        raise ValueError("key_cache and value_cache have to have the same strides")
+    _shaped("block_table", block_table, (requests, max_pages), torch.int32, 2)
+    _shaped("starts", starts, (requests + 1,), torch.int32)
+    _shaped("lengths", lengths, (requests,), torch.int32)
+    if key is not None:
+        if value is None or slots is None:
+            raise ValueError("key needs value and slots")
+        _shaped("key", key, (tokens, kv_heads, head_dim), dtype, 2)
+        _shaped("value", value, (tokens, kv_heads, head_dim), dtype, 2)
+        _shaped("slots", slots, (tokens,), torch.int64)
+    if lse is not None:
+        _shaped("lse", lse, (tokens, heads), torch.float32, 2)
+    if heads % kv_heads:
+        raise ValueError(f"{heads} query heads do not share {kv_heads} key-value heads evenly")
+    if workspace is None:
+        need = paged_attention_workspace(query, key_cache, block_table)
+        workspace = torch.empty(need, device=query.device, dtype=torch.uint8)
+    else:
+        _shaped("workspace", workspace, workspace.shape, torch.uint8, workspace.dim())
+    page_stride, token_stride, head_stride, _ = key_cache.stride()
+    args = _PAGED_ATTENTION_ARGS.pack(
+        kind, tokens, requests, heads, kv_heads, head_dim, pages, page_size, max_pages, query.data_ptr(), query.stride(0),
+        _ptr(key), 0 if key is None else key.stride(0), 0 if key is None else value.data_ptr(), 0 if key is None else value.stride(0),
+        0 if key is None else slots.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), page_stride, token_stride, head_stride,
+        starts.data_ptr(), lengths.data_ptr(), block_table.data_ptr(), int(causal), min(window, 1 << 30), min(max_new, 1 << 30),
+        1.0 / math.sqrt(head_dim) if scale is None else scale, out.data_ptr(), out.stride(0), _ptr(lse), workspace.data_ptr(),
+        workspace.numel(), _ptr(status))
+    L.check(_paged_attention(_stream(), args), "pk100_paged_attention")
     return out
