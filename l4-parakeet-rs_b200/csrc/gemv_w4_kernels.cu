@@ -2,13 +2,15 @@
 // m <= 16.
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "pk100_internal.h"
 #include "ptx_sm100.cuh"
 
 namespace pk100 {
 
 constexpr int kGroup = 128;
-constexpr int kGemvWarps = 8, kGemvThreads = kGemvWarps * 32;
+constexpr int kGemvWarps = 12, kGemvThreads = kGemvWarps * 32;
 
 struct GemvParams {
     int m, n, k;
@@ -32,151 +34,224 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 
 // D (16 x 8, fp32) += A (16 x 16) . B (16 x 8), fp16
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// 8 codes of a word -> 4 pairs of weights f16(code * scale), pair i = codes (i, i + 4).  A code with its sign bit
-// flipped is code + 8; behind the exponent of 1024 it is 1024 + code + 8, exactly.
-__device__ __forceinline__ void weights_of(uint32_t word, __half2 scale, uint32_t (&w)[4]) {
-    const uint32_t flipped = word ^ 0x88888888u;
-    const __half2 zero = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));       // 1032
+// 8 codes of a word -> 4 pairs of weights f16(code * scale), pair i = codes (i, i + 4).  With its sign bit flipped a code
+// is code + 8; in the low mantissa bits behind the exponent of 1024 it is 1024 + code + 8, four bits higher 1024 +
+// 16 (code + 8), and one subtraction or multiply-add gives the code, exactly.
+struct CodeMasks {
+    uint32_t low, low_magic, high, high_magic;
+    // (unknown to the compiler, which would otherwise split (a & low) ^ magic into two instructions with a constant each)
+    __device__ __forceinline__ CodeMasks() {
+        asm volatile("mov.b32 %0, 0x000f000f;\n\tmov.b32 %1, 0x64086408;\n\tmov.b32 %2, 0x00f000f0;\n\tmov.b32 %3, 0x64806480;"
+                     : "=r"(low), "=r"(low_magic), "=r"(high), "=r"(high_magic));
+    }
+};
+__device__ __forceinline__ __half2 and_xor(uint32_t a, uint32_t mask, uint32_t magic) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(a), "r"(mask), "r"(magic));
+    return *reinterpret_cast<const __half2*>(&r);
+}
+__device__ __forceinline__ void weights_of(uint32_t word, __half2 scale, const CodeMasks& m, uint32_t (&w)[4]) {
+    const __half2 low = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));        // 1032
+    const __half2 shift = __halves2half2(__ushort_as_half(0x2c00), __ushort_as_half(0x2c00));      // 1 / 16
+    const __half2 high = __halves2half2(__ushort_as_half(0xd480), __ushort_as_half(0xd480));       // -72
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t bits = ((flipped >> (4 * i)) & 0x000f000fu) | 0x64006400u;
-        const __half2 v = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&bits), zero), scale);
-        w[i] = *reinterpret_cast<const uint32_t*>(&v);
+    for (int i = 0; i < 4; i += 2) {
+        const uint32_t bits = word >> (4 * i);
+        const __half2 even = __hmul2(__hsub2(and_xor(bits, m.low, m.low_magic), low), scale);
+        const __half2 odd = __hmul2(__hfma2(and_xor(bits, m.high, m.high_magic), shift, high), scale);
+        w[i] = *reinterpret_cast<const uint32_t*>(&even);
+        w[i + 1] = *reinterpret_cast<const uint32_t*>(&odd);
     }
 }
 
-template <int RowTiles, int Tiles, int Stages>
+constexpr int kGemvTiles = 4;         // 16-row tiles of weights that a block takes at a time
+
+template <int RowTiles>
 struct GemvSmem {
-    uint4 ring[Stages][2 * Tiles][kGemvThreads];                       // codes, each piece private to its thread
-    float sums[kGemvWarps][16 * Tiles][8 * RowTiles + 1];
+    static constexpr int kStages = 3;
+    uint4 ring[kStages][2 * kGemvTiles][kGemvThreads];                 // codes, each piece private to its thread
+    float sums[kGemvWarps][16 * kGemvTiles][8 * RowTiles + 1];
 };
 
 // The weights are the A operand of the tensor instruction (16 weight rows x 16 k), the activations its B operand (up
 // to 8 rows each), so a product of 1 to 8 rows costs one instruction per 256 codes and the time is that of reading
 // and converting the codes.  The k order inside a group is free: a thread takes 32 consecutive codes of a row (one
-// 16-byte load) and pairs them as the nibbles fall, and the activations follow it.  A block owns 16 * Tiles weight
-// rows; its warps take the groups in turn and their sums are joined in a fixed order.  Codes come by asynchronous
-// copies into a ring in which every thread reads what it has copied itself: no barrier in the loop.
-template <int RowTiles, int Tiles, int Stages>
-__global__ void __launch_bounds__(kGemvThreads)
+// 16-byte load) and pairs them as the nibbles fall, and the activations follow it.
+// One block an SM owns a contiguous share of the 16-row tiles and takes them in chunks of up to four, which share the
+// activations that they read; its warps take the groups in turn and their sums are joined in a fixed order.  Codes
+// come by asynchronous copies, up to 96 KB of them in flight, into a ring in which every thread reads what it has
+// copied itself: no barrier in the loop, and the next chunk is on its way while this one is joined.  Activations and
+// scales of the next group are requested a group ahead.
+// 13 x 8192 by 28672 rows (122 MB): 50.5 us, 2.4 TB/s; 76.8 us with a block per 64 rows, 8 warps and no requests ahead.
+// Bound by the conversion: per 64 x 128 codes a warp issues about 750 instructions, half of them on half-rate pipes.
+template <int RowTiles>
+__global__ void __launch_bounds__(kGemvThreads, 1)
 gemv_w4g128_kernel(const GemvParams p) {
     extern __shared__ uint8_t gemv_raw[];
-    using Smem = GemvSmem<RowTiles, Tiles, Stages>;
+    using Smem = GemvSmem<RowTiles>;
+    constexpr int kStages = Smem::kStages;
     Smem& sm = *reinterpret_cast<Smem*>(gemv_raw);
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, c = lane % 4;
-    const int n0 = blockIdx.x * 16 * Tiles, groups = p.k / kGroup;
+    const int groups = p.k / kGroup, all = (p.n + 15) / 16;
+    const int first = static_cast<int>(static_cast<long long>(all) * blockIdx.x / gridDim.x);
+    const int last = static_cast<int>(static_cast<long long>(all) * (blockIdx.x + 1) / gridDim.x);
+    // chunks of nearly equal size
+    const int chunks = (last - first + kGemvTiles - 1) / kGemvTiles;
+    auto chunk_at = [&](int chunk) { return first + (last - first) * chunk / chunks; };
     grid_dependents_launch();
     grid_dependency_wait();
 
-    // weight rows of this thread: g and g + 8 of every tile (those behind the last one repeat it and are not stored)
-    long long code_at[2 * Tiles];
-    int scale_at[2 * Tiles];
+    const CodeMasks masks;
+    // what the ring is filled with next: a group of a chunk, rows g + 8 i < limit of it
+    const long long row_step = 8ll * (p.k / 2);
+    int f_chunk = -1, f_group = groups, f_limit = 0;
+    const uint8_t* f_src = nullptr;
+    auto fetch = [&](int stage) {
+        if (f_group >= groups) {                                       // (a warp without groups fetches nothing)
+            f_chunk = warp < groups ? f_chunk + 1 : chunks;
+            f_group = warp;
+            if (f_chunk < chunks) {
+                const int row = chunk_at(f_chunk) * 16 + g;
+                f_limit = min(chunk_at(f_chunk + 1) * 16, p.n) - row;
+                f_src = p.codes + static_cast<long long>(row) * (p.k / 2) + warp * (kGroup / 2) + 16 * c;
+            }
+        }
+        if (f_chunk < chunks) {
+            const uint8_t* src = f_src;
 #pragma unroll
-    for (int i = 0; i < 2 * Tiles; ++i) {
-        const int n = min(n0 + (i / 2) * 16 + (i % 2) * 8 + g, p.n - 1);
-        code_at[i] = static_cast<long long>(n) * (p.k / 2) + 16 * c;
-        scale_at[i] = n;
-    }
-    auto fetch = [&](int group, int stage) {
-        if (group < groups) {
-#pragma unroll
-            for (int i = 0; i < 2 * Tiles; ++i) cp_async_16(&sm.ring[stage][i][tid], p.codes + code_at[i] + static_cast<long long>(group) * (kGroup / 2));
+            for (int i = 0; i < 2 * kGemvTiles; ++i, src += row_step)
+                if (8 * i < f_limit) cp_async_16(&sm.ring[stage][i][tid], src);      // (rows that are not there keep what the ring holds)
+            f_group += kGemvWarps;
+            f_src += kGemvWarps * (kGroup / 2);
         }
         cp_async_commit();
     };
 #pragma unroll
-    for (int s = 0; s < Stages - 1; ++s) fetch(warp + s * kGemvWarps, s);
-
-    float acc[Tiles][RowTiles][4];
-#pragma unroll
-    for (int i = 0; i < Tiles; ++i)
-#pragma unroll
-        for (int j = 0; j < RowTiles; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.0f;
+    for (int s = 0; s < kStages - 1; ++s) fetch(s);
 
     int stage = 0;
 #pragma unroll 1
-    for (int group = warp; group < groups; group += kGemvWarps) {
-        uint4 x[RowTiles][4];
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        const int at = chunk_at(chunk), tiles = chunk_at(chunk + 1) - at, limit = min((at + tiles) * 16, p.n) - (at * 16 + g);
+        float acc[kGemvTiles][RowTiles][4];
 #pragma unroll
-        for (int j = 0; j < RowTiles; ++j) {
-            const int m = 8 * j + g;
-            const uint4* src = reinterpret_cast<const uint4*>(p.a + m * p.lda + group * kGroup + 32 * c);
+        for (int i = 0; i < kGemvTiles; ++i)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[j][i] = m < p.m ? src[i] : make_uint4(0, 0, 0, 0);
-        }
-        __half2 scale[2 * Tiles];
+            for (int j = 0; j < RowTiles; ++j)
 #pragma unroll
-        for (int i = 0; i < 2 * Tiles; ++i)
-            scale[i] = __half2half2(p.group_scales[static_cast<long long>(group) * p.n + scale_at[i]]);
-        cp_async_wait<Stages - 2>();
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {                                  // words of 8 codes
-            uint32_t b[RowTiles][4];
-#pragma unroll
-            for (int j = 0; j < RowTiles; ++j) {
-                b[j][0] = __byte_perm(x[j][w].x, x[j][w].z, 0x5410);   // (0, 4)
-                b[j][1] = __byte_perm(x[j][w].x, x[j][w].z, 0x7632);   // (1, 5)
-                b[j][2] = __byte_perm(x[j][w].y, x[j][w].w, 0x5410);   // (2, 6)
-                b[j][3] = __byte_perm(x[j][w].y, x[j][w].w, 0x7632);   // (3, 7)
-            }
-#pragma unroll
-            for (int i = 0; i < Tiles; ++i) {
-                uint32_t lo[4], hi[4];                                 // rows g and g + 8
-                weights_of(reinterpret_cast<const uint32_t*>(&sm.ring[stage][2 * i][tid])[w], scale[2 * i], lo);
-                weights_of(reinterpret_cast<const uint32_t*>(&sm.ring[stage][2 * i + 1][tid])[w], scale[2 * i + 1], hi);
-                const uint32_t first[4] = {lo[0], hi[0], lo[1], hi[1]}, second[4] = {lo[2], hi[2], lo[3], hi[3]};
-#pragma unroll
-                for (int j = 0; j < RowTiles; ++j) {
-                    mma_16x8x16(acc[i][j], first, b[j][0], b[j][1]);
-                    mma_16x8x16(acc[i][j], second, b[j][2], b[j][3]);
-                }
-            }
-        }
-        const int next = stage == 0 ? Stages - 1 : stage - 1;          // the stage read a group ago
-        fetch(group + (Stages - 1) * kGemvWarps, next);
-        stage = stage + 1 == Stages ? 0 : stage + 1;
-    }
-    cp_async_wait<0>();
-
-#pragma unroll
-    for (int i = 0; i < Tiles; ++i)
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.0f;
+        uint4 x_next[RowTiles][4];
+        __half scale_next[2 * kGemvTiles];
 #pragma unroll
         for (int j = 0; j < RowTiles; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sm.sums[warp][16 * i + g + (e / 2) * 8][8 * j + 2 * c + e % 2] = acc[i][j][e];
-    __syncthreads();
-    for (int o = tid; o < 16 * Tiles * p.m; o += kGemvThreads) {
-        const int row = o % (16 * Tiles), m = o / (16 * Tiles), n = n0 + row;
-        if (n >= p.n) continue;
-        float v = 0.0f;
+            for (int i = 0; i < 4; ++i) x_next[j][i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int w = 0; w < kGemvWarps; ++w) v += sm.sums[w][row][m];
-        v *= p.row_scales != nullptr ? p.row_scales[m] : p.row_scale;
-        if (p.col_scales != nullptr) v *= p.col_scales[n];
-        if (p.bias != nullptr) v += p.bias[n];
-        if (p.act == PK100_ACT_SILU) v = v / (1.0f + __expf(-v));
-        else if (p.act == PK100_ACT_RELU) v = fmaxf(v, 0.0f);
-        v = p.residual != nullptr ? fmaf(p.alpha, v, __half2float(p.residual[m * p.ld_res + n])) : p.alpha * v;
-        if (m >= p.valid_rows) v = 0.0f;
-        if (p.out_type == PK100_OUT_F16) static_cast<__half*>(p.out)[m * p.ld_out + n] = __float2half_rn(v);
-        else static_cast<float*>(p.out)[m * p.ld_out + n] = v;
+        for (int i = 0; i < 2 * kGemvTiles; ++i) scale_next[i] = __half();
+        const __half* x_src = p.a + g * p.lda + warp * kGroup + 32 * c;
+        const __half* scale_src = p.group_scales + static_cast<long long>(warp) * p.n + at * 16 + g;
+        auto request = [&](int group) {                                // activations and scales, a group ahead
+            if (group >= groups) return;
+#pragma unroll
+            for (int j = 0; j < RowTiles; ++j)
+                if (8 * j + g < p.m) {
+                    const uint4* src = reinterpret_cast<const uint4*>(x_src + 8 * j * p.lda);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x_next[j][i] = __ldg(src + i);
+                }
+#pragma unroll
+            for (int i = 0; i < 2 * kGemvTiles; ++i)
+                if (8 * i < limit) scale_next[i] = __ldg(scale_src + 8 * i);
+            x_src += kGemvWarps * kGroup;
+            scale_src += static_cast<long long>(kGemvWarps) * p.n;
+        };
+        request(warp);
+        uint32_t x[RowTiles][4][4];
+        __half scale[2 * kGemvTiles];
+        auto products = [&](auto count) {
+#pragma unroll
+            for (int i = 0; i < decltype(count)::value; ++i) {
+                const uint4 lo_codes = sm.ring[stage][2 * i][tid], hi_codes = sm.ring[stage][2 * i + 1][tid];    // rows g and g + 8
+                const uint32_t lo_words[4] = {lo_codes.x, lo_codes.y, lo_codes.z, lo_codes.w}, hi_words[4] = {hi_codes.x, hi_codes.y, hi_codes.z, hi_codes.w};
+                const __half2 lo_scale = __half2half2(scale[2 * i]), hi_scale = __half2half2(scale[2 * i + 1]);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t lo[4], hi[4];
+                    weights_of(lo_words[w], lo_scale, masks, lo);
+                    weights_of(hi_words[w], hi_scale, masks, hi);
+                    const uint32_t near[4] = {lo[0], hi[0], lo[1], hi[1]}, far[4] = {lo[2], hi[2], lo[3], hi[3]};
+#pragma unroll
+                    for (int j = 0; j < RowTiles; ++j) mma_16x8x16(acc[i][j], near, x[j][w][0], x[j][w][1]);
+#pragma unroll
+                    for (int j = 0; j < RowTiles; ++j) mma_16x8x16(acc[i][j], far, x[j][w][2], x[j][w][3]);
+                }
+            }
+        };
+#pragma unroll 1
+        for (int group = warp; group < groups; group += kGemvWarps) {
+#pragma unroll
+            for (int j = 0; j < RowTiles; ++j)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {                          // pairs (0, 4), (1, 5), (2, 6), (3, 7)
+                    x[j][w][0] = __byte_perm(x_next[j][w].x, x_next[j][w].z, 0x5410);
+                    x[j][w][1] = __byte_perm(x_next[j][w].x, x_next[j][w].z, 0x7632);
+                    x[j][w][2] = __byte_perm(x_next[j][w].y, x_next[j][w].w, 0x5410);
+                    x[j][w][3] = __byte_perm(x_next[j][w].y, x_next[j][w].w, 0x7632);
+                }
+#pragma unroll
+            for (int i = 0; i < 2 * kGemvTiles; ++i) scale[i] = scale_next[i];
+            request(group + kGemvWarps);
+            cp_async_wait<kStages - 2>();
+            // (straight code for each count, so that the conversions of one tile fill the waits of another's products)
+            if (tiles == 4) products(std::integral_constant<int, 4>());
+            else if (tiles == 3) products(std::integral_constant<int, 3>());
+            else if (tiles == 2) products(std::integral_constant<int, 2>());
+            else products(std::integral_constant<int, 1>());
+            fetch(stage == 0 ? kStages - 1 : stage - 1);               // the stage read a group ago
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+        }
+
+        if (chunk > 0) __syncthreads();                                // the sums of the chunk before have been read
+#pragma unroll
+        for (int i = 0; i < kGemvTiles; ++i)
+#pragma unroll
+            for (int j = 0; j < RowTiles; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sm.sums[warp][16 * i + g + (e / 2) * 8][8 * j + 2 * c + e % 2] = acc[i][j][e];
+        __syncthreads();
+        for (int o = tid; o < 16 * kGemvTiles * p.m; o += kGemvThreads) {
+            const int row = o % (16 * kGemvTiles), m = o / (16 * kGemvTiles), n = at * 16 + row;
+            if (row >= 16 * tiles || n >= p.n) continue;
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kGemvWarps; ++w) v += sm.sums[w][row][m];
+            v *= p.row_scales != nullptr ? p.row_scales[m] : p.row_scale;
+            if (p.col_scales != nullptr) v *= p.col_scales[n];
+            if (p.bias != nullptr) v += p.bias[n];
+            if (p.act == PK100_ACT_SILU) v = v / (1.0f + __expf(-v));
+            else if (p.act == PK100_ACT_RELU) v = fmaxf(v, 0.0f);
+            v = p.residual != nullptr ? fmaf(p.alpha, v, __half2float(p.residual[m * p.ld_res + n])) : p.alpha * v;
+            if (m >= p.valid_rows) v = 0.0f;
+            if (p.out_type == PK100_OUT_F16) static_cast<__half*>(p.out)[m * p.ld_out + n] = __float2half_rn(v);
+            else static_cast<float*>(p.out)[m * p.ld_out + n] = v;
+        }
     }
+    cp_async_wait<0>();
 }
 
-template <int RowTiles, int Tiles, int Stages>
+template <int RowTiles>
 static int launch_gemv(const GemvParams& p, cudaStream_t stream) {
-    constexpr auto kernel = gemv_w4g128_kernel<RowTiles, Tiles, Stages>;
-    constexpr int bytes = sizeof(GemvSmem<RowTiles, Tiles, Stages>);
+    constexpr auto kernel = gemv_w4g128_kernel<RowTiles>;
+    constexpr int bytes = sizeof(GemvSmem<RowTiles>);
     const cudaError_t granted = pk100_grant_smem<kernel>(bytes);
     if (granted != cudaSuccess) return static_cast<int>(granted);
-    pk100_launch_chained(kernel, dim3((p.n + 16 * Tiles - 1) / (16 * Tiles)), dim3(kGemvThreads), bytes, stream, p);
+    const int tiles = (p.n + 15) / 16, sms = pk100_cta_budget();
+    pk100_launch_chained(kernel, dim3(tiles < sms ? tiles : sms), dim3(kGemvThreads), bytes, stream, p);
     return pk100_launch_status();
 }
 
@@ -210,8 +285,5 @@ extern "C" int pk100_gemv_w4g128(void* stream_v, const pk100_gemm_args* a) {
     p.alpha = a->alpha; p.valid_rows = a->valid_rows <= 0 ? a->m : a->valid_rows;
     p.out = a->out; p.ld_out = a->ld_out; p.out_type = a->out_type;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-    // 64 weight rows a block share the activations that they read; 16 where that leaves SMs without a block
-    const bool wide = a->n >= 64 * pk100_sm_count();
-    if (a->m <= 8) return wide ? launch_gemv<1, 4, 4>(p, stream) : launch_gemv<1, 1, 6>(p, stream);
-    return wide ? launch_gemv<2, 4, 4>(p, stream) : launch_gemv<2, 1, 6>(p, stream);
+    return a->m <= 8 ? launch_gemv<1>(p, stream) : launch_gemv<2>(p, stream);
 }
