@@ -523,7 +523,8 @@ static int cache_map(CUtensorMap* map, const void* base, const pk100_paged_atten
 // Where the workspace's arrays lie.
 struct PagedPlan {
     int grid;                                            // blocks of the few-row kernel
-    long long begins, parts, part_out, bytes;
+    int pairs, shares;                                   // of the other one
+    long long begins, parts, part_out, share_ml, share_out, bytes;
 };
 
 static long long round256(long long n) { return (n + 255) / 256 * 256; }
@@ -539,7 +540,17 @@ static PagedPlan paged_plan_of(const pk100_paged_attention_args& a) {
     plan.begins = 0;
     plan.parts = round256(plan.grid * static_cast<long long>(sizeof(RowsBegin)));
     plan.part_out = plan.parts + round256(2ll * plan.grid * static_cast<long long>(sizeof(RowsPart)));
-    plan.bytes = plan.part_out + 2ll * plan.grid * kRows * a.head_dim * 4;
+    plan.share_ml = plan.part_out + round256(2ll * plan.grid * kRows * a.head_dim * 4);
+    // Keys are shared out where the pairs of tiles leave SMs idle: few new tokens over a long cache.
+    const long long rows = static_cast<long long>(a.tokens) * group, items = (rows + kPairRows - 1) / kPairRows * a.kv_heads;
+    plan.pairs = static_cast<int>(rows / kPairRows) + a.requests;
+    const long long by_keys = blocks / 8;                // 512 keys a share at least
+    long long shares = items > 0 ? pk100_sm_count() / items : 1;
+    if (shares > by_keys) shares = by_keys;
+    plan.shares = shares < 1 ? 1 : static_cast<int>(shares);
+    const long long share_rows = plan.shares > 1 ? static_cast<long long>(plan.shares) * a.tokens * a.heads : 0;
+    plan.share_out = plan.share_ml + round256(share_rows * 8);
+    plan.bytes = plan.share_out + round256(share_rows * a.head_dim * 4);
     return plan;
 }
 
@@ -617,8 +628,12 @@ extern "C" int pk100_paged_attention(void* stream_v, const pk100_paged_attention
     p.causal = a->causal != 0;
     p.window = a->window <= 0 ? 0 : (a->window < (1 << 30) ? a->window : (1 << 30));
     p.scale_log2 = a->scale * 1.4426950408889634f;
-    p.few_rows = 0x7fffffff;
+    p.few_rows = kRows;
     p.status = a->status;
+    // Where no request has more rows than the few-row kernel takes, it takes them all; the hint may be wrong, so it does then, too.
+    const int most_new = a->max_new > 0 && a->max_new < a->tokens ? a->max_new : a->tokens;
+    const bool many = static_cast<long long>(most_new) * p.group > kRows;
+    if (!many) p.few_rows = 0x7fffffff;
     if (a->key != nullptr) {
         AppendParams w{};
         w.key = static_cast<const uint16_t*>(a->key); w.value = static_cast<const uint16_t*>(a->value);
@@ -633,6 +648,12 @@ extern "C" int pk100_paged_attention(void* stream_v, const pk100_paged_attention
         if ((rc = pk100_launch_status()) != PK100_OK) return rc;
     }
     if (a->type == PK100_TYPE_F16)
-        return a->head_dim == 128 ? launch_rows<__half, 128>(*a, p, plan, map_k, map_v, stream) : launch_rows<__half, 64>(*a, p, plan, map_k, map_v, stream);
-    return a->head_dim == 128 ? launch_rows<__nv_bfloat16, 128>(*a, p, plan, map_k, map_v, stream) : launch_rows<__nv_bfloat16, 64>(*a, p, plan, map_k, map_v, stream);
+        rc = a->head_dim == 128 ? launch_rows<__half, 128>(*a, p, plan, map_k, map_v, stream) : launch_rows<__half, 64>(*a, p, plan, map_k, map_v, stream);
+    else
+        rc = a->head_dim == 128 ? launch_rows<__nv_bfloat16, 128>(*a, p, plan, map_k, map_v, stream)
+                                : launch_rows<__nv_bfloat16, 64>(*a, p, plan, map_k, map_v, stream);
+    if (rc != PK100_OK || !many) return rc;
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    return paged_attention_chunks(a->type, a->head_dim, p, map_k, map_v, plan.pairs, plan.shares, reinterpret_cast<float2*>(ws + plan.share_ml),
+                                  reinterpret_cast<float*>(ws + plan.share_out), stream);
 }

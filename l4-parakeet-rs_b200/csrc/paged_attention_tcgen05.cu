@@ -1,0 +1,484 @@
+// Attention of many new tokens over a paged key-value cache on the tcgen05 tensor cores.
+#include "paged_attention.cuh"
+
+namespace pk100 {
+namespace chunk {
+
+constexpr int kTile = 128;                      // (token, head) rows of an accumulator, and keys of a block
+constexpr int kTiles = 2;                       // tiles of a block of threads: one's softmax runs under the other's products
+constexpr int kSoftmaxWarps = 4 * kTiles;
+constexpr int kThreads = kSoftmaxWarps * 32 + 64;
+constexpr int kAtom = kTile * 128;              // 128 rows x 64 elements, 128-byte swizzle
+constexpr int kBox = 64;                        // most keys of a TMA box
+
+template <int D> constexpr int ring_slots() { return D == 128 ? 5 : 8; }
+
+template <int D>
+struct Smem {
+    uint8_t q[kTiles][D / 64][kAtom];
+    uint8_t ring[ring_slots<D>()][D / 64][kAtom];          // key and value blocks in turn
+    uint64_t full[ring_slots<D>()], empty[ring_slots<D>()];
+    uint64_t q_ready, s_full[kTiles], p_full[kTiles], o_done[kTiles];
+    uint32_t tmem;
+    int abort;
+};
+
+template <typename T> __host__ __device__ constexpr uint32_t type_bits() { return 0; }                                    // kind::f16 operands: fp16
+template <> __host__ __device__ constexpr uint32_t type_bits<__nv_bfloat16>() { return (1u << 7) | (1u << 10); }
+
+// D[tmem] (+)= A[tmem] * B[smem], 16 k, issued where `leader` is set
+__device__ __forceinline__ void mma_from_tmem(bool leader, uint32_t d, uint32_t a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+                 ::"r"(d), "r"(a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(static_cast<uint32_t>(leader)) : "memory");
+}
+
+// What a block of threads works on: 256 rows of one request and key-value head, over a share of their keys.
+struct Work {
+    PagedRequest at;
+    int request, head, row, rows;               // first row of the first tile inside the request; rows of both tiles that exist
+    int lo, hi;                                 // keys that any of the rows sees
+    int from, to;                               // key blocks of this share
+    __device__ __forceinline__ Work(const PagedParams& p, int request_, int head_, int pair) : at(p, request_), request(request_), head(head_) {
+        row = pair * kTiles * kTile;
+        rows = min(at.n * p.group - row, kTiles * kTile);
+        const int first = row / p.group, last = (row + max(rows, 1) - 1) / p.group;
+        lo = at.lo(p, first);
+        hi = at.hi(p, last);
+        from = lo / kTile;
+        to = max((hi + kTile - 1) / kTile, from);
+    }
+    // key blocks of this share that a row of tile t sees
+    __device__ __forceinline__ int tile_from(const PagedParams& p, int t) const {
+        return max(from, at.lo(p, (row + t * kTile) / p.group) / kTile);
+    }
+    __device__ __forceinline__ int tile_to(const PagedParams& p, int t) const {
+        const int left = min(rows - t * kTile, kTile);
+        if (left <= 0) return tile_from(p, t);
+        return max(tile_from(p, t), min(to, (at.hi(p, (row + t * kTile + left - 1) / p.group) + kTile - 1) / kTile));
+    }
+};
+
+// Pairs of tiles are numbered over the batch with gaps: request r begins at floor(first row / 256) + r, which leaves
+// room for its last, partial pair.  The last request that begins at or before `pair`, found 32 candidates at a time.
+__device__ __forceinline__ int request_of(const PagedParams& p, int pair, int& begin) {
+    const int lane = threadIdx.x % 32;
+    int lo = 0, hi = p.requests;                 // begin(lo) <= pair < begin(hi)
+    int begin_lo = 0;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, r = lo + lane * step;
+        long long b = 0x7fffffffll;
+        if (r < hi) b = static_cast<long long>(max(p.starts[r], 0)) * p.group / (kTiles * kTile) + r;
+        const uint32_t before = __ballot_sync(0xffffffffu, b <= pair);
+        const int last = before == 0 ? 0 : 31 - __clz(before);
+        begin_lo = static_cast<int>(__shfl_sync(0xffffffffu, b, last));
+        lo = min(lo + last * step, p.requests - 1);
+        hi = min(lo + step, hi);
+    }
+    if (p.requests == 1) begin_lo = static_cast<int>(static_cast<long long>(max(p.starts[0], 0)) * p.group / (kTiles * kTile));
+    begin = begin_lo;
+    return lo;
+}
+
+#define CHUNK_WAIT(bar, parity) \
+    if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&(bar), (parity), abort_flag)) != 0)) break
+
+// The query heads of a key-value head are rows of one tile (row = token * group + head), so a chunk of few tokens fills
+// its tiles and keys are read once for all of them.  One block of threads an SM: two 128-row tiles with a warpgroup of
+// softmax each (a row a thread: no exchange for maxima and sums), a TMA warp, an MMA warp.  Per 128-key block and tile
+//   S = Q K^T  (tcgen05, both operands from shared memory, 128 TMEM columns),
+//   P = exp2(scale S - m) back into the columns of S in 16 bits,
+//   O += P V   (A from tensor memory, V as it lies in the cache: MN-major), D TMEM columns.
+// While one tile's softmax runs, the tensor cores form the other's O and next S.  m follows the running maximum only
+// when that has grown by more than 2^8 (then O and l are scaled down, which is exact but for rounding): P stays below
+// 2^8, within fp16's range, and the rescaling of O all but disappears.
+// Scores, m, l and O are fp32; P is rounded to the type of V for the tensor cores, which costs what the rounding of the
+// output costs (the sum l is that of the unrounded P).
+// Two prompts of 7.2 k tokens, 16 / 4 heads of 128: 494 us, 870 TFLOP/s (the few-row kernel in the same place: 4.6 ms); 512 tokens over
+// 32 000, 16 / 2 heads: 159 us, 840 TFLOP/s (764 us).
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p,
+                             const int pairs, const int shares, float2* __restrict__ part_ml, float* __restrict__ part_out) {
+    extern __shared__ uint8_t chunk_raw[];
+    constexpr int kHalves = D / 64, kSlots = ring_slots<D>(), kSlotBytes = kHalves * kAtom;
+    Smem<D>& sm = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(chunk_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
+    grid_dependents_launch();
+    volatile int* abort_flag = &sm.abort;
+    if (tid == 0) {
+        sm.abort = 0;
+        for (int s = 0; s < kSlots; ++s) {
+            mbar_init(&sm.full[s], 1);
+            mbar_init(&sm.empty[s], 1);
+        }
+        mbar_init(&sm.q_ready, kSoftmaxWarps);
+        for (int t = 0; t < kTiles; ++t) {
+            mbar_init(&sm.s_full[t], 1);
+            mbar_init(&sm.p_full[t], 4);
+            mbar_init(&sm.o_done[t], 1);
+        }
+        fence_barrier_init();
+        prefetch_tensormap(&map_k);
+        prefetch_tensormap(&map_v);
+    }
+    if (warp == kSoftmaxWarps + 1) {
+        tmem_alloc(&sm.tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = sm.tmem;
+    grid_dependency_wait();
+
+    // the last pairs of a request see the most keys: they go first
+    const int head = blockIdx.x % p.kv_heads, share = blockIdx.x / p.kv_heads % shares, pair = pairs - 1 - blockIdx.x / p.kv_heads / shares;
+    int begin;
+    const int request = request_of(p, pair, begin);
+    Work w(p, request, head, pair - begin);
+    const bool mine = pair >= begin && w.rows > 0 && w.at.n * p.group > p.few_rows;
+    const int blocks = w.to - w.from;
+    // a share is two blocks of keys at least
+    const int parts = max(min(shares, blocks / 2), 1);
+    if (share >= parts) w.from = w.to;
+    else {
+        const int from = w.from;
+        w.from = from + static_cast<int>(static_cast<long long>(blocks) * share / parts);
+        w.to = from + static_cast<int>(static_cast<long long>(blocks) * (share + 1) / parts);
+    }
+    bool ok = true;
+    if (mine) {
+    if (warp == kSoftmaxWarps) {
+        // ------------------------------------------------------------ TMA
+        const int box = min(kBox, 1 << p.page_shift), boxes = kTile / box;         // boxes: up to 8
+        const int* table = p.table + static_cast<long long>(request) * p.max_pages;
+        int it = 0, held = -32, id = 0;
+        bool bad = w.at.cut;
+        for (int b = w.from; ok && b < w.to; ++b) {
+            const int key = b * kTile + min(lane, boxes - 1) * box, page = key >> p.page_shift;
+            if (((b * kTile + kTile - 1) >> p.page_shift) >= held + 32) {
+                held = (b * kTile) >> p.page_shift;
+                id = held + lane < p.max_pages ? table[held + lane] : -1;
+            }
+            int page_id = __shfl_sync(0xffffffffu, id, page - held);
+            const bool need = lane < boxes && key < w.hi && key + box > w.lo;
+            if (need && (page_id < 0 || page_id >= p.pages)) {
+                bad = true;
+                page_id = p.pages;                          // outside the tensor: zeros
+            }
+            const int count = __popc(__ballot_sync(0xffffffffu, need));
+            const int token = key & ((1 << p.page_shift) - 1);
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv, ++it) {
+                const int slot = it % kSlots;
+                CHUNK_WAIT(sm.empty[slot], (it / kSlots + 1) & 1);
+                if (lane == 0) mbar_arrive_expect_tx(&sm.full[slot], count * box * 128 * kHalves);
+                __syncwarp();
+                if (need) {
+#pragma unroll
+                    for (int half = 0; half < kHalves; ++half)
+                        tma_load_4d(sm.ring[slot][half] + lane * box * 128, kv == 0 ? &map_k : &map_v, &sm.full[slot], half * 64, token, head, page_id);
+                }
+                __syncwarp();
+            }
+        }
+        if (bad && p.status != nullptr) atomicOr(p.status, PK100_STATUS_PAGE);
+        // copies still in flight where a wait ran out: they must land before the block's memory is given away
+        if (!ok || *abort_flag != 0) {
+            const uint64_t start = global_timer_ns();
+            for (int i = max(it - kSlots, 0); i < it; ++i)
+                while (!mbar_try_wait(&sm.full[i % kSlots], (i / kSlots) & 1) && global_timer_ns() - start < 100000000ull) {}
+        }
+    } else if (warp == kSoftmaxWarps + 1) {
+        // ------------------------------------------------------------ MMA
+        constexpr uint32_t idesc_s = make_instr_desc<KIND_F16>(kTile, kTile) | type_bits<T>();
+        constexpr uint32_t idesc_o = make_instr_desc<KIND_F16>(kTile, D) | type_bits<T>() | (1u << 16);      // B is MN-major
+        const uint64_t desc_q = make_smem_desc<128>(smem_u32(sm.q)), desc_ring = make_smem_desc<128>(smem_u32(sm.ring));
+        // V[keys, features]: 8-key groups 1024 bytes apart, the second 64 features an atom on; 16 keys = 2048 bytes
+        const uint64_t desc_v = static_cast<uint64_t>((smem_u32(sm.ring) & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(kAtom >> 4) << 16) |
+                                (64ull << 32) | (1ull << 46) | (2ull << 61);
+        auto k_offset = [](int ks) { return static_cast<uint32_t>((ks / 4) * (kAtom / 16) + 2 * (ks % 4)); };
+        const bool leader = elect_one();
+        const int tile_from[kTiles] = {w.tile_from(p, 0), w.tile_from(p, 1)}, tile_to[kTiles] = {w.tile_to(p, 0), w.tile_to(p, 1)};
+        auto active = [&](int t, int b) { return b >= tile_from[t] && b < tile_to[t]; };
+        auto scores = [&](int t, int slot) {
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks)
+                tc_mma_if<KIND_F16>(leader, tmem + t * kTile, desc_q + t * (kSlotBytes / 16) + k_offset(ks), desc_ring + slot * (kSlotBytes / 16) + k_offset(ks),
+                                    idesc_s, ks > 0);
+            tc_commit_if(leader, &sm.s_full[t]);
+        };
+        uint32_t phase[kTiles] = {0, 0};                     // parity of the tile's next block
+        uint32_t filled[kTiles] = {0, 0};                    // O holds something
+        int it = 0;                                          // ring position of the block's keys; its values follow
+        do {
+            if (w.from >= w.to) break;
+            CHUNK_WAIT(sm.q_ready, 0);
+            CHUNK_WAIT(sm.full[0], 0);
+            tc_fence_after_sync();
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+                if (active(t, w.from)) scores(t, 0);
+            tc_commit_if(leader, &sm.empty[0]);
+#pragma unroll 1
+            for (int b = w.from; b < w.to; ++b, it += 2) {
+                const int v_slot = (it + 1) % kSlots, k_slot = (it + 2) % kSlots;
+                CHUNK_WAIT(sm.full[v_slot], ((it + 1) / kSlots) & 1);
+                // values that no row sees may be anything: zeros
+                const int k0 = b * kTile;
+                if (k0 < w.lo || k0 + kTile > w.hi) {
+                    for (int key = lane; key < kTile; key += 32)
+                        if (k0 + key < w.lo || k0 + key >= w.hi) {
+#pragma unroll
+                            for (int c = 0; c < kHalves * 8; ++c)
+                                *reinterpret_cast<uint4*>(sm.ring[v_slot][c / 8] + key * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                bool next_here = false;
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) {
+                    if (active(t, b)) {
+                        CHUNK_WAIT(sm.p_full[t], phase[t]);
+                        phase[t] ^= 1;
+                        tc_fence_after_sync();
+#pragma unroll
+                        for (int ks = 0; ks < kTile / 16; ++ks)
+                            mma_from_tmem(leader, tmem + kTiles * kTile + t * D, tmem + t * kTile + ks * 8, desc_v + v_slot * (kSlotBytes / 16) + ks * 128u, idesc_o,
+                                          ks > 0 ? 1u : filled[t]);
+                        filled[t] = 1;
+                        tc_commit_if(leader, &sm.o_done[t]);
+                    }
+                    if (b + 1 < w.to && active(t, b + 1)) {
+                        if (!next_here) {
+                            CHUNK_WAIT(sm.full[k_slot], ((it + 2) / kSlots) & 1);
+                            next_here = true;
+                            tc_fence_after_sync();
+                        }
+                        scores(t, k_slot);
+                    }
+                }
+                if (!ok) break;
+                if (b + 1 < w.to && !next_here) CHUNK_WAIT(sm.full[k_slot], ((it + 2) / kSlots) & 1);     // (every block has a tile that sees it)
+                tc_commit_if(leader, &sm.empty[v_slot]);
+                if (b + 1 < w.to) tc_commit_if(leader, &sm.empty[k_slot]);
+            }
+            // the last arrival of the tensor cores comes before the block leaves
+            if (ok) CHUNK_WAIT(sm.empty[(it - 1) % kSlots], ((it - 1) / kSlots) & 1);
+        } while (false);
+    } else {
+        // ------------------------------------------------------------ softmax, a row a thread
+        const int t = warp / 4, tile_row = (warp % 4) * 32 + lane;
+        {   // the queries of both tiles: 16 bytes a thread, rows that do not exist are zeros
+            constexpr int kChunks = D / 8;
+            for (int i = tid; i < kTiles * kTile * kChunks; i += kSoftmaxWarps * 32) {
+                const int r = i / kChunks, c = i % kChunks;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (r < w.rows) {
+                    const int index = w.row + r, token = index / p.group;
+                    v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.query) + (w.at.row0 + token) * p.ld_query +
+                                                        static_cast<long long>(head * p.group + index - token * p.group) * D + c * 8);
+                }
+                const int q_row = r % kTile;
+                *reinterpret_cast<uint4*>(sm.q[r / kTile][c / 8] + q_row * 128 + (((c % 8) ^ (q_row & 7)) << 4)) = v;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.q_ready);
+        }
+        const int index = w.row + t * kTile + tile_row, token = index / p.group;
+        const bool live = t * kTile + tile_row < w.rows;
+        const int row_lo = w.at.lo(p, token), row_hi = live ? w.at.hi(p, token) : 0;
+        // keys that every row of the tile sees
+        const int tile_rows = min(w.rows - t * kTile, kTile);
+        const int all_lo = w.at.lo(p, (w.row + t * kTile + max(tile_rows, 1) - 1) / p.group), all_hi = w.at.hi(p, (w.row + t * kTile) / p.group);
+        const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
+        const uint32_t s_cols = tmem + lanes + t * kTile, o_cols = tmem + lanes + kTiles * kTile + t * D;
+        const float scale = fmaxf(fabsf(p.scale_log2), 1e-37f);       // (-inf * 0 would be NaN; 1e-37 takes any score to 0)
+        float m = -INFINITY, l = 0.0f;                       // m: reference maximum of the raw scores
+        int done = 0;                                        // blocks of this tile
+        for (int b = w.tile_from(p, t), end = w.tile_to(p, t); b < end; ++b, ++done) {
+            CHUNK_WAIT(sm.s_full[t], done & 1);
+            tc_fence_after_sync();
+            float s[kTile];
+#pragma unroll
+            for (int c = 0; c < kTile; c += 32) tmem_ld_32x32(s_cols + c, reinterpret_cast<uint32_t(&)[32]>(s[c]));
+            tmem_ld_wait();
+            if (p.scale_log2 < 0.0f) {
+#pragma unroll
+                for (int i = 0; i < kTile; ++i) s[i] = -s[i];
+            }
+            const int k0 = b * kTile;
+            if (k0 < all_lo || k0 + kTile > all_hi) {
+                const int lo = row_lo - k0, hi = row_hi - k0;
+#pragma unroll
+                for (int i = 0; i < kTile; ++i) s[i] = i >= lo && i < hi ? s[i] : -INFINITY;
+            }
+            float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int i = 4; i < kTile; i += 4)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], s[i + j]);
+            const float seen = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+            // (-inf - -inf is NaN: no growth)
+            if (__any_sync(0xffffffffu, (seen - m) * scale > 8.0f || (done == 0 && seen > m))) {
+                const float factor = exp2_approx((m - (seen == -INFINITY ? 0.0f : seen)) * scale);
+                m = seen;
+                l *= factor;
+                if (done > 0) {
+                    CHUNK_WAIT(sm.o_done[t], (done - 1) & 1);
+                    tc_fence_after_sync();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld_32x16(o_cols + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                        tmem_st_32x16(o_cols + c, o);
+                    }
+                }
+            }
+            const float shift = m == -INFINITY ? 0.0f : -m * scale;
+            const Pair scale2 = pair_of(scale, scale), shift2 = pair_of(shift, shift);
+            Pair sum = pair_of(0.0f, 0.0f);
+#pragma unroll
+            for (int c = 0; c < kTile; c += 32) {
+                uint32_t packed[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float2 x = halves_of(pair_fma(pair_of(s[c + 2 * i], s[c + 2 * i + 1]), scale2, shift2));
+                    const float e0 = exp2_approx(x.x), e1 = exp2_approx(x.y);
+                    sum = pair_add(sum, pair_of(e0, e1));
+                    packed[i] = packed_of(e0, e1, T());
+                }
+                tmem_st_32x16(s_cols + c / 2, packed);
+            }
+            const float2 sums = halves_of(sum);
+            l += sums.x + sums.y;
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.p_full[t]);
+        }
+        // ------------------------------------------------------------ output
+        if (ok && done > 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], (done - 1) & 1, abort_flag)) != 0;
+            tc_fence_after_sync();
+        }
+        if (ok && tile_rows > 0) {
+            const long long row = static_cast<long long>(w.at.row0 + token) * p.heads + head * p.group + index - token * p.group;
+            const float inverse = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+            T* dst = static_cast<T*>(p.out) + (w.at.row0 + token) * p.ld_out + static_cast<long long>(head * p.group + index - token * p.group) * D;
+            const long long part = static_cast<long long>(share) * p.tokens * p.heads + row;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                if (done > 0) {
+                    tmem_ld_32x16(o_cols + c, o);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] = 0;
+                }
+                if (!live) continue;
+                if (shares > 1) {
+                    if (done > 0) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(part_out + part * D + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
+                } else {
+                    uint32_t v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = packed_of(__uint_as_float(o[2 * i]) * inverse, __uint_as_float(o[2 * i + 1]) * inverse, T());
+                    *reinterpret_cast<uint4*>(dst + c) = make_uint4(v[0], v[1], v[2], v[3]);
+                    *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+                }
+            }
+            if (live) {
+                if (shares > 1) part_ml[part] = make_float2(m * scale, l);
+                else if (p.lse != nullptr) p.lse[row] = l > 0.0f ? (m * scale + log2f(l)) * kLn2 : (l == 0.0f ? -INFINITY : l);
+            }
+        }
+    }
+    }
+    if (!ok && lane == 0 && p.status != nullptr) atomicOr(p.status, 1);
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == kSoftmaxWarps + 1) tmem_dealloc(tmem, 512);
+}
+
+// out of the shares of a row's keys, in their order, a warp a row.
+template <typename T, int D>
+__global__ void __launch_bounds__(128)
+shares_join_kernel(const PagedParams p, const int shares, const float2* __restrict__ part_ml, const float* __restrict__ part_out) {
+    grid_dependents_launch();
+    grid_dependency_wait();
+    const int token = blockIdx.x, lane = threadIdx.x % 32;
+    // the request that has the token: the last one that starts at or before it (an empty one never is)
+    int lo = 0, hi = p.requests;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, r = lo + lane * step;
+        const uint32_t before = __ballot_sync(0xffffffffu, r < hi && p.starts[r] <= token);
+        lo = min(lo + (before == 0 ? 0 : 31 - __clz(before)) * step, p.requests - 1);
+        hi = min(lo + step, hi);
+    }
+    const PagedRequest at(p, lo);
+    if (token < at.row0 || token >= at.row0 + at.n || at.n * p.group <= p.few_rows) return;
+    constexpr int kWidth = D / 32;
+    for (int h = blockIdx.y * 4 + threadIdx.x / 32; h < p.heads; h += gridDim.y * 4) {
+        const long long row = static_cast<long long>(token) * p.heads + h, step = static_cast<long long>(p.tokens) * p.heads;
+        float top = -INFINITY, sum = 0.0f, o[kWidth] = {};
+        for (int s = lane; s < shares; s += 32) {
+            const float2 ml = part_ml[s * step + row];
+            if (ml.y != 0.0f) top = fmaxf(top, ml.x);
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+#pragma unroll 4
+        for (int s = 0; s < shares; ++s) {
+            const float2 ml = part_ml[s * step + row];
+            if (ml.y == 0.0f) continue;                      // (a share that saw nothing left no output)
+            const float weight = exp2_approx(ml.x - top);
+            sum = fmaf(weight, ml.y, sum);
+#pragma unroll
+            for (int e = 0; e < kWidth; ++e) o[e] = fmaf(weight, part_out[(s * step + row) * D + lane * kWidth + e], o[e]);
+        }
+        const float inverse = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+        T* dst = static_cast<T*>(p.out) + token * p.ld_out + static_cast<long long>(h) * D + lane * kWidth;
+#pragma unroll
+        for (int e = 0; e < kWidth; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = packed_of(o[e] * inverse, o[e + 1] * inverse, T());
+        if (p.lse != nullptr && lane == 0) p.lse[row] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : (sum == 0.0f ? -INFINITY : sum);
+    }
+}
+
+template <typename T, int D>
+static int launch(const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares, float2* part_ml,
+                  float* part_out, cudaStream_t stream) {
+    constexpr auto kernel = paged_attention_chunk_kernel<T, D>;
+    constexpr int bytes = sizeof(Smem<D>) + 1024;
+    static_assert(bytes <= 227 * 1024, "shared memory");
+    const cudaError_t granted = pk100_grant_smem<kernel>(bytes);
+    if (granted != cudaSuccess) return static_cast<int>(granted);
+    pk100_launch_chained(kernel, dim3(static_cast<unsigned>(pairs) * shares * p.kv_heads), dim3(kThreads), bytes, stream, map_k, map_v, p, pairs, shares,
+                         part_ml, part_out);
+    const int rc = pk100_launch_status();
+    if (rc != PK100_OK || shares == 1) return rc;
+    pk100_launch_chained(shares_join_kernel<T, D>, dim3(p.tokens, (p.heads + 3) / 4 < 8 ? (p.heads + 3) / 4 : 8), dim3(128), 0, stream, p, shares, part_ml, part_out);
+    return pk100_launch_status();
+}
+
+}  // namespace chunk
+
+int paged_attention_chunks(int type, int head_dim, const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares,
+                           float2* part_ml, float* part_out, cudaStream_t stream) {
+    if (type == PK100_TYPE_F16)
+        return head_dim == 128 ? chunk::launch<__half, 128>(p, map_k, map_v, pairs, shares, part_ml, part_out, stream)
+                               : chunk::launch<__half, 64>(p, map_k, map_v, pairs, shares, part_ml, part_out, stream);
+    return head_dim == 128 ? chunk::launch<__nv_bfloat16, 128>(p, map_k, map_v, pairs, shares, part_ml, part_out, stream)
+                           : chunk::launch<__nv_bfloat16, 64>(p, map_k, map_v, pairs, shares, part_ml, part_out, stream);
+}
+
+}  // namespace pk100
