@@ -282,35 +282,42 @@ def _type(t):
     return code
 
 
-def _here(*tensors):
-    """The operators launch on the current device's stream: what they are given has to lie there."""
-    device = torch.cuda.current_device() if tensors[0].is_cuda else -1
-    for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != device):
-            raise L.Pk100Error("libpk100 operates on tensors of the current CUDA device only (there is no CPU path)")
+def _device(t):
+    """The operators launch on the current device's stream: its index, which what they are given has to have."""
+    return torch.cuda.current_device() if t.is_cuda else -2
 
 
-def _shaped(name, t, shape, dtype, inner=1):
-    """t has this shape and type; its last `inner` dimensions lie one behind the other."""
+def _refuse(name, t, shape, dtype, device):
+    if t.get_device() != device:
+        raise L.Pk100Error(f"{name}: libpk100 operates on tensors of the current CUDA device only (there is no CPU path)")
     if t.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    step = 1
-    for d in range(1, inner + 1):
-        if t.shape[-d] > 1 and t.stride(-d) != step and t.numel() > 0:
-            raise ValueError(f"{name}: the last {inner} dimension(s) have to be contiguous")
-        step *= t.shape[-d]
-    return t
+    raise ValueError(f"{name}: the elements of a row have to lie one behind the other")
 
 
-def _distance(t):
-    """Elements between the rows (a single row's stride may be anything)."""
-    return 0 if t is None else t.stride(0) if t.shape[0] > 1 else t[0].numel() if t.shape[0] else 0
+# (a tensor is looked at with as few calls as its checks take: they are most of the host time of a small launch)
+def _whole(name, t, shape, dtype, device):
+    """Address of a contiguous tensor of this shape and type."""
+    if t.dtype is not dtype or t.get_device() != device or t.shape != shape or not t.is_contiguous():
+        _refuse(name, t, shape, dtype, device)
+    return t.data_ptr()
+
+
+def _rows(name, t, shape, dtype, device):
+    """Address of [rows, ...] and elements between its rows, which are contiguous each."""
+    if t.dtype is not dtype or t.get_device() != device or t.shape != shape:
+        _refuse(name, t, shape, dtype, device)
+    if t.is_contiguous():
+        return t.data_ptr(), math.prod(shape[1:])
+    if shape[0] and not t[0].is_contiguous():
+        _refuse(name, t, shape, dtype, device)
+    return t.data_ptr(), t.stride(0) if shape[0] > 1 else math.prod(shape[1:])
 
 
 def _out_dtype(mode, dtype):
-    return {L.LN_F16: dtype, L.LN_E4M3_FIXED: torch.uint8, L.LN_E4M3_ROW: torch.uint8, L.LN_S8_ROW: torch.int8}[mode]
+    return dtype if mode == L.LN_F16 else torch.int8 if mode == L.LN_S8_ROW else torch.uint8
 
 
 def add_rms_norm(x, gamma, residual=None, mode=L.LN_F16, inv_scale=0.0, eps=EPS, out=None, residual_out=None, scales=None):
@@ -318,60 +325,57 @@ def add_rms_norm(x, gamma, residual=None, mode=L.LN_F16, inv_scale=0.0, eps=EPS,
 
     x, residual [rows, width] fp16 or bf16, rows any distance apart.  s is kept in residual_out (one of the inputs, or
     a new tensor when a residual is given) and is x itself without a residual.  scales is None for the modes without them."""
-    kind = _type(x)
-    if x.dim() != 2:
-        raise ValueError(f"x: expected [rows, width], got {tuple(x.shape)}")
-    rows, width = x.shape
+    kind, dtype, shape, device = _type(x), x.dtype, x.shape, _device(x)
+    if len(shape) != 2:
+        raise ValueError(f"x: expected [rows, width], got {tuple(shape)}")
+    rows, width = shape
     if mode not in (L.LN_F16, L.LN_E4M3_FIXED, L.LN_E4M3_ROW, L.LN_S8_ROW):
         raise ValueError(f"add_rms_norm has no output mode {mode}")
-    row_scales = mode in (L.LN_E4M3_ROW, L.LN_S8_ROW)
+    x_at, x_ld = _rows("x", x, shape, dtype, device)
+    gamma_at = _whole("gamma", gamma, (width,), dtype, device)
+    out_dtype = _out_dtype(mode, dtype)
     if out is None:
-        out = torch.empty((rows, width), device=x.device, dtype=_out_dtype(mode, x.dtype))
-    if residual_out is None and residual is not None:
-        residual_out = torch.empty((rows, width), device=x.device, dtype=x.dtype)
-    if scales is None and row_scales:
-        scales = torch.empty(rows, device=x.device, dtype=torch.float32)
-    _here(x, gamma, residual, out, residual_out, scales)
-    _shaped("x", x, x.shape, x.dtype)
-    _shaped("gamma", gamma, (width,), x.dtype)
-    _shaped("out", out, x.shape, _out_dtype(mode, x.dtype))
+        out = torch.empty(shape, device=x.device, dtype=out_dtype)
+    out_at, out_ld = _rows("out", out, shape, out_dtype, device)
+    res_at = res_ld = kept_at = kept_ld = scales_at = 0
     if residual is not None:
-        _shaped("residual", residual, x.shape, x.dtype)
+        res_at, res_ld = _rows("residual", residual, shape, dtype, device)
+        if residual_out is None:
+            residual_out = torch.empty(shape, device=x.device, dtype=dtype)
     if residual_out is not None:
-        _shaped("residual_out", residual_out, x.shape, x.dtype)
-    if row_scales:
-        _shaped("scales", scales, (rows,), torch.float32)
-    args = _RMS_NORM_ARGS.pack(
-        kind, mode, rows, width, x.data_ptr(), x.stride(0), _ptr(residual), 0 if residual is None else residual.stride(0),
-        _ptr(residual_out), 0 if residual_out is None else residual_out.stride(0), gamma.data_ptr(), eps, inv_scale,
-        out.data_ptr(), out.stride(0), _ptr(scales) if row_scales else 0)
-    L.check(_add_rms_norm(_stream(), args), "pk100_add_rms_norm")
-    return out, scales if row_scales else None, x if residual_out is None else residual_out
+        kept_at, kept_ld = _rows("residual_out", residual_out, shape, dtype, device)
+    if mode == L.LN_E4M3_ROW or mode == L.LN_S8_ROW:
+        if scales is None:
+            scales = torch.empty(rows, device=x.device, dtype=torch.float32)
+        scales_at = _whole("scales", scales, (rows,), torch.float32, device)
+    else:
+        scales = None
+    rc = _add_rms_norm(_stream(), _RMS_NORM_ARGS.pack(kind, mode, rows, width, x_at, x_ld, res_at, res_ld, kept_at, kept_ld, gamma_at, eps,
+                                                      inv_scale, out_at, out_ld, scales_at))
+    L.check(rc, "pk100_add_rms_norm")
+    return out, scales, x if residual_out is None else residual_out
 
 
 def gemv_w4g128(a, codes, group_scales, *, out=None, row_scales=None, row_scale=1.0, col_scales=None, bias=None, act=L.ACT_NONE,
                 residual=None, alpha=1.0, valid_rows=0, out_type=L.OUT_F16):
     """D = epilogue(A . W^T) for up to 16 rows, W from `pack_weight_rows(PACK_S4_G128)`; see `pk100_gemv_w4g128`."""
     m, k = a.shape
-    n = codes.shape[0]
+    n, device = codes.shape[0], _device(a)
+    a_at, a_ld = _rows("a", a, (m, k), torch.float16, device)
+    codes_at = _whole("codes", codes, (n, k // 2), torch.uint8, device)
+    groups_at = _whole("group_scales", group_scales, (k // 128, n), torch.float16, device)
     dtype = torch.float32 if out_type == L.OUT_F32 else torch.float16
     if out is None:
         out = torch.empty((m, n), device=a.device, dtype=dtype)
-    _here(a, codes, group_scales, out, row_scales, col_scales, bias, residual)
-    _shaped("a", a, (m, k), torch.float16)
-    _shaped("codes", codes, (n, k // 2), torch.uint8, 2)
-    _shaped("group_scales", group_scales, (k // 128, n), torch.float16, 2)
-    _shaped("out", out, (m, n), dtype)
-    for name, t, shape in (("row_scales", row_scales, (m,)), ("col_scales", col_scales, (n,)), ("bias", bias, (n,))):
-        if t is not None:
-            _shaped(name, t, shape, torch.float32)
-    if residual is not None:
-        _shaped("residual", residual, (m, n), torch.float16)
-    args = _GEMM_ARGS.pack(
-        L.KIND_F16_W4G128, L.EPI_LINEAR, m, n, k, a.data_ptr(), _distance(a), codes.data_ptr(), k // 2, _ptr(row_scales), row_scale,
-        _ptr(col_scales), _ptr(bias), act, _ptr(residual), _distance(residual), alpha, valid_rows,
-        out.data_ptr(), _distance(out), out_type, 1.0, 0.0, 0, 0, 0, 0, 0, group_scales.data_ptr())
-    L.check(_gemv_w4g128(_stream(), args), "pk100_gemv_w4g128")
+    out_at, out_ld = _rows("out", out, (m, n), dtype, device)
+    res_at, res_ld = (0, 0) if residual is None else _rows("residual", residual, (m, n), torch.float16, device)
+    rows_at = 0 if row_scales is None else _whole("row_scales", row_scales, (m,), torch.float32, device)
+    cols_at = 0 if col_scales is None else _whole("col_scales", col_scales, (n,), torch.float32, device)
+    bias_at = 0 if bias is None else _whole("bias", bias, (n,), torch.float32, device)
+    rc = _gemv_w4g128(_stream(), _GEMM_ARGS.pack(
+        L.KIND_F16_W4G128, L.EPI_LINEAR, m, n, k, a_at, a_ld, codes_at, k // 2, rows_at, row_scale, cols_at, bias_at, act, res_at, res_ld, alpha,
+        valid_rows, out_at, out_ld, out_type, 1.0, 0.0, 0, 0, 0, 0, 0, groups_at))
+    L.check(rc, "pk100_gemv_w4g128")
     return out
 
 
@@ -385,39 +389,44 @@ def paged_plan(cached, new_tokens, block_table, free_pages, free_count, *, token
     free_count [1], all int32.  `tokens` rows of positions (int32) and slots (int64) are returned in a PagedPlan with
     starts [requests + 1], lengths [requests] and used [1]; `out`: such a tuple to write to."""
     requests, max_pages = block_table.shape
+    device, i32 = _device(block_table), torch.int32
+    table_at = _whole("block_table", block_table, (requests, max_pages), i32, device)
+    cached_at = _whole("cached", cached, (requests,), i32, device)
+    new_at = _whole("new_tokens", new_tokens, (requests,), i32, device)
+    free_at = _whole("free_pages", free_pages, (free_pages.numel(),), i32, device)
+    count_at = _whole("free_count", free_count, (1,), i32, device)
+    status_at = 0 if status is None else _whole("status", status, (1,), i32, device)
     if out is None:
-        new = functools.partial(torch.empty, device=block_table.device)
-        words = new(2 * requests + 2 + tokens, dtype=torch.int32)
-        out = PagedPlan(*words[:2 * requests + 1].split([requests + 1, requests]), words[2 * requests + 1:-1],
-                        new(tokens, dtype=torch.int64), words[-1:])
-    _here(block_table, cached, new_tokens, free_pages, free_count, status, *out)
-    i32 = torch.int32
-    _shaped("block_table", block_table, (requests, max_pages), i32, 2)
-    for name, t, shape, dtype in (("cached", cached, (requests,), i32), ("new_tokens", new_tokens, (requests,), i32),
-                                  ("free_pages", free_pages, (free_pages.numel(),), i32), ("free_count", free_count, (1,), i32),
-                                  ("starts", out.starts, (requests + 1,), i32), ("lengths", out.lengths, (requests,), i32),
-                                  ("positions", out.positions, (tokens,), i32), ("slots", out.slots, (tokens,), torch.int64),
-                                  ("used", out.used, (1,), i32)):
-        _shaped(name, t, shape, dtype)
-    args = _PAGED_PLAN_ARGS.pack(
-        requests, tokens, page_size, max_pages, cached.data_ptr(), new_tokens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
-        block_table.data_ptr(), out.starts.data_ptr(), out.lengths.data_ptr(), out.positions.data_ptr(), out.slots.data_ptr(),
-        out.used.data_ptr(), _ptr(status))
-    L.check(_paged_plan(_stream(), args), "pk100_paged_plan")
+        words = torch.empty(2 * requests + 2 + tokens, device=block_table.device, dtype=i32)
+        starts, lengths, positions, used = words.split([requests + 1, requests, tokens, 1])
+        slots = torch.empty(tokens, device=block_table.device, dtype=torch.int64)
+        out = PagedPlan(starts, lengths, positions, slots, used)
+        at = words.data_ptr()
+        starts_at, lengths_at, positions_at, used_at = at, at + 4 * (requests + 1), at + 4 * (2 * requests + 1), at + 4 * (2 * requests + 1 + tokens)
+        slots_at = slots.data_ptr()
+    else:
+        starts_at = _whole("starts", out.starts, (requests + 1,), i32, device)
+        lengths_at = _whole("lengths", out.lengths, (requests,), i32, device)
+        positions_at = _whole("positions", out.positions, (tokens,), i32, device)
+        slots_at = _whole("slots", out.slots, (tokens,), torch.int64, device)
+        used_at = _whole("used", out.used, (1,), i32, device)
+    rc = _paged_plan(_stream(), _PAGED_PLAN_ARGS.pack(requests, tokens, page_size, max_pages, cached_at, new_at, free_at, count_at, table_at, starts_at,
+                                                      lengths_at, positions_at, slots_at, used_at, status_at))
+    L.check(rc, "pk100_paged_plan")
     return out
 
 
 @functools.lru_cache(maxsize=1024)
-def _paged_workspace(device, tokens, requests, heads, kv_heads, head_dim, page_size, max_pages, pages):
-    args = L.PagedAttentionArgs(tokens=tokens, requests=requests, heads=heads, kv_heads=kv_heads, head_dim=head_dim, pages=pages,
-                                page_size=page_size, max_pages=max_pages)
+def _paged_workspace(device, tokens, requests, heads, kv_heads, head_dim, page_size, max_pages):
+    args = L.PagedAttentionArgs(tokens=tokens, requests=requests, heads=heads, kv_heads=kv_heads, head_dim=head_dim, pages=1, page_size=page_size,
+                                max_pages=max_pages)
     return L.lib.pk100_paged_attention_workspace_bytes(args)
 
 
 def paged_attention_workspace(query, key_cache, block_table):
     """Bytes that `paged_attention` needs for these tensors on the current device."""
     return _paged_workspace(torch.cuda.current_device(), query.shape[0], block_table.shape[0], query.shape[1], key_cache.shape[2],
-                            query.shape[2], key_cache.shape[1], block_table.shape[1], key_cache.shape[0])
+                            query.shape[2], key_cache.shape[1], block_table.shape[1])
 
 
 def paged_attention(query, key_cache, value_cache, block_table, starts, lengths, *, key=None, value=None, slots=None, causal=True,
@@ -429,44 +438,45 @@ def paged_attention(query, key_cache, value_cache, block_table, starts, lengths,
     [requests + 1] and lengths [requests] int32.  key, value [tokens, kv_heads, head_dim] with slots [tokens] int64 are
     written to the cache first.  scale: 1 / sqrt(head_dim) by default.  workspace (uint8): allocated for the call where
     it is not given; one that is given is not used by another call at the same time."""
-    kind, dtype = _type(query), query.dtype
-    tokens, heads, head_dim = query.shape
-    pages, page_size, kv_heads, _ = key_cache.shape
-    requests, max_pages = block_table.shape
-    if out is None:
-        out = torch.empty((tokens, heads, head_dim), device=query.device, dtype=dtype)
-    _here(query, key_cache, value_cache, block_table, starts, lengths, key, value, slots, out, lse, workspace, status)
-    _shaped("query", query, (tokens, heads, head_dim), dtype, 2)
-    _shaped("out", out, (tokens, heads, head_dim), dtype, 2)
-    _shaped("key_cache", key_cache, (pages, page_size, kv_heads, head_dim), dtype)
-    _shaped("value_cache", value_cache, (pages, page_size, kv_heads, head_dim), dtype)
-    if key_cache.stride() != value_cache.stride():
+    kind, dtype, device, shape, i32 = _type(query), query.dtype, _device(query), query.shape, torch.int32
+    tokens, heads, head_dim = shape
+    pages, page_size, kv_heads, _ = cache_shape = key_cache.shape
+    requests, max_pages = table_shape = block_table.shape
+    query_at, query_ld = _rows("query", query, shape, dtype, device)
+    strides = key_cache.stride()
+    for name, t in (("key_cache", key_cache), ("value_cache", value_cache)):
+        if t.dtype is not dtype or t.get_device() != device or t.shape != cache_shape or cache_shape[3] != head_dim or strides[3] != 1:
+            _refuse(name, t, (pages, page_size, kv_heads, head_dim), dtype, device)
+    if value_cache.stride() != strides:
         raise ValueError("key_cache and value_cache have to have the same strides")
-    _shaped("block_table", block_table, (requests, max_pages), torch.int32, 2)
-    _shaped("starts", starts, (requests + 1,), torch.int32)
-    _shaped("lengths", lengths, (requests,), torch.int32)
+    table_at = _whole("block_table", block_table, table_shape, i32, device)
+    starts_at = _whole("starts", starts, (requests + 1,), i32, device)
+    lengths_at = _whole("lengths", lengths, (requests,), i32, device)
+    key_at = key_ld = value_at = value_ld = slots_at = 0
     if key is not None:
         if value is None or slots is None:
             raise ValueError("key needs value and slots")
-        _shaped("key", key, (tokens, kv_heads, head_dim), dtype, 2)
-        _shaped("value", value, (tokens, kv_heads, head_dim), dtype, 2)
-        _shaped("slots", slots, (tokens,), torch.int64)
-    if lse is not None:
-        _shaped("lse", lse, (tokens, heads), torch.float32, 2)
+        new_shape = (tokens, kv_heads, head_dim)
+        key_at, key_ld = _rows("key", key, new_shape, dtype, device)
+        value_at, value_ld = _rows("value", value, new_shape, dtype, device)
+        slots_at = _whole("slots", slots, (tokens,), torch.int64, device)
     if heads % kv_heads:
         raise ValueError(f"{heads} query heads do not share {kv_heads} key-value heads evenly")
+    if out is None:
+        out = torch.empty(shape, device=query.device, dtype=dtype)
+    out_at, out_ld = _rows("out", out, shape, dtype, device)
+    lse_at = 0 if lse is None else _whole("lse", lse, (tokens, heads), torch.float32, device)
+    status_at = 0 if status is None else _whole("status", status, (1,), i32, device)
     if workspace is None:
-        need = paged_attention_workspace(query, key_cache, block_table)
+        need = _paged_workspace(device, tokens, requests, heads, kv_heads, head_dim, page_size, max_pages)
         workspace = torch.empty(need, device=query.device, dtype=torch.uint8)
     else:
-        _shaped("workspace", workspace, workspace.shape, torch.uint8, workspace.dim())
-    page_stride, token_stride, head_stride, _ = key_cache.stride()
-    args = _PAGED_ATTENTION_ARGS.pack(
-        kind, tokens, requests, heads, kv_heads, head_dim, pages, page_size, max_pages, query.data_ptr(), query.stride(0),
-        _ptr(key), 0 if key is None else key.stride(0), 0 if key is None else value.data_ptr(), 0 if key is None else value.stride(0),
-        0 if key is None else slots.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), page_stride, token_stride, head_stride,
-        starts.data_ptr(), lengths.data_ptr(), block_table.data_ptr(), int(causal), min(window, 1 << 30), min(max_new, 1 << 30),
-        1.0 / math.sqrt(head_dim) if scale is None else scale, out.data_ptr(), out.stride(0), _ptr(lse), workspace.data_ptr(),
-        workspace.numel(), _ptr(status))
-    L.check(_paged_attention(_stream(), args), "pk100_paged_attention")
+        need = workspace.numel()
+        _whole("workspace", workspace, (need,), torch.uint8, device)
+    rc = _paged_attention(_stream(), _PAGED_ATTENTION_ARGS.pack(
+        kind, tokens, requests, heads, kv_heads, head_dim, pages, page_size, max_pages, query_at, query_ld, key_at, key_ld, value_at, value_ld,
+        slots_at, key_cache.data_ptr(), value_cache.data_ptr(), strides[0], strides[1], strides[2], starts_at, lengths_at, table_at, int(causal),
+        min(window, 1 << 30), min(max_new, 1 << 30), head_dim ** -0.5 if scale is None else scale, out_at, out_ld, lse_at,
+        workspace.data_ptr(), need, status_at))
+    L.check(rc, "pk100_paged_attention")
     return out
