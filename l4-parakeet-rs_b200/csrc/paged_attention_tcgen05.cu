@@ -6,10 +6,12 @@ namespace chunk {
 
 constexpr int kTile = 128;                      // (token, head) rows of an accumulator, and keys of a block
 constexpr int kTiles = 2;                       // tiles of a block of threads: one's softmax runs under the other's products
-constexpr int kSoftmaxWarps = 4 * kTiles;
+constexpr int kTileWarps = 8;                   // softmax warps of a tile: four lane quadrants, two halves of the keys
+constexpr int kSoftmaxWarps = kTileWarps * kTiles;
 constexpr int kThreads = kSoftmaxWarps * 32 + 64;
 constexpr int kAtom = kTile * 128;              // 128 rows x 64 elements, 128-byte swizzle
 constexpr int kBox = 64;                        // most keys of a TMA box
+constexpr int kByFma = 4;                       // of 16 pairs of scores, whose exponentials the FMA pipe forms
 
 template <int D> constexpr int ring_slots() { return D == 128 ? 5 : 8; }
 
@@ -18,6 +20,7 @@ struct Smem {
     uint8_t q[kTiles][D / 64][kAtom];
     uint8_t ring[ring_slots<D>()][D / 64][kAtom];          // key and value blocks in turn
     uint64_t full[ring_slots<D>()], empty[ring_slots<D>()];
+    float top[kTiles][2][kTile];                           // row maxima of the halves; then sums
     uint64_t q_ready, s_full[kTiles], p_full[kTiles], o_done[kTiles];
     uint32_t tmem;
     int abort;
@@ -31,6 +34,53 @@ __device__ __forceinline__ void mma_from_tmem(bool leader, uint32_t d, uint32_t 
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
                  "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
                  ::"r"(d), "r"(a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(static_cast<uint32_t>(leader)) : "memory");
+}
+
+// 2^x for two values at most 9: n = rint(x), a polynomial of the remainder (minimax of the relative error, degree 4: 2.7e-6,
+// far below the rounding of P), n into the exponent.  x below -126 counts as -126.  On the FMA pipe, where
+// ex2.approx (16 a clock and SM) would take as long as the tensor cores' products.
+__device__ __forceinline__ Pair exp2_fma(Pair x) {
+    const float2 v = halves_of(x);
+    x = pair_of(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
+    const Pair magic = pair_of(12582912.0f, 12582912.0f), back = pair_of(-12582912.0f, -12582912.0f);       // 1.5 * 2^23
+    const Pair n = pair_add(x, magic);
+    const Pair r = pair_fma(pair_add(n, back), pair_of(-1.0f, -1.0f), x);
+    Pair y = pair_fma(r, pair_of(0.009570102207362652f, 0.009570102207362652f), pair_of(0.05591785907745361f, 0.05591785907745361f));
+    y = pair_fma(r, y, pair_of(0.240247443318367f, 0.240247443318367f));
+    y = pair_fma(r, y, pair_of(0.6931217908859253f, 0.6931217908859253f));
+    y = pair_fma(r, y, pair_of(0.9999992847442627f, 0.9999992847442627f));
+    const float2 whole = halves_of(n), part = halves_of(y);
+    return pair_of(__uint_as_float(__float_as_uint(part.x) + (__float_as_uint(whole.x) << 23)),
+                   __uint_as_float(__float_as_uint(part.y) + (__float_as_uint(whole.y) << 23)));
+}
+
+// P = exp2(s * scale + shift) of 64 scores, stored as 16-bit pairs; the sum of the unrounded values.  ByFma: of 16 pairs
+// of scores, how many go to the FMA pipe (none where scores are masked: their -infinity has to give an exact zero).
+template <typename T, int ByFma>
+__device__ __forceinline__ float weights_of_scores(const float (&s)[64], float scale, float shift, uint32_t p_cols) {
+    const Pair scale2 = pair_of(scale, scale), shift2 = pair_of(shift, shift);
+    Pair sum = pair_of(0.0f, 0.0f);
+#pragma unroll
+    for (int c = 0; c < 64; c += 32) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const Pair x = pair_fma(pair_of(s[c + 2 * i], s[c + 2 * i + 1]), scale2, shift2);
+            Pair e;
+            if (i * ByFma % 16 + ByFma >= 16) {              // spread evenly
+                e = exp2_fma(x);
+            } else {
+                const float2 v = halves_of(x);
+                e = pair_of(exp2_approx(v.x), exp2_approx(v.y));
+            }
+            sum = pair_add(sum, e);
+            const float2 v = halves_of(e);
+            packed[i] = packed_of(v.x, v.y, T());
+        }
+        tmem_st_32x16(p_cols + c / 2, packed);
+    }
+    const float2 sums = halves_of(sum);
+    return sums.x + sums.y;
 }
 
 // What a block of threads works on: 256 rows of one request and key-value head, over a share of their keys.
@@ -100,9 +150,9 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p,
                              const int pairs, const int shares, float2* __restrict__ part_ml, float* __restrict__ part_out) {
-    extern __shared__ uint8_t chunk_raw[];
+    extern __shared__ __align__(1024) uint8_t chunk_raw[];             // (the swizzled atoms need it)
     constexpr int kHalves = D / 64, kSlots = ring_slots<D>(), kSlotBytes = kHalves * kAtom;
-    Smem<D>& sm = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(chunk_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    Smem<D>& sm = *reinterpret_cast<Smem<D>*>(chunk_raw);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
     grid_dependents_launch();
     volatile int* abort_flag = &sm.abort;
@@ -115,7 +165,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         mbar_init(&sm.q_ready, kSoftmaxWarps);
         for (int t = 0; t < kTiles; ++t) {
             mbar_init(&sm.s_full[t], 1);
-            mbar_init(&sm.p_full[t], 4);
+            mbar_init(&sm.p_full[t], kTileWarps);
             mbar_init(&sm.o_done[t], 1);
         }
         fence_barrier_init();
@@ -269,8 +319,8 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             if (ok) CHUNK_WAIT(sm.empty[(it - 1) % kSlots], ((it - 1) / kSlots) & 1);
         } while (false);
     } else {
-        // ------------------------------------------------------------ softmax, a row a thread
-        const int t = warp / 4, tile_row = (warp % 4) * 32 + lane;
+        // ------------------------------------------------------------ softmax: half a row a thread
+        const int t = warp / kTileWarps, half = (warp / 4) % 2, quad = warp % 4, tile_row = quad * 32 + lane;
         {   // the queries of both tiles: 16 bytes a thread, rows that do not exist are zeros
             constexpr int kChunks = D / 8;
             for (int i = tid; i < kTiles * kTile * kChunks; i += kSoftmaxWarps * 32) {
@@ -288,50 +338,58 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.q_ready);
         }
+        // the two warps of a quadrant of a tile
+        auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + quad) : "memory"); };
         const int index = w.row + t * kTile + tile_row, token = index / p.group;
         const bool live = t * kTile + tile_row < w.rows;
         const int row_lo = w.at.lo(p, token), row_hi = live ? w.at.hi(p, token) : 0;
         // keys that every row of the tile sees
         const int tile_rows = min(w.rows - t * kTile, kTile);
         const int all_lo = w.at.lo(p, (w.row + t * kTile + max(tile_rows, 1) - 1) / p.group), all_hi = w.at.hi(p, (w.row + t * kTile) / p.group);
-        const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
-        const uint32_t s_cols = tmem + lanes + t * kTile, o_cols = tmem + lanes + kTiles * kTile + t * D;
+        const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+        const uint32_t s_cols = tmem + lanes + t * kTile + half * 64, p_cols = tmem + lanes + t * kTile + half * 32;
+        const uint32_t o_cols = tmem + lanes + kTiles * kTile + t * D + half * (D / 2);
         const float scale = fmaxf(fabsf(p.scale_log2), 1e-37f);       // (-inf * 0 would be NaN; 1e-37 takes any score to 0)
-        float m = -INFINITY, l = 0.0f;                       // m: reference maximum of the raw scores
+        float m = -INFINITY, l = 0.0f;                       // m: reference maximum of the raw scores; l: sum over this half of the keys
         int done = 0;                                        // blocks of this tile
+        // (a wait that ran out does not end the loop: the other warp of the pair would wait at the barrier for ever)
         for (int b = w.tile_from(p, t), end = w.tile_to(p, t); b < end; ++b, ++done) {
-            CHUNK_WAIT(sm.s_full[t], done & 1);
+            ok &= __all_sync(0xffffffffu, mbar_wait_bounded(&sm.s_full[t], done & 1, abort_flag)) != 0;
             tc_fence_after_sync();
-            float s[kTile];
-#pragma unroll
-            for (int c = 0; c < kTile; c += 32) tmem_ld_32x32(s_cols + c, reinterpret_cast<uint32_t(&)[32]>(s[c]));
+            float s[64];
+            tmem_ld_32x32(s_cols, reinterpret_cast<uint32_t(&)[32]>(s[0]));
+            tmem_ld_32x32(s_cols + 32, reinterpret_cast<uint32_t(&)[32]>(s[32]));
             tmem_ld_wait();
             if (p.scale_log2 < 0.0f) {
 #pragma unroll
-                for (int i = 0; i < kTile; ++i) s[i] = -s[i];
+                for (int i = 0; i < 64; ++i) s[i] = -s[i];
             }
             const int k0 = b * kTile;
-            if (k0 < all_lo || k0 + kTile > all_hi) {
-                const int lo = row_lo - k0, hi = row_hi - k0;
+            const bool masked = k0 < all_lo || k0 + kTile > all_hi;
+            if (masked) {
+                const int lo = row_lo - k0 - half * 64, hi = row_hi - k0 - half * 64;
 #pragma unroll
-                for (int i = 0; i < kTile; ++i) s[i] = i >= lo && i < hi ? s[i] : -INFINITY;
+                for (int i = 0; i < 64; ++i) s[i] = i >= lo && i < hi ? s[i] : -INFINITY;
             }
             float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int i = 4; i < kTile; i += 4)
+            for (int i = 4; i < 64; i += 4)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], s[i + j]);
-            const float seen = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+            const float own = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            sm.top[t][half][tile_row] = own;                 // (the partner has read the last one: S of this block came after its P)
+            pair_sync();                                     // (also: both halves of S have been read, P may take their place)
+            const float seen = fmaxf(m, fmaxf(own, sm.top[t][half ^ 1][tile_row]));
             // (-inf - -inf is NaN: no growth)
             if (__any_sync(0xffffffffu, (seen - m) * scale > 8.0f || (done == 0 && seen > m))) {
                 const float factor = exp2_approx((m - (seen == -INFINITY ? 0.0f : seen)) * scale);
                 m = seen;
                 l *= factor;
                 if (done > 0) {
-                    CHUNK_WAIT(sm.o_done[t], (done - 1) & 1);
+                    ok &= __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], (done - 1) & 1, abort_flag)) != 0;
                     tc_fence_after_sync();
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 16) {
+                    for (int c = 0; c < D / 2; c += 16) {
                         uint32_t o[16];
                         tmem_ld_32x16(o_cols + c, o);
                         tmem_ld_wait();
@@ -342,28 +400,17 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 }
             }
             const float shift = m == -INFINITY ? 0.0f : -m * scale;
-            const Pair scale2 = pair_of(scale, scale), shift2 = pair_of(shift, shift);
-            Pair sum = pair_of(0.0f, 0.0f);
-#pragma unroll
-            for (int c = 0; c < kTile; c += 32) {
-                uint32_t packed[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float2 x = halves_of(pair_fma(pair_of(s[c + 2 * i], s[c + 2 * i + 1]), scale2, shift2));
-                    const float e0 = exp2_approx(x.x), e1 = exp2_approx(x.y);
-                    sum = pair_add(sum, pair_of(e0, e1));
-                    packed[i] = packed_of(e0, e1, T());
-                }
-                tmem_st_32x16(s_cols + c / 2, packed);
-            }
-            const float2 sums = halves_of(sum);
-            l += sums.x + sums.y;
+            l += masked ? weights_of_scores<T, 0>(s, scale, shift, p_cols) : weights_of_scores<T, kByFma>(s, scale, shift, p_cols);
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.p_full[t]);
         }
-        // ------------------------------------------------------------ output
+        // ------------------------------------------------------------ output: half the features a thread
+        pair_sync();
+        sm.top[t][half][tile_row] = l;
+        pair_sync();
+        l += sm.top[t][half ^ 1][tile_row];
         if (ok && done > 0) {
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], (done - 1) & 1, abort_flag)) != 0;
             tc_fence_after_sync();
@@ -371,10 +418,11 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         if (ok && tile_rows > 0) {
             const long long row = static_cast<long long>(w.at.row0 + token) * p.heads + head * p.group + index - token * p.group;
             const float inverse = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-            T* dst = static_cast<T*>(p.out) + (w.at.row0 + token) * p.ld_out + static_cast<long long>(head * p.group + index - token * p.group) * D;
+            T* dst = static_cast<T*>(p.out) + (w.at.row0 + token) * p.ld_out + static_cast<long long>(head * p.group + index - token * p.group) * D + half * (D / 2);
             const long long part = static_cast<long long>(share) * p.tokens * p.heads + row;
+            float* part_dst = part_out + part * D + half * (D / 2);
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
+            for (int c = 0; c < D / 2; c += 16) {
                 uint32_t o[16];
                 if (done > 0) {
                     tmem_ld_32x16(o_cols + c, o);
@@ -387,7 +435,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 if (shares > 1) {
                     if (done > 0) {
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(part_out + part * D + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(part_dst + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                     }
                 } else {
                     uint32_t v[8];
@@ -397,7 +445,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                     *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(v[4], v[5], v[6], v[7]);
                 }
             }
-            if (live) {
+            if (live && half == 0) {
                 if (shares > 1) part_ml[part] = make_float2(m * scale, l);
                 else if (p.lse != nullptr) p.lse[row] = l > 0.0f ? (m * scale + log2f(l)) * kLn2 : (l == 0.0f ? -INFINITY : l);
             }
@@ -458,7 +506,7 @@ template <typename T, int D>
 static int launch(const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares, float2* part_ml,
                   float* part_out, cudaStream_t stream) {
     constexpr auto kernel = paged_attention_chunk_kernel<T, D>;
-    constexpr int bytes = sizeof(Smem<D>) + 1024;
+    constexpr int bytes = sizeof(Smem<D>);
     static_assert(bytes <= 227 * 1024, "shared memory");
     const cudaError_t granted = pk100_grant_smem<kernel>(bytes);
     if (granted != cudaSuccess) return static_cast<int>(granted);
