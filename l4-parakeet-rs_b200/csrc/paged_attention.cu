@@ -1,5 +1,5 @@
 // Attention of new tokens over a paged key-value cache: the copy of new keys and values into their slots, the kernel
-// for requests of few rows (single tokens), the join of what several blocks found out about one row, and the host side.
+// for requests of few rows (single tokens), and the host side.
 #include <mutex>
 
 #include "paged_attention.cuh"
@@ -14,6 +14,7 @@ struct AppendParams {
     long long page_stride, token_stride, head_stride;
     int tokens, kv_heads, head_dim, page_shift;
     long long capacity;                                // slots of the cache
+    int* counts; int n_counts;                         // of the kernel behind: zeroed
     int* status;
 };
 
@@ -22,6 +23,7 @@ __global__ void __launch_bounds__(256)
 paged_append_kernel(const AppendParams p) {
     grid_dependents_launch();
     grid_dependency_wait();
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < p.n_counts; i += gridDim.x * blockDim.x) p.counts[i] = 0;
     const int chunks = p.head_dim / 8, per_token = p.kv_heads * chunks;
     const long long work = static_cast<long long>(p.tokens) * per_token;
     for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < work; i += static_cast<long long>(gridDim.x) * blockDim.x) {
@@ -49,8 +51,6 @@ constexpr int kRowThreads = kRowWarps * 32 + 32;
 
 // What a block found out about a tile of which it had a part: row maxima (log2 scale) and sums, and the unscaled output.
 struct RowsPart { float m[kRows], l[kRows]; };
-// The tile in which a block's work begins.
-struct RowsBegin { long long share, first, last; int request, head, tile, unused; };   // units [first, last) of the tile
 
 template <int D> constexpr int rows_stages() { return D == 128 ? 3 : 6; }
 
@@ -63,8 +63,8 @@ struct RowsSmem {
     float sum[kRowWarps][kRows];
     long long scan[kRowThreads / 32];
     uint64_t full[rows_stages<D>()], empty[rows_stages<D>()];
-    long long total, base;
-    int request, abort;
+    long long base;
+    int request, abort, last;
 };
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -118,10 +118,59 @@ __device__ __forceinline__ void rows_walk(const PagedParams& p, int request, lon
     }
 }
 
+// out of the parts that blocks [before, last] had of a row, by a warp.  (Written by other SMs: read past the L1.)
+template <typename T, int D>
+__device__ __forceinline__ void join_row(const PagedParams& p, const PagedRequest& at, int head, int index, int row, int before, int last,
+                                         long long opening, const RowsPart* parts, const float* part_out) {
+    const int lane = threadIdx.x % 32;
+    auto part_of = [&](int block) { return block == before ? opening : 2ll * block; };
+    float top = -INFINITY;
+    for (int k = before + lane; k <= last; k += 32) top = fmaxf(top, __ldcg(&parts[part_of(k)].m[row]));
+#pragma unroll
+    for (int off = 16; off > 0; off /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    const float zero = top == -INFINITY ? 0.0f : top;
+    constexpr int kWidth = D / 32;
+    float o[kWidth] = {}, sum = 0.0f;
+    for (int k0 = before; k0 <= last; k0 += 32) {
+        const int count = min(32, last - k0 + 1);
+        float weight = 0.0f;
+        if (lane < count) {
+            const RowsPart& q = parts[part_of(k0 + lane)];
+            weight = exp2_approx(__ldcg(&q.m[row]) - zero);
+            sum += weight * __ldcg(&q.l[row]);
+        }
+#pragma unroll 8
+        for (int k = 0; k < count; ++k) {
+            const float w = __shfl_sync(0xffffffffu, weight, k);
+            const float* src = part_out + (part_of(k0 + k) * kRows + row) * D + lane * kWidth;
+            if constexpr (kWidth == 4) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+                o[0] = fmaf(w, v.x, o[0]);
+                o[1] = fmaf(w, v.y, o[1]);
+                o[2] = fmaf(w, v.z, o[2]);
+                o[3] = fmaf(w, v.w, o[3]);
+            } else {
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+                o[0] = fmaf(w, v.x, o[0]);
+                o[1] = fmaf(w, v.y, o[1]);
+            }
+        }
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    const float inverse = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+    const int i = index / p.group;
+    const long long h = head * p.group + index - i * p.group;
+    T* dst = static_cast<T*>(p.out) + (at.row0 + i) * p.ld_out + h * D + lane * kWidth;
+#pragma unroll
+    for (int e = 0; e < kWidth; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = packed_of(o[e] * inverse, o[e + 1] * inverse, T());
+    if (p.lse != nullptr && lane == 0) p.lse[static_cast<long long>(at.row0 + i) * p.heads + h] = (top + log2f(sum)) * kLn2;
+}
+
 // Single tokens are bound by reading the cache once.  All (request, head, 64-key block) units of the step lie on one
 // line that the blocks share evenly, whatever the lengths: a block's part of the line is a run of blocks, with a
-// tile's beginning or end wherever they fall; what a block has of a tile that others share goes to the workspace and
-// rows_join_kernel adds it up in a fixed order.  The query heads of a key-value head are rows of one 16-row tile, so
+// tile's beginning or end wherever they fall; what a block has of a tile that others share goes to the workspace, and
+// the block that comes last adds the parts up, in the order of the blocks.  The query heads of a key-value head are rows of one 16-row tile, so
 // keys and values are read once for all of them.
 // A warp requests 64-key stages by TMA (a page or part of one a box, 128-byte swizzle), two blocks an SM keep up to
 // six of them in flight.  Q.K: each of four warps 16 keys; the row maxima are exchanged, so that all warps scale
@@ -131,7 +180,7 @@ __device__ __forceinline__ void rows_walk(const PagedParams& p, int request, lon
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads, 2)
 paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p,
-                            RowsBegin* begins, RowsPart* parts, float* part_out) {
+                            int* counts, RowsPart* parts, float* part_out) {
     extern __shared__ uint8_t rows_raw[];
     constexpr int kStages = rows_stages<D>(), kHalves = D / 64;
     RowsSmem<D>& sm = *reinterpret_cast<RowsSmem<D>*>((reinterpret_cast<uintptr_t>(rows_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -181,16 +230,6 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
     __syncthreads();
     const int first_request = sm.request;
     const long long first_base = sm.base;
-    if (tid == 0) {
-        RowsBegin b{share, -1, -1, 0, 0, 0, 0};
-        if (begin < end) {
-            const RowsShape s(p, first_request);
-            const long long tile_at = (begin - first_base) / s.blocks;
-            b = RowsBegin{share, first_base + tile_at * s.blocks, first_base + (tile_at + 1) * s.blocks, first_request,
-                          static_cast<int>(tile_at / s.tiles), static_cast<int>(tile_at % s.tiles), 0};
-        }
-        begins[blockIdx.x] = b;
-    }
     volatile int* abort_flag = &sm.abort;
 
     if (warp == kRowWarps) {
@@ -427,60 +466,21 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
                     parts[part].l[g] = l0;
                     parts[part].l[g + 8] = l1;
                 }
+                // the last of the tile's blocks adds the parts up
+                __threadfence();
+                row_warps_sync();
+                const int before = static_cast<int>(tile_first / share), last = static_cast<int>((tile_first + s.blocks - 1) / share);
+                if (tid == 0) sm.last = atomicAdd(&counts[before], 1) == last - before;
+                row_warps_sync();
+                if (sm.last) {
+                    __threadfence();
+                    const long long opening = 2ll * before + (tile_first == share * before ? 0 : 1);      // the others are first parts
+                    for (int row = warp; row < min(rows, kRows); row += kRowWarps)
+                        join_row<T, D>(p, s.at, head, tile * kRows + row, row, before, last, opening, parts, part_out);
+                }
             }
         });
     }
-}
-
-// out of the parts of a tile that several blocks had, a warp a row, in the order of the blocks.  Block x stands at the
-// border between two blocks of the kernel above and joins the tile that lies on it, if that is the tile's first border.
-template <typename T, int D>
-__global__ void __launch_bounds__(128)
-rows_join_kernel(const PagedParams p, const RowsBegin* begins, const RowsPart* parts, const float* part_out) {
-    grid_dependents_launch();
-    grid_dependency_wait();
-    const int border = blockIdx.x + 1, row = blockIdx.y * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
-    const RowsBegin b = begins[border];
-    if (b.first < 0 || b.first >= b.share * border || b.first < b.share * (border - 1)) return;
-    const PagedRequest at(p, b.request);
-    const int index = b.tile * kRows + row;
-    if (index >= at.n * p.group) return;
-    const int before = border - 1, last = static_cast<int>((b.last - 1) / b.share);
-    const long long opening = 2ll * before + (b.first == b.share * before ? 0 : 1);       // the others are first parts
-    auto part_of = [&](int block) { return block == before ? opening : 2ll * block; };
-
-    float top = -INFINITY;
-    for (int k = before + lane; k <= last; k += 32) top = fmaxf(top, parts[part_of(k)].m[row]);
-#pragma unroll
-    for (int off = 16; off > 0; off /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    const float zero = top == -INFINITY ? 0.0f : top;
-    constexpr int kWidth = D / 32;
-    float o[kWidth] = {}, sum = 0.0f;
-    for (int k0 = before; k0 <= last; k0 += 32) {
-        const int count = min(32, last - k0 + 1);
-        float weight = 0.0f;
-        if (lane < count) {
-            const RowsPart& q = parts[part_of(k0 + lane)];
-            weight = exp2_approx(q.m[row] - zero);
-            sum += weight * q.l[row];
-        }
-#pragma unroll 4
-        for (int k = 0; k < count; ++k) {
-            const float w = __shfl_sync(0xffffffffu, weight, k);
-            const float* src = part_out + (part_of(k0 + k) * kRows + row) * D + lane * kWidth;
-#pragma unroll
-            for (int e = 0; e < kWidth; ++e) o[e] = fmaf(w, src[e], o[e]);
-        }
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    const float inverse = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-    const int i = index / p.group;
-    const long long h = b.head * p.group + index - i * p.group;
-    T* dst = static_cast<T*>(p.out) + (at.row0 + i) * p.ld_out + h * D + lane * kWidth;
-#pragma unroll
-    for (int e = 0; e < kWidth; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = packed_of(o[e] * inverse, o[e + 1] * inverse, T());
-    if (p.lse != nullptr && lane == 0) p.lse[static_cast<long long>(at.row0 + i) * p.heads + h] = (top + log2f(sum)) * kLn2;
 }
 
 // ------------------------------------------------------------- host
@@ -524,7 +524,7 @@ static int cache_map(CUtensorMap* map, const void* base, const pk100_paged_atten
 struct PagedPlan {
     int grid;                                            // blocks of the few-row kernel
     int pairs, shares;                                   // of the other one
-    long long begins, parts, part_out, share_ml, share_out, bytes;
+    long long counts, parts, part_out, share_ml, share_out, bytes;
 };
 
 static long long round256(long long n) { return (n + 255) / 256 * 256; }
@@ -537,8 +537,8 @@ static PagedPlan paged_plan_of(const pk100_paged_attention_args& a) {
     const long long blocks = (static_cast<long long>(a.max_pages) * a.page_size + kBlock - 1) / kBlock;
     const long long most = 2ll * pk100_sm_count();
     plan.grid = static_cast<int>(tiles * a.kv_heads >= most || tiles * a.kv_heads * blocks >= most ? most : tiles * a.kv_heads * blocks);
-    plan.begins = 0;
-    plan.parts = round256(plan.grid * static_cast<long long>(sizeof(RowsBegin)));
+    plan.counts = 0;
+    plan.parts = round256(plan.grid * 4ll);
     plan.part_out = plan.parts + round256(2ll * plan.grid * static_cast<long long>(sizeof(RowsPart)));
     plan.share_ml = plan.part_out + round256(2ll * plan.grid * kRows * a.head_dim * 4);
     // Keys are shared out where the pairs of tiles leave SMs idle: few new tokens over a long cache.
@@ -574,13 +574,9 @@ static int launch_rows(const pk100_paged_attention_args& a, const PagedParams& p
     const cudaError_t granted = pk100_grant_smem<kernel>(bytes);
     if (granted != cudaSuccess) return static_cast<int>(granted);
     uint8_t* ws = static_cast<uint8_t*>(a.workspace);
-    RowsBegin* begins = reinterpret_cast<RowsBegin*>(ws + plan.begins);
     RowsPart* parts = reinterpret_cast<RowsPart*>(ws + plan.parts);
     float* part_out = reinterpret_cast<float*>(ws + plan.part_out);
-    pk100_launch_chained(kernel, dim3(plan.grid), dim3(kRowThreads), bytes, stream, map_k, map_v, p, begins, parts, part_out);
-    int rc = pk100_launch_status();
-    if (rc != PK100_OK || plan.grid == 1) return rc;
-    pk100_launch_chained(rows_join_kernel<T, D>, dim3(plan.grid - 1, kRows / 4), dim3(128), 0, stream, p, begins, parts, part_out);
+    pk100_launch_chained(kernel, dim3(plan.grid), dim3(kRowThreads), bytes, stream, map_k, map_v, p, reinterpret_cast<int*>(ws + plan.counts), parts, part_out);
     return pk100_launch_status();
 }
 
@@ -642,10 +638,15 @@ extern "C" int pk100_paged_attention(void* stream_v, const pk100_paged_attention
         w.page_stride = a->page_stride; w.token_stride = a->token_stride; w.head_stride = a->head_stride;
         w.tokens = a->tokens; w.kv_heads = a->kv_heads; w.head_dim = a->head_dim; w.page_shift = p.page_shift;
         w.capacity = static_cast<long long>(a->pages) * a->page_size;
+        w.counts = reinterpret_cast<int*>(static_cast<uint8_t*>(a->workspace) + plan.counts);
+        w.n_counts = plan.grid;
         w.status = a->status;
         const long long work = a->tokens * (kv_row / 8), blocks = (work + 255) / 256, most = 8ll * pk100_sm_count();
         pk100_launch_chained(paged_append_kernel, dim3(static_cast<int>(blocks < most ? blocks : most)), dim3(256), 0, stream, w);
         if ((rc = pk100_launch_status()) != PK100_OK) return rc;
+    } else {
+        const cudaError_t err = cudaMemsetAsync(static_cast<uint8_t*>(a->workspace) + plan.counts, 0, plan.grid * 4ull, stream);
+        if (err != cudaSuccess) return static_cast<int>(err);
     }
     if (a->type == PK100_TYPE_F16)
         rc = a->head_dim == 128 ? launch_rows<__half, 128>(*a, p, plan, map_k, map_v, stream) : launch_rows<__half, 64>(*a, p, plan, map_k, map_v, stream);

@@ -306,14 +306,32 @@ def _whole(name, t, shape, dtype, device):
 
 
 def _rows(name, t, shape, dtype, device):
-    """Address of [rows, ...] and elements between its rows, which are contiguous each."""
+    """Address of [rows, width] and elements between its rows."""
     if t.dtype is not dtype or t.get_device() != device or t.shape != shape:
         _refuse(name, t, shape, dtype, device)
     if t.is_contiguous():
-        return t.data_ptr(), math.prod(shape[1:])
-    if shape[0] and not t[0].is_contiguous():
+        return t.data_ptr(), shape[1]
+    step, inner = t.stride()
+    if inner != 1 and shape[1] > 1 and shape[0] > 0:
         _refuse(name, t, shape, dtype, device)
-    return t.data_ptr(), t.stride(0) if shape[0] > 1 else math.prod(shape[1:])
+    return t.data_ptr(), step if shape[0] > 1 else shape[1]           # (a single row's stride may be anything)
+
+
+def _heads(name, t, shape, dtype, device):
+    """Address of [tokens, heads, head_dim] and elements between its tokens."""
+    if t.dtype is not dtype or t.get_device() != device or t.shape != shape:
+        _refuse(name, t, shape, dtype, device)
+    tokens, heads, dim = shape
+    if t.is_contiguous():
+        return t.data_ptr(), heads * dim
+    step, head, inner = t.stride()
+    if (inner != 1 or (head != dim and heads > 1)) and tokens > 0:
+        _refuse(name, t, shape, dtype, device)
+    return t.data_ptr(), step if tokens > 1 else heads * dim
+
+
+def _stream_of(device):
+    return _stream() if _raw_stream is None else _raw_stream(device)
 
 
 def _out_dtype(mode, dtype):
@@ -350,7 +368,7 @@ def add_rms_norm(x, gamma, residual=None, mode=L.LN_F16, inv_scale=0.0, eps=EPS,
         scales_at = _whole("scales", scales, (rows,), torch.float32, device)
     else:
         scales = None
-    rc = _add_rms_norm(_stream(), _RMS_NORM_ARGS.pack(kind, mode, rows, width, x_at, x_ld, res_at, res_ld, kept_at, kept_ld, gamma_at, eps,
+    rc = _add_rms_norm(_stream_of(device), _RMS_NORM_ARGS.pack(kind, mode, rows, width, x_at, x_ld, res_at, res_ld, kept_at, kept_ld, gamma_at, eps,
                                                       inv_scale, out_at, out_ld, scales_at))
     L.check(rc, "pk100_add_rms_norm")
     return out, scales, x if residual_out is None else residual_out
@@ -372,7 +390,7 @@ def gemv_w4g128(a, codes, group_scales, *, out=None, row_scales=None, row_scale=
     rows_at = 0 if row_scales is None else _whole("row_scales", row_scales, (m,), torch.float32, device)
     cols_at = 0 if col_scales is None else _whole("col_scales", col_scales, (n,), torch.float32, device)
     bias_at = 0 if bias is None else _whole("bias", bias, (n,), torch.float32, device)
-    rc = _gemv_w4g128(_stream(), _GEMM_ARGS.pack(
+    rc = _gemv_w4g128(_stream_of(device), _GEMM_ARGS.pack(
         L.KIND_F16_W4G128, L.EPI_LINEAR, m, n, k, a_at, a_ld, codes_at, k // 2, rows_at, row_scale, cols_at, bias_at, act, res_at, res_ld, alpha,
         valid_rows, out_at, out_ld, out_type, 1.0, 0.0, 0, 0, 0, 0, 0, groups_at))
     L.check(rc, "pk100_gemv_w4g128")
@@ -398,7 +416,7 @@ def paged_plan(cached, new_tokens, block_table, free_pages, free_count, *, token
     status_at = 0 if status is None else _whole("status", status, (1,), i32, device)
     if out is None:
         words = torch.empty(2 * requests + 2 + tokens, device=block_table.device, dtype=i32)
-        starts, lengths, positions, used = words.split([requests + 1, requests, tokens, 1])
+        starts, lengths, positions, used = words.split_with_sizes((requests + 1, requests, tokens, 1))
         slots = torch.empty(tokens, device=block_table.device, dtype=torch.int64)
         out = PagedPlan(starts, lengths, positions, slots, used)
         at = words.data_ptr()
@@ -410,7 +428,7 @@ def paged_plan(cached, new_tokens, block_table, free_pages, free_count, *, token
         positions_at = _whole("positions", out.positions, (tokens,), i32, device)
         slots_at = _whole("slots", out.slots, (tokens,), torch.int64, device)
         used_at = _whole("used", out.used, (1,), i32, device)
-    rc = _paged_plan(_stream(), _PAGED_PLAN_ARGS.pack(requests, tokens, page_size, max_pages, cached_at, new_at, free_at, count_at, table_at, starts_at,
+    rc = _paged_plan(_stream_of(device), _PAGED_PLAN_ARGS.pack(requests, tokens, page_size, max_pages, cached_at, new_at, free_at, count_at, table_at, starts_at,
                                                       lengths_at, positions_at, slots_at, used_at, status_at))
     L.check(rc, "pk100_paged_plan")
     return out
@@ -442,7 +460,7 @@ def paged_attention(query, key_cache, value_cache, block_table, starts, lengths,
     tokens, heads, head_dim = shape
     pages, page_size, kv_heads, _ = cache_shape = key_cache.shape
     requests, max_pages = table_shape = block_table.shape
-    query_at, query_ld = _rows("query", query, shape, dtype, device)
+    query_at, query_ld = _heads("query", query, shape, dtype, device)
     strides = key_cache.stride()
     for name, t in (("key_cache", key_cache), ("value_cache", value_cache)):
         if t.dtype is not dtype or t.get_device() != device or t.shape != cache_shape or cache_shape[3] != head_dim or strides[3] != 1:
@@ -457,14 +475,14 @@ def paged_attention(query, key_cache, value_cache, block_table, starts, lengths,
         if value is None or slots is None:
             raise ValueError("key needs value and slots")
         new_shape = (tokens, kv_heads, head_dim)
-        key_at, key_ld = _rows("key", key, new_shape, dtype, device)
-        value_at, value_ld = _rows("value", value, new_shape, dtype, device)
+        key_at, key_ld = _heads("key", key, new_shape, dtype, device)
+        value_at, value_ld = _heads("value", value, new_shape, dtype, device)
         slots_at = _whole("slots", slots, (tokens,), torch.int64, device)
     if heads % kv_heads:
         raise ValueError(f"{heads} query heads do not share {kv_heads} key-value heads evenly")
     if out is None:
         out = torch.empty(shape, device=query.device, dtype=dtype)
-    out_at, out_ld = _rows("out", out, shape, dtype, device)
+    out_at, out_ld = _heads("out", out, shape, dtype, device)
     lse_at = 0 if lse is None else _whole("lse", lse, (tokens, heads), torch.float32, device)
     status_at = 0 if status is None else _whole("status", status, (1,), i32, device)
     if workspace is None:
@@ -473,7 +491,7 @@ def paged_attention(query, key_cache, value_cache, block_table, starts, lengths,
     else:
         need = workspace.numel()
         _whole("workspace", workspace, (need,), torch.uint8, device)
-    rc = _paged_attention(_stream(), _PAGED_ATTENTION_ARGS.pack(
+    rc = _paged_attention(_stream_of(device), _PAGED_ATTENTION_ARGS.pack(
         kind, tokens, requests, heads, kv_heads, head_dim, pages, page_size, max_pages, query_at, query_ld, key_at, key_ld, value_at, value_ld,
         slots_at, key_cache.data_ptr(), value_cache.data_ptr(), strides[0], strides[1], strides[2], starts_at, lengths_at, table_at, int(causal),
         min(window, 1 << 30), min(max_new, 1 << 30), head_dim ** -0.5 if scale is None else scale, out_at, out_ld, lse_at,

@@ -469,6 +469,20 @@ def test_attention_captured_and_replayed_on_other_lengths(pk, cuda):
         s.check(out)
 
 
+def test_attention_captured_without_new_keys(pk, cuda):
+    s = Step([1, 300], [3000, 40], 8, 2, 128, 16, F16)
+    want = s.run(pk).clone()
+    out = torch.empty_like(want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s.run(pk, key=None, value=None, slots=None, out=out)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
 def test_calls_on_two_streams_at_once(pk, cuda):
     steps = [Step([1] * 8, [800 + 100 * i] * 8, 8, 2, 128, 16, F16, seed=i) for i in range(2)]
     want = [s.run(pk).clone() for s in steps]
