@@ -32,10 +32,10 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int column, int width,
 // A row belongs to a warp (8 rows a block) or to a whole block; every thread keeps Chunks x 8 of its elements, so
 // the row is read once.  Mean square and max |s * gamma| leave in ONE reduction: max |y| = rstd * max |s * gamma|.
 // Sums are fp32 in a fixed order.  The codes are formed from the fp32 y: rounding it to 16 bits first would cost
-// bf16 rows a bit of their 7-bit codes.  Bound by HBM for many rows, by the latency of load, reduction and store
-// for a few.
-template <typename T, int Mode, int Chunks>
-__global__ void __launch_bounds__(1024)
+// bf16 rows a bit of their 7-bit codes.  Bound by HBM for many rows (16 384 x 4096 bf16 to E4M3, 470 MB: 79 us, 5.9 TB/s),
+// by the latency of load, reduction and store for a few.
+template <typename T, int Mode, int Chunks, int Block>
+__global__ void __launch_bounds__(Block, 1024 / Block)
 add_rms_norm_kernel(const RmsNormParams p) {
     __shared__ float part_sum[32], part_max[32];
     grid_dependents_launch();
@@ -45,7 +45,7 @@ add_rms_norm_kernel(const RmsNormParams p) {
     if (row >= p.rows) return;                          // (whole warps; blocks of one row have none)
     const T* in = static_cast<const T*>(p.input) + row * p.ld_in;
     const T* gamma = static_cast<const T*>(p.gamma);
-    uint4 s[Chunks], g[Chunks];
+    uint4 s[Chunks];
 #pragma unroll
     for (int c = 0; c < Chunks; ++c) s[c] = load8(in, (c * p.threads + t) * 8, p.width, p.vec_in);
     if (p.residual != nullptr) {
@@ -69,14 +69,13 @@ add_rms_norm_kernel(const RmsNormParams p) {
 #pragma unroll
         for (int c = 0; c < Chunks; ++c) store8(o, (c * p.threads + t) * 8, p.width, p.vec_res_out, s[c]);
     }
-#pragma unroll
-    for (int c = 0; c < Chunks; ++c) g[c] = load8(gamma, (c * p.threads + t) * 8, p.width, p.vec_gamma);
     constexpr bool kRowScale = Mode == PK100_LN_E4M3_ROW || Mode == PK100_LN_S8_ROW;
     float sum = 0.0f, top = 0.0f;
 #pragma unroll
     for (int c = 0; c < Chunks; ++c) {
         const uint32_t* a = reinterpret_cast<const uint32_t*>(&s[c]);
-        const uint32_t* b = reinterpret_cast<const uint32_t*>(&g[c]);
+        const uint4 g = kRowScale ? load8(gamma, (c * p.threads + t) * 8, p.width, p.vec_gamma) : make_uint4(0, 0, 0, 0);
+        const uint32_t* b = reinterpret_cast<const uint32_t*>(&g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 x = floats_of(a[i], T());
@@ -122,7 +121,8 @@ add_rms_norm_kernel(const RmsNormParams p) {
     for (int c = 0; c < Chunks; ++c) {
         const int column = (c * p.threads + t) * 8;
         const uint32_t* a = reinterpret_cast<const uint32_t*>(&s[c]);
-        const uint32_t* b = reinterpret_cast<const uint32_t*>(&g[c]);
+        const uint4 g = load8(gamma, column, p.width, p.vec_gamma);        // (again, from the L1: registers are blocks in flight)
+        const uint32_t* b = reinterpret_cast<const uint32_t*>(&g);
         float y[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -156,9 +156,10 @@ add_rms_norm_kernel(const RmsNormParams p) {
 
 template <typename T, int Mode>
 static void launch_rms_norm(const RmsNormParams& p, int chunks, int blocks, int block, cudaStream_t stream) {
-    if (chunks == 1) pk100_launch_chained(add_rms_norm_kernel<T, Mode, 1>, dim3(blocks), dim3(block), 0, stream, p);
-    else if (chunks == 2) pk100_launch_chained(add_rms_norm_kernel<T, Mode, 2>, dim3(blocks), dim3(block), 0, stream, p);
-    else pk100_launch_chained(add_rms_norm_kernel<T, Mode, 4>, dim3(blocks), dim3(block), 0, stream, p);
+    if (chunks == 1) pk100_launch_chained(add_rms_norm_kernel<T, Mode, 1, 1024>, dim3(blocks), dim3(block), 0, stream, p);
+    else if (chunks == 2) pk100_launch_chained(add_rms_norm_kernel<T, Mode, 2, 1024>, dim3(blocks), dim3(block), 0, stream, p);
+    else if (block <= 256) pk100_launch_chained(add_rms_norm_kernel<T, Mode, 4, 256>, dim3(blocks), dim3(block), 0, stream, p);
+    else pk100_launch_chained(add_rms_norm_kernel<T, Mode, 4, 1024>, dim3(blocks), dim3(block), 0, stream, p);
 }
 
 template <typename T>
@@ -206,12 +207,13 @@ extern "C" int pk100_add_rms_norm(void* stream, const pk100_rms_norm_args* a) {
     p.vec_res_out = vec(a->residual_out, a->ld_res_out, 16);
     p.vec_gamma = vec(a->gamma, 8, 16);
     p.vec_out = vec(a->output, a->ld_out, a->mode == PK100_LN_F16 ? 16 : 8);
-    // Few rows: one chunk a thread, the shortest chain.  Many: two chunks in flight a thread.  A row that 32
-    // threads hold goes to a warp, without the exchange through shared memory.
+    // As few chunks a thread as have all rows resident at once, the shortest chain (777 x 2560: 5.1 us with two, 7.3 with four);
+    // more rows: four in flight a thread (16 384 x 4096 in 79 us; two: 91 to 128, eight: 117).  A row that 32 threads hold
+    // goes to a warp, without the exchange through shared memory.
     const int need = (a->width + 7) / 8;
-    const bool many = a->rows > 4 * pk100_sm_count();
-    int chunks = many ? 2 : 1;
-    if (need <= 32) chunks = 1;
+    int chunks = 1;
+    while (chunks < 4 && static_cast<long long>(a->rows) * ((need + chunks - 1) / chunks) > 1536ll * pk100_sm_count()) chunks *= 2;
+    while (chunks > 1 && need <= 16 * chunks) chunks /= 2;             // (half of them would do for a warp)
     while (chunks < 4 && (need + chunks - 1) / chunks > 1024) chunks *= 2;
     p.threads = ((need + chunks - 1) / chunks + 31) / 32 * 32;
     const int block = p.threads == 32 ? 256 : p.threads;
