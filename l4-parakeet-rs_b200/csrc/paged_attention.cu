@@ -180,7 +180,7 @@ __device__ __forceinline__ void join_row(const PagedParams& p, const PagedReques
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads, 2)
 paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p,
-                            int* counts, RowsPart* parts, float* part_out) {
+                            const bool beside, int* counts, RowsPart* parts, float* part_out) {
     extern __shared__ uint8_t rows_raw[];
     constexpr int kStages = rows_stages<D>(), kHalves = D / 64;
     RowsSmem<D>& sm = *reinterpret_cast<RowsSmem<D>*>((reinterpret_cast<uintptr_t>(rows_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -198,7 +198,10 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
         prefetch_tensormap(&map_k);
         prefetch_tensormap(&map_v);
     }
-    grid_dependency_wait();
+    // beside: the chunk kernel is in front.  It lets this one start when all that stands before it is complete, and the
+    // two have nothing to do with each other: this one runs where that leaves SMs free and waits for it at its end, so
+    // that what comes behind finds both complete.
+    if (!beside) grid_dependency_wait();
 
     // this block's units: where the requests' prefix sum crosses them
     const int each = (p.requests + kRowThreads - 1) / kRowThreads, r0 = min(tid * each, p.requests), r1 = min(r0 + each, p.requests);
@@ -481,6 +484,7 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
             }
         });
     }
+    if (beside) grid_dependency_wait();
 }
 
 // ------------------------------------------------------------- host
@@ -568,7 +572,7 @@ static int paged_check(const pk100_paged_attention_args* a) {
 
 template <typename T, int D>
 static int launch_rows(const pk100_paged_attention_args& a, const PagedParams& p, const PagedPlan& plan, const CUtensorMap& map_k,
-                       const CUtensorMap& map_v, cudaStream_t stream) {
+                       const CUtensorMap& map_v, bool beside, cudaStream_t stream) {
     constexpr auto kernel = paged_attention_rows_kernel<T, D>;
     constexpr int bytes = sizeof(RowsSmem<D>) + 1024;
     const cudaError_t granted = pk100_grant_smem<kernel>(bytes);
@@ -576,7 +580,8 @@ static int launch_rows(const pk100_paged_attention_args& a, const PagedParams& p
     uint8_t* ws = static_cast<uint8_t*>(a.workspace);
     RowsPart* parts = reinterpret_cast<RowsPart*>(ws + plan.parts);
     float* part_out = reinterpret_cast<float*>(ws + plan.part_out);
-    pk100_launch_chained(kernel, dim3(plan.grid), dim3(kRowThreads), bytes, stream, map_k, map_v, p, reinterpret_cast<int*>(ws + plan.counts), parts, part_out);
+    pk100_launch_chained(kernel, dim3(plan.grid), dim3(kRowThreads), bytes, stream, map_k, map_v, p, beside, reinterpret_cast<int*>(ws + plan.counts),
+                         parts, part_out);
     return pk100_launch_status();
 }
 
@@ -648,13 +653,15 @@ extern "C" int pk100_paged_attention(void* stream_v, const pk100_paged_attention
         const cudaError_t err = cudaMemsetAsync(static_cast<uint8_t*>(a->workspace) + plan.counts, 0, plan.grid * 4ull, stream);
         if (err != cudaSuccess) return static_cast<int>(err);
     }
-    if (a->type == PK100_TYPE_F16)
-        rc = a->head_dim == 128 ? launch_rows<__half, 128>(*a, p, plan, map_k, map_v, stream) : launch_rows<__half, 64>(*a, p, plan, map_k, map_v, stream);
-    else
-        rc = a->head_dim == 128 ? launch_rows<__nv_bfloat16, 128>(*a, p, plan, map_k, map_v, stream)
-                                : launch_rows<__nv_bfloat16, 64>(*a, p, plan, map_k, map_v, stream);
-    if (rc != PK100_OK || !many) return rc;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-    return paged_attention_chunks(a->type, a->head_dim, p, map_k, map_v, plan.pairs, plan.shares, reinterpret_cast<float2*>(ws + plan.share_ml),
-                                  reinterpret_cast<float*>(ws + plan.share_out), stream);
+    float2* share_ml = reinterpret_cast<float2*>(ws + plan.share_ml);
+    float* share_out = reinterpret_cast<float*>(ws + plan.share_out);
+    if (many && (rc = paged_attention_chunks(a->type, a->head_dim, p, map_k, map_v, plan.pairs, plan.shares, share_ml, share_out, stream)) != PK100_OK) return rc;
+    if (a->type == PK100_TYPE_F16)
+        rc = a->head_dim == 128 ? launch_rows<__half, 128>(*a, p, plan, map_k, map_v, many, stream) : launch_rows<__half, 64>(*a, p, plan, map_k, map_v, many, stream);
+    else
+        rc = a->head_dim == 128 ? launch_rows<__nv_bfloat16, 128>(*a, p, plan, map_k, map_v, many, stream)
+                                : launch_rows<__nv_bfloat16, 64>(*a, p, plan, map_k, map_v, many, stream);
+    if (rc != PK100_OK || !many || plan.shares == 1) return rc;
+    return paged_attention_join(a->type, a->head_dim, p, plan.shares, share_ml, share_out, stream);
 }

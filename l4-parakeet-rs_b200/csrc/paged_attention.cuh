@@ -59,5 +59,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 constexpr int kPairRows = 256;
 int paged_attention_chunks(int type, int head_dim, const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares,
                            float2* part_ml, float* part_out, cudaStream_t stream);
+// Adds the shares up.
+int paged_attention_join(int type, int head_dim, const PagedParams& p, int shares, const float2* part_ml, const float* part_out, cudaStream_t stream);
 
 }  // namespace pk100

@@ -36,8 +36,14 @@ __device__ __forceinline__ void mma_from_tmem(bool leader, uint32_t d, uint32_t 
                  ::"r"(d), "r"(a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(static_cast<uint32_t>(leader)) : "memory");
 }
 
-// 2^x for two values at most 9: n = rint(x), a polynomial of the remainder (minimax of the relative error, degree 4: 2.7e-6,
-// far below the rounding of P), n into the exponent.  x below -126 counts as -126.  On the FMA pipe, where
+__device__ __forceinline__ float max_of(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// 2^x for two values at most 9: n = rint(x), a polynomial of the remainder (minimax of the relative error, degree 3: 7.5e-5,
+// a sixth of half a step of an fp16 P), n into the exponent.  x below -126 counts as -126.  On the FMA pipe, where
 // ex2.approx (16 a clock and SM) would take as long as the tensor cores' products.
 __device__ __forceinline__ Pair exp2_fma(Pair x) {
     const float2 v = halves_of(x);
@@ -45,10 +51,9 @@ __device__ __forceinline__ Pair exp2_fma(Pair x) {
     const Pair magic = pair_of(12582912.0f, 12582912.0f), back = pair_of(-12582912.0f, -12582912.0f);       // 1.5 * 2^23
     const Pair n = pair_add(x, magic);
     const Pair r = pair_fma(pair_add(n, back), pair_of(-1.0f, -1.0f), x);
-    Pair y = pair_fma(r, pair_of(0.009570102207362652f, 0.009570102207362652f), pair_of(0.05591785907745361f, 0.05591785907745361f));
-    y = pair_fma(r, y, pair_of(0.240247443318367f, 0.240247443318367f));
-    y = pair_fma(r, y, pair_of(0.6931217908859253f, 0.6931217908859253f));
-    y = pair_fma(r, y, pair_of(0.9999992847442627f, 0.9999992847442627f));
+    Pair y = pair_fma(r, pair_of(0.0551716685295105f, 0.0551716685295105f), pair_of(0.2426111251115799f, 0.2426111251115799f));
+    y = pair_fma(r, y, pair_of(0.6932609677314758f, 0.6932609677314758f));
+    y = pair_fma(r, y, pair_of(0.9999280571937561f, 0.9999280571937561f));
     const float2 whole = halves_of(n), part = halves_of(y);
     return pair_of(__uint_as_float(__float_as_uint(part.x) + (__float_as_uint(whole.x) << 23)),
                    __uint_as_float(__float_as_uint(part.y) + (__float_as_uint(whole.y) << 23)));
@@ -154,7 +159,6 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
     constexpr int kHalves = D / 64, kSlots = ring_slots<D>(), kSlotBytes = kHalves * kAtom;
     Smem<D>& sm = *reinterpret_cast<Smem<D>*>(chunk_raw);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
-    grid_dependents_launch();
     volatile int* abort_flag = &sm.abort;
     if (tid == 0) {
         sm.abort = 0;
@@ -181,6 +185,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
     tc_fence_after_sync();
     const uint32_t tmem = sm.tmem;
     grid_dependency_wait();
+    grid_dependents_launch();                   // (only now: the few-row kernel behind this one does not wait for what is in front of it)
 
     // the last pairs of a request see the most keys: they go first
     const int head = blockIdx.x % p.kv_heads, share = blockIdx.x / p.kv_heads % shares, pair = pairs - 1 - blockIdx.x / p.kv_heads / shares;
@@ -373,10 +378,10 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             }
             float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int i = 4; i < 64; i += 4)
+            for (int i = 4; i < 60; i += 8)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], s[i + j]);
-            const float own = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                for (int j = 0; j < 4; ++j) top[j] = max_of(top[j], s[i + 2 * j], s[i + 2 * j + 1]);
+            const float own = max_of(max_of(top[0], s[60], s[61]), max_of(top[1], s[62], s[63]), fmaxf(top[2], top[3]));
             sm.top[t][half][tile_row] = own;                 // (the partner has read the last one: S of this block came after its P)
             pair_sync();                                     // (also: both halves of S have been read, P may take their place)
             const float seen = fmaxf(m, fmaxf(own, sm.top[t][half ^ 1][tile_row]));
@@ -512,8 +517,11 @@ static int launch(const PagedParams& p, const CUtensorMap& map_k, const CUtensor
     if (granted != cudaSuccess) return static_cast<int>(granted);
     pk100_launch_chained(kernel, dim3(static_cast<unsigned>(pairs) * shares * p.kv_heads), dim3(kThreads), bytes, stream, map_k, map_v, p, pairs, shares,
                          part_ml, part_out);
-    const int rc = pk100_launch_status();
-    if (rc != PK100_OK || shares == 1) return rc;
+    return pk100_launch_status();
+}
+
+template <typename T, int D>
+static int launch_join(const PagedParams& p, int shares, const float2* part_ml, const float* part_out, cudaStream_t stream) {
     pk100_launch_chained(shares_join_kernel<T, D>, dim3(p.tokens, (p.heads + 3) / 4 < 8 ? (p.heads + 3) / 4 : 8), dim3(128), 0, stream, p, shares, part_ml, part_out);
     return pk100_launch_status();
 }
@@ -527,6 +535,13 @@ int paged_attention_chunks(int type, int head_dim, const PagedParams& p, const C
                                : chunk::launch<__half, 64>(p, map_k, map_v, pairs, shares, part_ml, part_out, stream);
     return head_dim == 128 ? chunk::launch<__nv_bfloat16, 128>(p, map_k, map_v, pairs, shares, part_ml, part_out, stream)
                            : chunk::launch<__nv_bfloat16, 64>(p, map_k, map_v, pairs, shares, part_ml, part_out, stream);
+}
+
+int paged_attention_join(int type, int head_dim, const PagedParams& p, int shares, const float2* part_ml, const float* part_out, cudaStream_t stream) {
+    if (type == PK100_TYPE_F16)
+        return head_dim == 128 ? chunk::launch_join<__half, 128>(p, shares, part_ml, part_out, stream) : chunk::launch_join<__half, 64>(p, shares, part_ml, part_out, stream);
+    return head_dim == 128 ? chunk::launch_join<__nv_bfloat16, 128>(p, shares, part_ml, part_out, stream)
+                           : chunk::launch_join<__nv_bfloat16, 64>(p, shares, part_ml, part_out, stream);
 }
 
 }  // namespace pk100
