@@ -546,10 +546,11 @@ static PagedPlan paged_plan_of(const pk100_paged_attention_args& a) {
     plan.part_out = plan.parts + round256(2ll * plan.grid * static_cast<long long>(sizeof(RowsPart)));
     plan.share_ml = plan.part_out + round256(2ll * plan.grid * kRows * a.head_dim * 4);
     // Keys are shared out where the pairs of tiles leave SMs idle: few new tokens over a long cache.
-    const long long rows = static_cast<long long>(a.tokens) * group, items = (rows + kPairRows - 1) / kPairRows * a.kv_heads;
-    plan.pairs = static_cast<int>(rows / kPairRows) + a.requests;
+    const long long rows = static_cast<long long>(a.tokens) * group, each = pair_rows(a.head_dim);
+    const long long items = (rows + each - 1) / each * a.kv_heads;
+    plan.pairs = static_cast<int>(rows / each) + a.requests;
     const long long by_keys = blocks / 8;                // 512 keys a share at least
-    long long shares = items > 0 ? pk100_sm_count() / items : 1;
+    long long shares = items > 0 ? pk100_sm_count() * (256 / each) / items : 1;      // (two blocks of one tile an SM)
     if (shares > by_keys) shares = by_keys;
     plan.shares = shares < 1 ? 1 : static_cast<int>(shares);
     const long long share_rows = plan.shares > 1 ? static_cast<long long>(plan.shares) * a.tokens * a.heads : 0;

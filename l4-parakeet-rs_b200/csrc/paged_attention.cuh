@@ -53,10 +53,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-// The kernel for requests of more than p.few_rows rows (paged_attention_tcgen05.cu): `pairs` numbers of 256-row pairs
-// of tiles (tokens * group / 256 + requests), `shares` parts of a row's keys; part_ml [shares, tokens, heads] and
+// The kernel for requests of more than p.few_rows rows (paged_attention_tcgen05.cu): `pairs` numbers of pairs of tiles
+// (tokens * group / pair_rows + requests), `shares` parts of a row's keys; part_ml [shares, tokens, heads] and
 // part_out [shares, tokens, heads, head_dim] where shares > 1.
-constexpr int kPairRows = 256;
+constexpr int pair_rows(int head_dim) { return head_dim == 128 ? 256 : 128; }
 int paged_attention_chunks(int type, int head_dim, const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares,
                            float2* part_ml, float* part_out, cudaStream_t stream);
 // Adds the shares up.

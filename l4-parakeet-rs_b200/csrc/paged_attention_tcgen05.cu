@@ -5,18 +5,21 @@ namespace pk100 {
 namespace chunk {
 
 constexpr int kTile = 128;                      // (token, head) rows of an accumulator, and keys of a block
-constexpr int kTiles = 2;                       // tiles of a block of threads: one's softmax runs under the other's products
 constexpr int kTileWarps = 8;                   // softmax warps of a tile: four lane quadrants, two halves of the keys
-constexpr int kSoftmaxWarps = kTileWarps * kTiles;
-constexpr int kThreads = kSoftmaxWarps * 32 + 64;
+// Tiles of a block of threads.  Two, so that one's softmax runs under the other's products; of 64 features two blocks with a
+// tile each fit an SM, which also covers one's beginning and end with the other's work.
+template <int D> constexpr int tiles() { return D == 128 ? 2 : 1; }
+template <int D> constexpr int softmax_warps() { return kTileWarps * tiles<D>(); }
+template <int D> constexpr int threads() { return softmax_warps<D>() * 32 + 64; }
 constexpr int kAtom = kTile * 128;              // 128 rows x 64 elements, 128-byte swizzle
 constexpr int kBox = 64;                        // most keys of a TMA box
 constexpr int kByFma = 4;                       // of 16 pairs of scores, whose exponentials the FMA pipe forms
 
-template <int D> constexpr int ring_slots() { return D == 128 ? 5 : 8; }
+template <int D> constexpr int ring_slots() { return 5; }
 
 template <int D>
 struct Smem {
+    static constexpr int kTiles = tiles<D>();
     uint8_t q[kTiles][D / 64][kAtom];
     uint8_t ring[ring_slots<D>()][D / 64][kAtom];          // key and value blocks in turn
     uint64_t full[ring_slots<D>()], empty[ring_slots<D>()];
@@ -89,6 +92,7 @@ __device__ __forceinline__ float weights_of_scores(const float (&s)[64], float s
 }
 
 // What a block of threads works on: 256 rows of one request and key-value head, over a share of their keys.
+template <int kTiles>
 struct Work {
     PagedRequest at;
     int request, head, row, rows;               // first row of the first tile inside the request; rows of both tiles that exist
@@ -114,8 +118,9 @@ struct Work {
     }
 };
 
-// Pairs of tiles are numbered over the batch with gaps: request r begins at floor(first row / 256) + r, which leaves
-// room for its last, partial pair.  The last request that begins at or before `pair`, found 32 candidates at a time.
+// Pairs of tiles are numbered over the batch with gaps: request r begins at floor(first row / rows of a pair) + r, which leaves
+// room for its last, partial one (pairs of one tile where D is 64).  The last request that begins at or before `pair`, found 32 candidates at a time.
+template <int kTiles>
 __device__ __forceinline__ int request_of(const PagedParams& p, int pair, int& begin) {
     const int lane = threadIdx.x % 32;
     int lo = 0, hi = p.requests;                 // begin(lo) <= pair < begin(hi)
@@ -152,11 +157,12 @@ __device__ __forceinline__ int request_of(const PagedParams& p, int pair, int& b
 // Two prompts of 7.2 k tokens, 16 / 4 heads of 128: 494 us, 870 TFLOP/s (the few-row kernel in the same place: 4.6 ms); 512 tokens over
 // 32 000, 16 / 2 heads: 159 us, 840 TFLOP/s (764 us).
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(threads<D>(), 3 - tiles<D>())
 paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p,
                              const int pairs, const int shares, float2* __restrict__ part_ml, float* __restrict__ part_out) {
     extern __shared__ __align__(1024) uint8_t chunk_raw[];             // (the swizzled atoms need it)
-    constexpr int kHalves = D / 64, kSlots = ring_slots<D>(), kSlotBytes = kHalves * kAtom;
+    constexpr int kHalves = D / 64, kSlots = ring_slots<D>(), kSlotBytes = kHalves * kAtom, kTiles = tiles<D>(), kSoftmaxWarps = softmax_warps<D>();
+    constexpr uint32_t kColumns = 256 * kTiles;                 // of tensor memory: S and O of the tiles
     Smem<D>& sm = *reinterpret_cast<Smem<D>*>(chunk_raw);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
     volatile int* abort_flag = &sm.abort;
@@ -177,7 +183,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         prefetch_tensormap(&map_v);
     }
     if (warp == kSoftmaxWarps + 1) {
-        tmem_alloc(&sm.tmem, 512);
+        tmem_alloc(&sm.tmem, kColumns);
         tmem_relinquish();
     }
     tc_fence_before_sync();
@@ -190,8 +196,8 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
     // the last pairs of a request see the most keys: they go first
     const int head = blockIdx.x % p.kv_heads, share = blockIdx.x / p.kv_heads % shares, pair = pairs - 1 - blockIdx.x / p.kv_heads / shares;
     int begin;
-    const int request = request_of(p, pair, begin);
-    Work w(p, request, head, pair - begin);
+    const int request = request_of<kTiles>(p, pair, begin);
+    Work<kTiles> w(p, request, head, pair - begin);
     const bool mine = pair >= begin && w.rows > 0 && w.at.n * p.group > p.few_rows;
     const int blocks = w.to - w.from;
     // a share is two blocks of keys at least
@@ -255,7 +261,12 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                                 (64ull << 32) | (1ull << 46) | (2ull << 61);
         auto k_offset = [](int ks) { return static_cast<uint32_t>((ks / 4) * (kAtom / 16) + 2 * (ks % 4)); };
         const bool leader = elect_one();
-        const int tile_from[kTiles] = {w.tile_from(p, 0), w.tile_from(p, 1)}, tile_to[kTiles] = {w.tile_to(p, 0), w.tile_to(p, 1)};
+        int tile_from[kTiles], tile_to[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            tile_from[t] = w.tile_from(p, t);
+            tile_to[t] = w.tile_to(p, t);
+        }
         auto active = [&](int t, int b) { return b >= tile_from[t] && b < tile_to[t]; };
         auto scores = [&](int t, int slot) {
 #pragma unroll
@@ -264,8 +275,8 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                                     idesc_s, ks > 0);
             tc_commit_if(leader, &sm.s_full[t]);
         };
-        uint32_t phase[kTiles] = {0, 0};                     // parity of the tile's next block
-        uint32_t filled[kTiles] = {0, 0};                    // O holds something
+        uint32_t phase[kTiles] = {};                     // parity of the tile's next block
+        uint32_t filled[kTiles] = {};                    // O holds something
         int it = 0;                                          // ring position of the block's keys; its values follow
         do {
             if (w.from >= w.to) break;
@@ -460,7 +471,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
     if (!ok && lane == 0 && p.status != nullptr) atomicOr(p.status, 1);
     tc_fence_before_sync();
     __syncthreads();
-    if (warp == kSoftmaxWarps + 1) tmem_dealloc(tmem, 512);
+    if (warp == kSoftmaxWarps + 1) tmem_dealloc(tmem, kColumns);
 }
 
 // out of the shares of a row's keys, in their order, a warp a row.
@@ -512,10 +523,10 @@ static int launch(const PagedParams& p, const CUtensorMap& map_k, const CUtensor
                   float* part_out, cudaStream_t stream) {
     constexpr auto kernel = paged_attention_chunk_kernel<T, D>;
     constexpr int bytes = sizeof(Smem<D>);
-    static_assert(bytes <= 227 * 1024, "shared memory");
+    static_assert(bytes <= 227 * 1024 / (3 - tiles<D>()) - (D == 64 ? 1024 : 0), "shared memory");
     const cudaError_t granted = pk100_grant_smem<kernel>(bytes);
     if (granted != cudaSuccess) return static_cast<int>(granted);
-    pk100_launch_chained(kernel, dim3(static_cast<unsigned>(pairs) * shares * p.kv_heads), dim3(kThreads), bytes, stream, map_k, map_v, p, pairs, shares,
+    pk100_launch_chained(kernel, dim3(static_cast<unsigned>(pairs) * shares * p.kv_heads), dim3(threads<D>()), bytes, stream, map_k, map_v, p, pairs, shares,
                          part_ml, part_out);
     return pk100_launch_status();
 }
