@@ -670,7 +670,7 @@ int pk100_add_rms_norm(void* stream, const pk100_rms_norm_args* args);
  * weights' bytes and pk100_gemm's tiles are mostly padding: the same arguments, weights W = f16(code * scale) and
  * epilogue algebra, fp32 sums (in another order than pk100_gemm's).  Any n; k % 128 == 0; a and b 16-byte
  * aligned, lda % 8 == 0; out and residual of any leading dimension; PK100_EPI_LINEAR; out_type PK100_OUT_F16 or
- * _F32.  More than 16 rows: PK100_ERR_LIMIT.  tau, keep_*, stats_out, status and max_ctas are not read. */
+ * _F32.  More than 16 rows: PK100_ERR_LIMIT.  tau, keep_*, stats_out and max_ctas are not read. */
 int pk100_gemv_w4g128(void* stream, const pk100_gemm_args* args);
 
 /* One step's bookkeeping of a paged key-value cache, from the request lengths alone:

@@ -1,29 +1,13 @@
 // Products of a few rows with INT4 group-128 weights: D[m, n] = epilogue(A[m, k] . W[n, k]^T), W = f16(code * scale),
 // m <= 16.
-#include <cuda_fp16.h>
-
 #include <type_traits>
 
-#include "pk100_internal.h"
+#include "gemv_w4.cuh"
 #include "ptx_sm100.cuh"
 
 namespace pk100 {
 
-constexpr int kGroup = 128;
 constexpr int kGemvWarps = 12, kGemvThreads = kGemvWarps * 32;
-
-struct GemvParams {
-    int m, n, k;
-    const __half* a; long long lda;
-    const uint8_t* codes;             // [n, k / 2]
-    const __half* group_scales;       // [k / 128, n]
-    const float* row_scales; float row_scale;
-    const float* col_scales; const float* bias;
-    int act;
-    const __half* residual; long long ld_res;
-    float alpha; int valid_rows;
-    void* out; long long ld_out; int out_type;
-};
 
 __device__ __forceinline__ void cp_async_16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -39,36 +23,7 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// 8 codes of a word -> 4 pairs of weights f16(code * scale), pair i = codes (i, i + 4).  With its sign bit flipped a code
-// is code + 8; in the low mantissa bits behind the exponent of 1024 it is 1024 + code + 8, four bits higher 1024 +
-// 16 (code + 8), and one subtraction or multiply-add gives the code, exactly.
-struct CodeMasks {
-    uint32_t low, low_magic, high, high_magic;
-    // (unknown to the compiler, which would otherwise split (a & low) ^ magic into two instructions with a constant each)
-    __device__ __forceinline__ CodeMasks() {
-        asm volatile("mov.b32 %0, 0x000f000f;\n\tmov.b32 %1, 0x64086408;\n\tmov.b32 %2, 0x00f000f0;\n\tmov.b32 %3, 0x64806480;"
-                     : "=r"(low), "=r"(low_magic), "=r"(high), "=r"(high_magic));
-    }
-};
-__device__ __forceinline__ __half2 and_xor(uint32_t a, uint32_t mask, uint32_t magic) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(a), "r"(mask), "r"(magic));
-    return *reinterpret_cast<const __half2*>(&r);
-}
-__device__ __forceinline__ void weights_of(uint32_t word, __half2 scale, const CodeMasks& m, uint32_t (&w)[4]) {
-    const __half2 low = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));        // 1032
-    const __half2 shift = __halves2half2(__ushort_as_half(0x2c00), __ushort_as_half(0x2c00));      // 1 / 16
-    const __half2 high = __halves2half2(__ushort_as_half(0xd480), __ushort_as_half(0xd480));       // -72
-#pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-        const uint32_t bits = word >> (4 * i);
-        const __half2 even = __hmul2(__hsub2(and_xor(bits, m.low, m.low_magic), low), scale);
-        const __half2 odd = __hmul2(__hfma2(and_xor(bits, m.high, m.high_magic), shift, high), scale);
-        w[i] = *reinterpret_cast<const uint32_t*>(&even);
-        w[i + 1] = *reinterpret_cast<const uint32_t*>(&odd);
-    }
-}
-
+constexpr int kWideRows = 16384;      // weight rows from which the wide kernel takes them
 constexpr int kGemvTiles = 4;         // 16-row tiles of weights that a block takes at a time
 
 template <int RowTiles>
@@ -230,15 +185,7 @@ gemv_w4g128_kernel(const GemvParams p) {
             float v = 0.0f;
 #pragma unroll
             for (int w = 0; w < kGemvWarps; ++w) v += sm.sums[w][row][m];
-            v *= p.row_scales != nullptr ? p.row_scales[m] : p.row_scale;
-            if (p.col_scales != nullptr) v *= p.col_scales[n];
-            if (p.bias != nullptr) v += p.bias[n];
-            if (p.act == PK100_ACT_SILU) v = v / (1.0f + __expf(-v));
-            else if (p.act == PK100_ACT_RELU) v = fmaxf(v, 0.0f);
-            v = p.residual != nullptr ? fmaf(p.alpha, v, __half2float(p.residual[m * p.ld_res + n])) : p.alpha * v;
-            if (m >= p.valid_rows) v = 0.0f;
-            if (p.out_type == PK100_OUT_F16) static_cast<__half*>(p.out)[m * p.ld_out + n] = __float2half_rn(v);
-            else static_cast<float*>(p.out)[m * p.ld_out + n] = v;
+            gemv_store(p, v, m, n);
         }
     }
     cp_async_wait<0>();
@@ -272,7 +219,7 @@ extern "C" int pk100_gemv_w4g128(void* stream_v, const pk100_gemm_args* a) {
     if (a->m > 1 && (a->lda < a->k || a->lda % 8 != 0 || a->ld_out < a->n || (a->residual != nullptr && a->ld_res < a->n))) return PK100_ERR_SHAPE;
     auto off = [](const void* ptr, unsigned bytes) { return reinterpret_cast<uintptr_t>(ptr) % bytes != 0; };
     if (off(a->a, 16) || off(a->b, 16) || off(a->b_group_scales, 2) || off(a->residual, 2) || off(a->row_scales, 4) ||
-        off(a->col_scales, 4) || off(a->bias, 4) || off(a->out, a->out_type == PK100_OUT_F16 ? 2 : 4))
+        off(a->col_scales, 4) || off(a->bias, 4) || off(a->status, 4) || off(a->out, a->out_type == PK100_OUT_F16 ? 2 : 4))
         return PK100_ERR_ALIGN;
     GemvParams p{};
     p.m = a->m; p.n = a->n; p.k = a->k;
@@ -285,5 +232,12 @@ extern "C" int pk100_gemv_w4g128(void* stream_v, const pk100_gemm_args* a) {
     p.alpha = a->alpha; p.valid_rows = a->valid_rows <= 0 ? a->m : a->valid_rows;
     p.out = a->out; p.ld_out = a->ld_out; p.out_type = a->out_type;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+    p.status = a->status;
+    // From 16 384 weight rows on (three and a half tiles a cluster) the wide kernel: 13 rows by 28 672 x 8192 in 36 us against 50, x 1024
+    // in 10.7 against 14.9; one row about the same; 8192 x 4096 9.7 against 9.4, 4096 x 14 336 17.5 against 15.0.
+    if (a->n >= kWideRows && a->k <= gemv_wide_limit()) {
+        const int rc = launch_gemv_wide(p, stream);
+        if (rc != PK100_ERR_UNSUPPORTED) return rc;                    // (no cluster fits the device or the budget)
+    }
     return a->m <= 8 ? launch_gemv<1>(p, stream) : launch_gemv<2>(p, stream);
 }

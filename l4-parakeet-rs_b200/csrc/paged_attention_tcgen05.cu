@@ -32,13 +32,6 @@ struct Smem {
 template <typename T> __host__ __device__ constexpr uint32_t type_bits() { return 0; }                                    // kind::f16 operands: fp16
 template <> __host__ __device__ constexpr uint32_t type_bits<__nv_bfloat16>() { return (1u << 7) | (1u << 10); }
 
-// D[tmem] (+)= A[tmem] * B[smem], 16 k, issued where `leader` is set
-__device__ __forceinline__ void mma_from_tmem(bool leader, uint32_t d, uint32_t a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
-                 ::"r"(d), "r"(a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(static_cast<uint32_t>(leader)) : "memory");
-}
-
 __device__ __forceinline__ float max_of(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));

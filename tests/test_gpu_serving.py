@@ -138,7 +138,9 @@ def _packed(n, k, seed, cuda):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 1, 128), (1, 16, 256), (2, 17, 128), (3, 100, 1024), (8, 64, 2048), (9, 63, 1152), (16, 257, 4096),
-                                   (1, 1024, 4096), (7, 9473, 384), (16, 9500, 1280), (13, 4096, 16384)])
+                                   (1, 1024, 4096), (7, 9473, 384), (16, 9500, 1280), (13, 4096, 16384), (1, 70001, 1024),
+                                   (16, 16390, 9088), (5, 33000, 2176), (2, 20000, 128),
+                                   (3, 16400, 16384), (9, 16400, 16512)])
 def test_gemv_sizes(pk, cuda, m, n, k):
     codes, scales = _packed(n, k, m + n + k, cuda)
     w, x = R.w4_weights(codes, scales), _normal(5, m, k)
