@@ -642,9 +642,9 @@ enum {
 };
 
 /* Residual addition and root-mean-square norm:
- *   s = round(input + residual)  (residual == NULL: s = input), written to residual_out when given (may alias
- *       either input);
- *   y = s * rsqrt(mean(s^2) + eps) * gamma, in fp32 from the rounded s;
+ *   s = round(input + residual)  (residual == NULL: s = input), written to residual_out when given (may be either
+ *       input itself, not a shifted view of one);
+ *   y = s * rsqrt(mean(s^2) + eps) * gamma, in fp32 from the rounded s (bf16 rows whose squares exceed fp32 give 0);
  *   output in `mode`: PK100_LN_F16 = round(y) in the input's type; PK100_LN_E4M3_FIXED = E4M3(y * inv_scale);
  *   PK100_LN_E4M3_ROW = E4M3(y / c), c = max|y| / 448; PK100_LN_S8_ROW = rne(y / c), c = max|y| / 127, c -> scales
  *   (0 -> 1): the operands of pk100_gemm kinds E4M3 and S8.  A row with a NaN or an infinity takes its maximum over
@@ -670,7 +670,8 @@ int pk100_add_rms_norm(void* stream, const pk100_rms_norm_args* args);
  * weights' bytes and pk100_gemm's tiles are mostly padding: the same arguments, weights W = f16(code * scale) and
  * epilogue algebra, fp32 sums (in another order than pk100_gemm's).  Any n; k % 128 == 0; a and b 16-byte
  * aligned, lda % 8 == 0; out and residual of any leading dimension; PK100_EPI_LINEAR; out_type PK100_OUT_F16 or
- * _F32.  More than 16 rows: PK100_ERR_LIMIT.  tau, keep_*, stats_out and max_ctas are not read. */
+ * _F32.  More than 16 rows: PK100_ERR_LIMIT.  A row's bits depend on its own values, n and k alone.  tau, keep_*,
+ * stats_out and max_ctas are not read. */
 int pk100_gemv_w4g128(void* stream, const pk100_gemm_args* args);
 
 /* One step's bookkeeping of a paged key-value cache, from the request lengths alone:
@@ -680,15 +681,16 @@ int pk100_gemv_w4g128(void* stream, const pk100_gemm_args* args);
  *   token t of request r, i-th new one: positions[t] = cached[r] + i,
  *   slots[t] = block_table[r][positions[t] / page_size] * page_size + positions[t] % page_size.
  * Rows t >= starts[requests] get slot and position -1.  Where the step does not fit (a negative length, more new
- * tokens than `tokens`, more pages than *free_count or max_pages) nothing is taken: PK100_STATUS_PLAN is set in
+ * tokens than `tokens`, more pages than *free_count, free_capacity or max_pages) nothing is taken: PK100_STATUS_PLAN is set in
  * *status, starts and *used are 0, lengths = cached, every slot and position -1, block_table as it was.  At most
- * PK100_PLAN_MAX_REQUESTS requests (PK100_ERR_LIMIT).  Outputs overlap no input (lengths == cached is refused). */
+ * PK100_PLAN_MAX_REQUESTS requests (PK100_ERR_LIMIT).  Outputs overlap no input (lengths equal to cached or
+ * new_tokens is refused). */
 #define PK100_PLAN_MAX_REQUESTS 4096
 typedef struct pk100_paged_plan_args {
-    int requests, tokens, page_size, max_pages;
+    int requests, tokens, page_size, max_pages, free_capacity;
     const int* cached;                            /* [requests] */
     const int* new_tokens;                        /* [requests] */
-    const int* free_pages; const int* free_count; /* page ids (NULL: none); device count of them */
+    const int* free_pages; const int* free_count; /* [free_capacity] page ids (NULL: none); device count of them */
     int* block_table;                             /* [requests, max_pages], rows beyond a request's pages are not read */
     int* starts;                                  /* [requests + 1] */
     int* lengths;                                 /* [requests] */
@@ -717,7 +719,8 @@ int pk100_paged_plan(void* stream, const pk100_paged_plan_args* args);
  * request that do not see it.  A page id outside [0, pages) reads as zeros, a slot outside the cache is not
  * written, a length beyond max_pages pages is cut; each sets PK100_STATUS_PAGE.  Bit 0: a bounded wait expired.
  * max_new: no request has more new tokens than this (<= 0: not known).  It chooses kernels, no result but rounding
- * depends on it; requests beyond it are attended all the same.
+ * depends on it; requests beyond it are attended all the same.  Rounding depends on the lengths of the other requests,
+ * too (the work is shared out by them); the same call gives the same bits.
  * workspace: >= pk100_paged_attention_workspace_bytes(args) bytes, 256-byte aligned, used by the call until it has
  * completed; calls that may overlap on the GPU need one each. */
 typedef struct pk100_paged_attention_args {

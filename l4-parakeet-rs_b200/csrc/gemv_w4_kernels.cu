@@ -237,7 +237,7 @@ extern "C" int pk100_gemv_w4g128(void* stream_v, const pk100_gemm_args* a) {
     // in 10.7 against 14.9; one row about the same; 8192 x 4096 9.7 against 9.4, 4096 x 14 336 17.5 against 15.0.
     if (a->n >= kWideRows && a->k <= gemv_wide_limit()) {
         const int rc = launch_gemv_wide(p, stream);
-        if (rc != PK100_ERR_UNSUPPORTED) return rc;                    // (no cluster fits the device or the budget)
+        if (rc != PK100_ERR_UNSUPPORTED) return rc;                    // (the device holds no such cluster)
     }
     return a->m <= 8 ? launch_gemv<1>(p, stream) : launch_gemv<2>(p, stream);
 }

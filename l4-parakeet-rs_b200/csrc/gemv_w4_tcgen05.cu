@@ -267,9 +267,11 @@ int gemv_wide_limit() { return wide::kCluster * wide::kMostGroups * kGroup; }
 int launch_gemv_wide(const GemvParams& p, cudaStream_t stream) {
     const cudaError_t granted = pk100_grant_smem<wide::gemv_w4g128_wide_kernel>(sizeof(wide::Smem));
     if (granted != cudaSuccess) return static_cast<int>(granted);
-    const int budget = pk100_cta_budget() / wide::kCluster, held = wide_clusters(), tiles = (p.n + wide::kTile - 1) / wide::kTile;
-    int clusters = held < budget ? held : budget;
-    if (clusters < 1) return PK100_ERR_UNSUPPORTED;
+    const int held = wide_clusters(), tiles = (p.n + wide::kTile - 1) / wide::kTile;
+    if (held < 1) return PK100_ERR_UNSUPPORTED;
+    int clusters = pk100_cta_budget() / wide::kCluster;
+    if (clusters < 1) clusters = 1;                      // (not another kernel: no result depends on the cap)
+    if (clusters > held) clusters = held;
     if (clusters > tiles) clusters = tiles;
     CUtensorMap map;
     const int rc = pk100_tensor_map_2d(&map, p.codes, 1, p.n, p.k / 2, p.k / 2, wide::kTile, 128);

@@ -566,7 +566,8 @@ static int paged_check(const pk100_paged_attention_args* a) {
     if (a->heads % a->kv_heads != 0) return PK100_ERR_SHAPE;
     if (a->head_dim != 64 && a->head_dim != 128) return PK100_ERR_UNSUPPORTED;
     if (a->page_size != 16 && a->page_size != 32 && a->page_size != 64 && a->page_size != 128 && a->page_size != 256) return PK100_ERR_UNSUPPORTED;
-    if (static_cast<long long>(a->max_pages) * a->page_size > (1ll << 30) || static_cast<long long>(a->tokens) * a->heads > (1ll << 30))
+    if (static_cast<long long>(a->max_pages) * a->page_size > (1ll << 30) || static_cast<long long>(a->tokens) * a->heads > (1ll << 30) ||
+        static_cast<long long>(a->requests) * a->heads > (1ll << 30))
         return PK100_ERR_LIMIT;
     return PK100_OK;
 }

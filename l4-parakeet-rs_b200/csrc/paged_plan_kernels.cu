@@ -58,7 +58,7 @@ paged_plan_kernel(const pk100_paged_plan_args p) {
         all_tokens += warp_tokens[w];
         all_pages += warp_pages[w];
     }
-    const int free_count = p.free_pages != nullptr ? *p.free_count : 0;
+    const int free_count = p.free_pages != nullptr ? min(*p.free_count, p.free_capacity) : 0;
     const bool no = refused != 0 || all_tokens > p.tokens || all_pages > free_count;
     const bool leader = blockIdx.x == 0;
 #pragma unroll
@@ -121,13 +121,13 @@ using namespace pk100;
 
 extern "C" int pk100_paged_plan(void* stream, const pk100_paged_plan_args* a) {
     if (a == nullptr) return PK100_ERR_NULL;
-    if (a->requests < 0 || a->tokens < 0 || a->page_size <= 0 || a->max_pages <= 0) return PK100_ERR_SHAPE;
+    if (a->requests < 0 || a->tokens < 0 || a->page_size <= 0 || a->max_pages <= 0 || a->free_capacity < 0) return PK100_ERR_SHAPE;
     if (a->requests > PK100_PLAN_MAX_REQUESTS) return PK100_ERR_LIMIT;
     if (a->starts == nullptr || a->used == nullptr || a->free_count == nullptr) return PK100_ERR_NULL;
     if (a->requests > 0 && (a->cached == nullptr || a->new_tokens == nullptr || a->block_table == nullptr || a->lengths == nullptr))
         return PK100_ERR_NULL;
     if (a->tokens > 0 && (a->positions == nullptr || a->slots == nullptr)) return PK100_ERR_NULL;
-    if (a->requests > 0 && a->lengths == a->cached) return PK100_ERR_UNSUPPORTED;      // blocks read what others would have written
+    if (a->requests > 0 && (a->lengths == a->cached || a->lengths == a->new_tokens)) return PK100_ERR_UNSUPPORTED;      // blocks read what others would have written
     const uintptr_t words = reinterpret_cast<uintptr_t>(a->cached) | reinterpret_cast<uintptr_t>(a->new_tokens) | reinterpret_cast<uintptr_t>(a->free_pages) |
                             reinterpret_cast<uintptr_t>(a->free_count) | reinterpret_cast<uintptr_t>(a->block_table) | reinterpret_cast<uintptr_t>(a->starts) |
                             reinterpret_cast<uintptr_t>(a->lengths) | reinterpret_cast<uintptr_t>(a->positions) | reinterpret_cast<uintptr_t>(a->used) |

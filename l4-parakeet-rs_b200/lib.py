@@ -46,7 +46,7 @@ class RmsNormArgs(C.Structure):
 class PagedPlanArgs(C.Structure):
     """Mirror of `pk100_paged_plan_args`."""
     _fields_ = [
-        ("requests", i32), ("tokens", i32), ("page_size", i32), ("max_pages", i32),
+        ("requests", i32), ("tokens", i32), ("page_size", i32), ("max_pages", i32), ("free_capacity", i32),
         ("cached", vp), ("new_tokens", vp), ("free_pages", vp), ("free_count", vp), ("block_table", vp), ("starts", vp),
         ("lengths", vp), ("positions", vp), ("slots", vp), ("used", vp), ("status", vp),
     ]

@@ -375,7 +375,7 @@ def add_rms_norm(x, gamma, residual=None, mode=L.LN_F16, inv_scale=0.0, eps=EPS,
 
 
 def gemv_w4g128(a, codes, group_scales, *, out=None, row_scales=None, row_scale=1.0, col_scales=None, bias=None, act=L.ACT_NONE,
-                residual=None, alpha=1.0, valid_rows=0, out_type=L.OUT_F16):
+                residual=None, alpha=1.0, valid_rows=0, out_type=L.OUT_F16, status=None):
     """D = epilogue(A . W^T) for up to 16 rows, W from `pack_weight_rows(PACK_S4_G128)`; see `pk100_gemv_w4g128`."""
     m, k = a.shape
     n, device = codes.shape[0], _device(a)
@@ -390,9 +390,10 @@ def gemv_w4g128(a, codes, group_scales, *, out=None, row_scales=None, row_scale=
     rows_at = 0 if row_scales is None else _whole("row_scales", row_scales, (m,), torch.float32, device)
     cols_at = 0 if col_scales is None else _whole("col_scales", col_scales, (n,), torch.float32, device)
     bias_at = 0 if bias is None else _whole("bias", bias, (n,), torch.float32, device)
+    status_at = 0 if status is None else _whole("status", status, (1,), torch.int32, device)
     rc = _gemv_w4g128(_stream_of(device), _GEMM_ARGS.pack(
         L.KIND_F16_W4G128, L.EPI_LINEAR, m, n, k, a_at, a_ld, codes_at, k // 2, rows_at, row_scale, cols_at, bias_at, act, res_at, res_ld, alpha,
-        valid_rows, out_at, out_ld, out_type, 1.0, 0.0, 0, 0, 0, 0, 0, groups_at))
+        valid_rows, out_at, out_ld, out_type, 1.0, 0.0, 0, 0, 0, status_at, 0, groups_at))
     L.check(rc, "pk100_gemv_w4g128")
     return out
 
@@ -411,7 +412,7 @@ def paged_plan(cached, new_tokens, block_table, free_pages, free_count, *, token
     table_at = _whole("block_table", block_table, (requests, max_pages), i32, device)
     cached_at = _whole("cached", cached, (requests,), i32, device)
     new_at = _whole("new_tokens", new_tokens, (requests,), i32, device)
-    free_at = _whole("free_pages", free_pages, (free_pages.numel(),), i32, device)
+    free_at = _whole("free_pages", free_pages, (len(free_pages),), i32, device)
     count_at = _whole("free_count", free_count, (1,), i32, device)
     status_at = 0 if status is None else _whole("status", status, (1,), i32, device)
     if out is None:
@@ -428,7 +429,7 @@ def paged_plan(cached, new_tokens, block_table, free_pages, free_count, *, token
         positions_at = _whole("positions", out.positions, (tokens,), i32, device)
         slots_at = _whole("slots", out.slots, (tokens,), torch.int64, device)
         used_at = _whole("used", out.used, (1,), i32, device)
-    rc = _paged_plan(_stream_of(device), _PAGED_PLAN_ARGS.pack(requests, tokens, page_size, max_pages, cached_at, new_at, free_at, count_at, table_at, starts_at,
+    rc = _paged_plan(_stream_of(device), _PAGED_PLAN_ARGS.pack(requests, tokens, page_size, max_pages, free_pages.shape[0], cached_at, new_at, free_at, count_at, table_at, starts_at,
                                                       lengths_at, positions_at, slots_at, used_at, status_at))
     L.check(rc, "pk100_paged_plan")
     return out

@@ -250,6 +250,31 @@ def test_plan_refuses_a_step_that_does_not_fit(pk, cuda, cached, new, max_pages,
     assert (p.positions == -1).all() and (p.slots == -1).all()
 
 
+def test_plan_reads_no_further_than_the_free_list(pk, cuda):
+    """A count that is larger than the list: what the list does not hold is not there."""
+    table, status = _int([[-1] * 4]), _int([0])
+    p = pk.ops.paged_plan(_int([0]), _int([40]), table, _int([5, 6]), _int([1000]), tokens=40, page_size=16, status=status)
+    assert int(status) == pk.lib.STATUS_PLAN and p.used.tolist() == [0] and (table == -1).all()
+
+
+def test_plan_captured_and_replayed(pk, cuda):
+    cached, new, table, free, count = _int([0, 20]), _int([1, 1]), _int([[-1] * 4, [7, 3, -1, -1]]), _int(list(range(10, 20))), _int([10])
+    before = table.clone()
+    pk.ops.paged_plan(cached, new, table, free, count, tokens=8, page_size=16)
+    table.copy_(before)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        p = pk.ops.paged_plan(cached, new, table, free, count, tokens=8, page_size=16)
+    for c, n in (([0, 20], [1, 1]), ([0, 20], [5, 3]), ([0, 31], [0, 2])):
+        cached.copy_(_int(c))
+        new.copy_(_int(n))
+        table.copy_(before)
+        graph.replay()
+        want = R.plan(c, n, before.tolist(), free.tolist(), 16)
+        pad = 8 - sum(n)
+        assert table.tolist() == want[0] and p.starts.tolist() == want[1] and p.slots.tolist() == want[4] + [-1] * pad and p.used.tolist() == [want[5]]
+
+
 def test_plan_without_requests_or_tokens(pk, cuda):
     none = torch.empty(0, dtype=torch.int32, device=cuda)
     p = pk.ops.paged_plan(none, none, none.reshape(0, 4), none, _int([0]), tokens=3, page_size=16)
@@ -483,6 +508,52 @@ def test_attention_captured_without_new_keys(pk, cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dim,kv", [(128, 2), (64, 4)])
+def test_attention_of_single_tokens_beside_chunks(pk, cuda, dim, kv):
+    """The kernels for single tokens and for chunks run side by side: the same bits every time, and what each request gets
+    alone."""
+    new = [1] * 30 + [700, 3, 90] + [1] * 10
+    cached = [100 * i for i in range(30)] + [1300, 50, 0] + [37 * i for i in range(10)]
+    s = Step(new, cached, 8, kv, dim, 32, BF16, seed=3)
+    want = s.run(pk).clone()
+    s.check(want)
+    for _ in range(10):
+        assert torch.equal(s.run(pk), want)
+
+
+@pytest.mark.parametrize("n,k", [(1000, 1024), (20000, 1024)])
+def test_gemv_captured_and_under_a_cap(pk, cuda, n, k):
+    codes, scales = _packed(n, k, 1, cuda)
+    x, status = _normal(2, 3, k), _int([0])
+    want = pk.ops.gemv_w4g128(x, codes, scales, status=status).clone()
+    out = torch.empty_like(want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pk.ops.gemv_w4g128(x, codes, scales, out=out, status=status)
+    graph.replay()
+    assert torch.equal(out, want)
+    x.mul_(2.0)                                                            # (a power of two: twice the result, to the bit)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want * 2) and int(status) == 0
+    try:
+        for cap in (1, 3, 50):
+            pk.lib.lib.pk100_set_gemm_cta_cap(cap)
+            assert torch.equal(pk.ops.gemv_w4g128(x, codes, scales), out)
+    finally:
+        pk.lib.lib.pk100_set_gemm_cta_cap(0)
+
+
+def test_gemv_rows_of_the_wide_kernel_stay_alone(pk, cuda):
+    codes, scales = _packed(16500, 1152, 4, cuda)
+    x = _normal(2, 4, 1152)
+    clean = pk.ops.gemv_w4g128(x, codes, scales)
+    x[2, 700], x[3, 1100] = math.inf, math.nan
+    got = pk.ops.gemv_w4g128(x, codes, scales)
+    assert torch.equal(got[:2], clean[:2]) and torch.isnan(got[3]).all()
+    assert torch.equal(pk.ops.gemv_w4g128(x[1:2], codes, scales), clean[1:2])
 
 
 def test_calls_on_two_streams_at_once(pk, cuda):

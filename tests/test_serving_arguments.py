@@ -47,7 +47,7 @@ def test_gemv_refusals(pk):
 
 
 def _plan(L, **changes):
-    a = L.PagedPlanArgs(requests=2, tokens=8, page_size=16, max_pages=4, cached=256, new_tokens=512, free_pages=1024, free_count=1280,
+    a = L.PagedPlanArgs(requests=2, tokens=8, page_size=16, max_pages=4, free_capacity=9, cached=256, new_tokens=512, free_pages=1024, free_count=1280,
                         block_table=2048, starts=4096, lengths=4352, positions=4608, slots=5120, used=6144)
     for name, value in changes.items():
         setattr(a, name, value)
@@ -61,7 +61,9 @@ def test_plan_refusals(pk):
         assert _plan(L, **{name: None}) == L.ERR_NULL, name
     assert _plan(L, requests=-1) == _plan(L, tokens=-1) == _plan(L, page_size=0) == _plan(L, max_pages=0) == L.ERR_SHAPE
     assert _plan(L, requests=L.PLAN_MAX_REQUESTS + 1) == L.ERR_LIMIT
-    assert _plan(L, lengths=256) == L.ERR_UNSUPPORTED                       # in place: other blocks read what one has written
+    # in place: other blocks read what one has written
+    assert _plan(L, lengths=256) == _plan(L, lengths=512) == L.ERR_UNSUPPORTED
+    assert _plan(L, free_capacity=-1) == L.ERR_SHAPE
     assert _plan(L, cached=258) == _plan(L, slots=5124) == _plan(L, status=2) == L.ERR_ALIGN
 
 
@@ -88,7 +90,7 @@ def test_attention_refusals(pk):
     assert _attention(L, **dict(new, ld_key=100)) == _attention(L, **dict(new, ld_value=132)) == L.ERR_SHAPE
     assert _attention(L, token_stride=60) == _attention(L, head_stride=68) == _attention(L, page_stride=4) == L.ERR_SHAPE
     assert _attention(L, page_stride=1 << 39) == L.ERR_SHAPE
-    assert _attention(L, max_pages=1 << 27) == _attention(L, tokens=1 << 28) == L.ERR_LIMIT
+    assert _attention(L, max_pages=1 << 27) == _attention(L, tokens=1 << 28) == _attention(L, requests=1 << 28) == L.ERR_LIMIT
     assert _attention(L, workspace_bytes=1000) == L.ERR_LIMIT
     assert _attention(L, query=4104) == _attention(L, key_cache=8200) == _attention(L, workspace=65552) == L.ERR_ALIGN
     assert _attention(L, **dict(new, key=4104)) == _attention(L, **dict(new, slots=516)) == _attention(L, starts=258) == L.ERR_ALIGN
