@@ -42,8 +42,8 @@ struct GemvSmem {
 // come by asynchronous copies, up to 96 KB of them in flight, into a ring in which every thread reads what it has
 // copied itself: no barrier in the loop, and the next chunk is on its way while this one is joined.  Activations and
 // scales of the next group are requested a group ahead.
-// 13 x 8192 by 28672 rows (122 MB): 50.5 us, 2.4 TB/s; 76.8 us with a block per 64 rows, 8 warps and no requests ahead.
-// Bound by the conversion: per 64 x 128 codes a warp issues about 750 instructions, half of them on half-rate pipes.
+// One row by 8192 x 4096 (17 MB): 6.8 us; 1024 x 4096: 3.9 us.  Bound by the conversion and by mma.sync, whose ten issue
+// cycles nothing else fills; small products by their chain of load, conversion and join.
 template <int RowTiles>
 __global__ void __launch_bounds__(kGemvThreads, 1)
 gemv_w4g128_kernel(const GemvParams p) {

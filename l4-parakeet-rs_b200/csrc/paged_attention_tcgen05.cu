@@ -147,8 +147,9 @@ __device__ __forceinline__ int request_of(const PagedParams& p, int pair, int& b
 // 2^8, within fp16's range, and the rescaling of O all but disappears.
 // Scores, m, l and O are fp32; P is rounded to the type of V for the tensor cores, which costs what the rounding of the
 // output costs (the sum l is that of the unrounded P).
-// Two prompts of 7.2 k tokens, 16 / 4 heads of 128: 494 us, 870 TFLOP/s (the few-row kernel in the same place: 4.6 ms); 512 tokens over
-// 32 000, 16 / 2 heads: 159 us, 840 TFLOP/s (764 us).
+// Bound by a tile's chain of scores, softmax and products: 3200 cycles per 128 keys of both tiles, of which the MMAs are
+// 2300.  Two prompts of 7.2 k tokens, 16 / 4 heads of 128: 437 us, 990 TFLOP/s (the few-row kernel in the same place: 4.6 ms);
+// 512 tokens over 32 000, 16 / 2 heads: 141 us, 960 TFLOP/s (764 us).
 template <typename T, int D>
 __global__ void __launch_bounds__(threads<D>(), 3 - tiles<D>())
 paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p,

@@ -282,9 +282,12 @@ def _type(t):
     return code
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)      # (without the look whether CUDA is up)
+
+
 def _device(t):
     """The operators launch on the current device's stream: its index, which what they are given has to have."""
-    return torch.cuda.current_device() if t.is_cuda else -2
+    return _current_device() if t.is_cuda else -2
 
 
 def _refuse(name, t, shape, dtype, device):
@@ -349,7 +352,7 @@ def add_rms_norm(x, gamma, residual=None, mode=L.LN_F16, inv_scale=0.0, eps=EPS,
     rows, width = shape
     if mode not in (L.LN_F16, L.LN_E4M3_FIXED, L.LN_E4M3_ROW, L.LN_S8_ROW):
         raise ValueError(f"add_rms_norm has no output mode {mode}")
-    x_at, x_ld = _rows("x", x, shape, dtype, device)
+    x_at, x_ld = (x.data_ptr(), width) if x.is_contiguous() and device >= 0 and x.get_device() == device else _rows("x", x, shape, dtype, device)
     gamma_at = _whole("gamma", gamma, (width,), dtype, device)
     out_dtype = _out_dtype(mode, dtype)
     if out is None:
@@ -416,9 +419,9 @@ def paged_plan(cached, new_tokens, block_table, free_pages, free_count, *, token
     count_at = _whole("free_count", free_count, (1,), i32, device)
     status_at = 0 if status is None else _whole("status", status, (1,), i32, device)
     if out is None:
-        words = torch.empty(2 * requests + 2 + tokens, device=block_table.device, dtype=i32)
+        words = block_table.new_empty(2 * requests + 2 + tokens)
         starts, lengths, positions, used = words.split_with_sizes((requests + 1, requests, tokens, 1))
-        slots = torch.empty(tokens, device=block_table.device, dtype=torch.int64)
+        slots = block_table.new_empty(tokens, dtype=torch.int64)
         out = PagedPlan(starts, lengths, positions, slots, used)
         at = words.data_ptr()
         starts_at, lengths_at, positions_at, used_at = at, at + 4 * (requests + 1), at + 4 * (2 * requests + 1), at + 4 * (2 * requests + 1 + tokens)
@@ -488,7 +491,7 @@ def paged_attention(query, key_cache, value_cache, block_table, starts, lengths,
     status_at = 0 if status is None else _whole("status", status, (1,), i32, device)
     if workspace is None:
         need = _paged_workspace(device, tokens, requests, heads, kv_heads, head_dim, page_size, max_pages)
-        workspace = torch.empty(need, device=query.device, dtype=torch.uint8)
+        workspace = block_table.new_empty(need // 4)         # (whole multiples of 256 bytes)
     else:
         need = workspace.numel()
         _whole("workspace", workspace, (need,), torch.uint8, device)

@@ -510,6 +510,29 @@ def test_attention_captured_without_new_keys(pk, cuda):
         assert torch.equal(out, want)
 
 
+def test_attention_of_a_wrong_hint(pk, cuda):
+    """max_new below what a request brings: slower, not wrong."""
+    s = Step([300, 1, 40], [500, 77, 0], 8, 2, 64, 16, F16)
+    s.check(s.run(pk, max_new=1))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_a_mixed_step_captured(pk, cuda, dim):
+    """New keys, chunk kernel over shares of the keys, few-row kernel beside it and the join, replayed on other data."""
+    s = Step([1, 200, 3], [3000, 1500, 0], 8, 2, dim, 32, BF16)
+    out = torch.empty_like(s.q)
+    s.run(pk, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s.run(pk, out=out)
+    for seed in range(3):
+        s.q.copy_(_normal(100 + seed, *s.q.shape, dtype=BF16))
+        s.v.copy_(_normal(200 + seed, *s.v.shape, dtype=BF16))
+        graph.replay()
+        torch.cuda.synchronize()
+        s.check(out)
+
+
 @pytest.mark.parametrize("dim,kv", [(128, 2), (64, 4)])
 def test_attention_of_single_tokens_beside_chunks(pk, cuda, dim, kv):
     """The kernels for single tokens and for chunks run side by side: the same bits every time, and what each request gets
