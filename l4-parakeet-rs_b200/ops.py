@@ -415,7 +415,7 @@ def paged_plan(cached, new_tokens, block_table, free_pages, free_count, *, token
     table_at = _whole("block_table", block_table, (requests, max_pages), i32, device)
     cached_at = _whole("cached", cached, (requests,), i32, device)
     new_at = _whole("new_tokens", new_tokens, (requests,), i32, device)
-    free_at = _whole("free_pages", free_pages, (len(free_pages),), i32, device)
+    free_at = _whole("free_pages", free_pages, free_pages.shape, i32, device)
     count_at = _whole("free_count", free_count, (1,), i32, device)
     status_at = 0 if status is None else _whole("status", status, (1,), i32, device)
     if out is None:
