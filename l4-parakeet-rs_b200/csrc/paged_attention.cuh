@@ -27,6 +27,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 struct PagedRequest {
     int row0, n, len;
     bool cut;
+    __device__ __forceinline__ PagedRequest(int row0_, int n_, int len_, bool cut_) : row0(row0_), n(n_), len(len_), cut(cut_) {}
     __device__ __forceinline__ PagedRequest(const PagedParams& p, int r) {
         const int first = p.starts[r], end = p.starts[r + 1], length = p.lengths[r];
         row0 = min(max(first, 0), p.tokens);

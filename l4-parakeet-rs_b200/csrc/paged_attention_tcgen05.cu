@@ -91,7 +91,7 @@ struct Work {
     int request, head, row, rows;               // first row of the first tile inside the request; rows of both tiles that exist
     int lo, hi;                                 // keys that any of the rows sees
     int from, to;                               // key blocks of this share
-    __device__ __forceinline__ Work(const PagedParams& p, int request_, int head_, int pair) : at(p, request_), request(request_), head(head_) {
+    __device__ __forceinline__ Work(const PagedParams& p, const PagedRequest& at_, int request_, int head_, int pair) : at(at_), request(request_), head(head_) {
         row = pair * kTiles * kTile;
         rows = min(at.n * p.group - row, kTiles * kTile);
         const int first = row / p.group, last = (row + max(rows, 1) - 1) / p.group;
@@ -111,45 +111,68 @@ struct Work {
     }
 };
 
-// Pairs of tiles are numbered over the batch with gaps: request r begins at floor(first row / rows of a pair) + r, which leaves
-// room for its last, partial one (pairs of one tile where D is 64).  The last request that begins at or before `pair`, found 32 candidates at a time.
+// The pair of tiles with this number: its request and place there (pairs of one tile where D is 64); none: request < 0.
+// The pairs with the most keys come first, so that the last blocks to start are the short ones.
+struct Place { int request, pair; PagedRequest at; };
 template <int kTiles>
-__device__ __forceinline__ int request_of(const PagedParams& p, int pair, int& begin) {
+__device__ __forceinline__ Place place_of(const PagedParams& p, int number, int pairs) {
+    constexpr int kRows = kTiles * kTile;
     const int lane = threadIdx.x % 32;
-    int lo = 0, hi = p.requests;                 // begin(lo) <= pair < begin(hi)
-    int begin_lo = 0;
+    if (p.requests <= 32) {
+        // a request a lane, the longest first; a request's last pairs see the most keys
+        const bool there = lane < p.requests;
+        const PagedRequest at = there ? PagedRequest(p, lane) : PagedRequest(0, 0, 0, false);
+        const int rows = at.n * p.group, mine = rows > p.few_rows ? (rows + kRows - 1) / kRows : 0;
+        const int keys = there ? (p.window > 0 ? min(at.len, p.window) : at.len) : -1;
+        int before = 0;
+        for (int r = 0; r < p.requests; ++r) {
+            const int other = __shfl_sync(0xffffffffu, keys, r), count = __shfl_sync(0xffffffffu, mine, r);
+            if (other > keys || (other == keys && r < lane)) before += count;
+        }
+        const uint32_t has = __ballot_sync(0xffffffffu, there && number >= before && number < before + mine);
+        const int request = has == 0 ? 0 : __ffs(has) - 1;
+        const int pair = __shfl_sync(0xffffffffu, mine - 1 - (number - before), request);
+        return Place{has == 0 ? -1 : request, pair,
+                     PagedRequest(__shfl_sync(0xffffffffu, at.row0, request), __shfl_sync(0xffffffffu, at.n, request),
+                                  __shfl_sync(0xffffffffu, at.len, request), __shfl_sync(0xffffffffu, static_cast<int>(at.cut), request) != 0)};
+    }
+    // More requests: numbered over the batch with gaps, request r from floor(first row / rows of a pair) + r on, which leaves room
+    // for its last, partial one; the last request that begins at or before the number, found 32 candidates at a time.
+    const int wanted = pairs - 1 - number;
+    int lo = 0, hi = p.requests, begin = 0;      // begin(lo) <= wanted < begin(hi)
     while (hi - lo > 1) {
         const int step = (hi - lo + 31) / 32, r = lo + lane * step;
         long long b = 0x7fffffffll;
-        if (r < hi) b = static_cast<long long>(max(p.starts[r], 0)) * p.group / (kTiles * kTile) + r;
-        const uint32_t before = __ballot_sync(0xffffffffu, b <= pair);
+        if (r < hi) b = static_cast<long long>(max(p.starts[r], 0)) * p.group / kRows + r;
+        const uint32_t before = __ballot_sync(0xffffffffu, b <= wanted);
         const int last = before == 0 ? 0 : 31 - __clz(before);
-        begin_lo = static_cast<int>(__shfl_sync(0xffffffffu, b, last));
+        begin = static_cast<int>(__shfl_sync(0xffffffffu, b, last));
         lo = min(lo + last * step, p.requests - 1);
         hi = min(lo + step, hi);
     }
-    if (p.requests == 1) begin_lo = static_cast<int>(static_cast<long long>(max(p.starts[0], 0)) * p.group / (kTiles * kTile));
-    begin = begin_lo;
-    return lo;
+    const PagedRequest at(p, lo);
+    const int rows = at.n * p.group, pair = wanted - begin;
+    return Place{pair >= 0 && pair * kRows < rows && rows > p.few_rows ? lo : -1, max(pair, 0), at};
 }
 
 #define CHUNK_WAIT(bar, parity) \
     if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&(bar), (parity), abort_flag)) != 0)) break
 
 // The query heads of a key-value head are rows of one tile (row = token * group + head), so a chunk of few tokens fills
-// its tiles and keys are read once for all of them.  One block of threads an SM: two 128-row tiles with a warpgroup of
-// softmax each (a row a thread: no exchange for maxima and sums), a TMA warp, an MMA warp.  Per 128-key block and tile
+// its tiles and keys are read once for all of them.  A tile of 128 rows has eight softmax warps (half a row a thread, the
+// halves' maxima meet in shared memory); a block has one TMA and one MMA warp.  Per 128-key block and tile
 //   S = Q K^T  (tcgen05, both operands from shared memory, 128 TMEM columns),
 //   P = exp2(scale S - m) back into the columns of S in 16 bits,
 //   O += P V   (A from tensor memory, V as it lies in the cache: MN-major), D TMEM columns.
-// While one tile's softmax runs, the tensor cores form the other's O and next S.  m follows the running maximum only
-// when that has grown by more than 2^8 (then O and l are scaled down, which is exact but for rounding): P stays below
-// 2^8, within fp16's range, and the rescaling of O all but disappears.
+// While one tile's softmax runs, the tensor cores form the other's O and next S (heads of 64: the other block's of the
+// SM).  m follows the running maximum only when that has grown by more than 2^8 (then O and l are scaled down, which is
+// exact but for rounding): P stays below 2^8, within fp16's range, and the rescaling of O all but disappears.
 // Scores, m, l and O are fp32; P is rounded to the type of V for the tensor cores, which costs what the rounding of the
 // output costs (the sum l is that of the unrounded P).
 // Bound by a tile's chain of scores, softmax and products: 3200 cycles per 128 keys of both tiles, of which the MMAs are
 // 2300.  Two prompts of 7.2 k tokens, 16 / 4 heads of 128: 437 us, 990 TFLOP/s (the few-row kernel in the same place: 4.6 ms);
-// 512 tokens over 32 000, 16 / 2 heads: 141 us, 960 TFLOP/s (764 us).
+// 512 tokens over 32 000, 16 / 2 heads: 134 to 141 us, 1 PFLOP/s (764 us).  Nine chunks of 5 to 561 tokens, 16 heads of 64,
+// window 1024: 27 us, the latency of the longest block (32.8 with the requests in their own order).
 template <typename T, int D>
 __global__ void __launch_bounds__(threads<D>(), 3 - tiles<D>())
 paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p,
@@ -187,12 +210,11 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
     grid_dependency_wait();
     grid_dependents_launch();                   // (only now: the few-row kernel behind this one does not wait for what is in front of it)
 
-    // the last pairs of a request see the most keys: they go first
-    const int head = blockIdx.x % p.kv_heads, share = blockIdx.x / p.kv_heads % shares, pair = pairs - 1 - blockIdx.x / p.kv_heads / shares;
-    int begin;
-    const int request = request_of<kTiles>(p, pair, begin);
-    Work<kTiles> w(p, request, head, pair - begin);
-    const bool mine = pair >= begin && w.rows > 0 && w.at.n * p.group > p.few_rows;
+    const int head = blockIdx.x % p.kv_heads, share = blockIdx.x / p.kv_heads % shares;
+    const Place place = place_of<kTiles>(p, blockIdx.x / p.kv_heads / shares, pairs);
+    const int request = place.request;
+    Work<kTiles> w(p, place.at, request, head, place.pair);
+    const bool mine = request >= 0;
     const int blocks = w.to - w.from;
     // a share is two blocks of keys at least
     const int parts = max(min(shares, blocks / 2), 1);
