@@ -13,7 +13,8 @@ template <int D> constexpr int softmax_warps() { return kTileWarps * tiles<D>();
 template <int D> constexpr int threads() { return softmax_warps<D>() * 32 + 64; }
 constexpr int kAtom = kTile * 128;              // 128 rows x 64 elements, 128-byte swizzle
 constexpr int kBox = 64;                        // most keys of a TMA box
-constexpr int kByFma = 4;                       // of 16 pairs of scores, whose exponentials the FMA pipe forms
+constexpr int kByFma = 5;                       // of 16 pairs of scores, whose exponentials the FMA pipe forms (two prompts: 2 434,
+                                                // 4 459, 5 425, 6 427, 7 443 us: the order of the instructions moves with it)
 
 template <int D> constexpr int ring_slots() { return 5; }
 
@@ -170,9 +171,9 @@ __device__ __forceinline__ Place place_of(const PagedParams& p, int number, int 
 // Scores, m, l and O are fp32; P is rounded to the type of V for the tensor cores, which costs what the rounding of the
 // output costs (the sum l is that of the unrounded P).
 // Bound by a tile's chain of scores, softmax and products: 3200 cycles per 128 keys of both tiles, of which the MMAs are
-// 2300.  Two prompts of 7.2 k tokens, 16 / 4 heads of 128: 437 us, 990 TFLOP/s (the few-row kernel in the same place: 4.6 ms);
+// 2300.  Two prompts of 7.2 k tokens, 16 / 4 heads of 128: 425 to 440 us, 1 PFLOP/s (the few-row kernel in the same place: 4.6 ms);
 // 512 tokens over 32 000, 16 / 2 heads: 134 to 141 us, 1 PFLOP/s (764 us).  Nine chunks of 5 to 561 tokens, 16 heads of 64,
-// window 1024: 27 us, the latency of the longest block (32.8 with the requests in their own order).
+// window 1024: 25 us, the latency of the longest block (32.8 with the requests in their own order).
 template <typename T, int D>
 __global__ void __launch_bounds__(threads<D>(), 3 - tiles<D>())
 paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p,
@@ -354,17 +355,21 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         // ------------------------------------------------------------ softmax: half a row a thread
         const int t = warp / kTileWarps, half = (warp / 4) % 2, quad = warp % 4, tile_row = quad * 32 + lane;
         {   // the queries of both tiles: 16 bytes a thread, rows that do not exist are zeros
-            constexpr int kChunks = D / 8;
-            for (int i = tid; i < kTiles * kTile * kChunks; i += kSoftmaxWarps * 32) {
-                const int r = i / kChunks, c = i % kChunks;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (r < w.rows) {
-                    const int index = w.row + r, token = index / p.group;
-                    v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.query) + (w.at.row0 + token) * p.ld_query +
-                                                        static_cast<long long>(head * p.group + index - token * p.group) * D + c * 8);
-                }
-                const int q_row = r % kTile;
-                *reinterpret_cast<uint4*>(sm.q[r / kTile][c / 8] + q_row * 128 + (((c % 8) ^ (q_row & 7)) << 4)) = v;
+            constexpr int kChunks = D / 8, kEach = kTiles * kTile * kChunks / (kSoftmaxWarps * 32);
+            const uint32_t sign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;      // a negative scale turns the queries round
+            uint4 v[kEach];                                  // (all requested before the first is stored)
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                const int r = (tid + j * kSoftmaxWarps * 32) / kChunks, index = w.row + r, token = index / p.group;
+                v[j] = r < w.rows ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.query) + (w.at.row0 + token) * p.ld_query +
+                                                                    static_cast<long long>(head * p.group + index - token * p.group) * D + tid % kChunks * 8)
+                                  : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                const int r = (tid + j * kSoftmaxWarps * 32) / kChunks, c = tid % kChunks, q_row = r % kTile;
+                *reinterpret_cast<uint4*>(sm.q[r / kTile][c / 8] + q_row * 128 + (((c % 8) ^ (q_row & 7)) << 4)) =
+                    make_uint4(v[j].x ^ sign, v[j].y ^ sign, v[j].z ^ sign, v[j].w ^ sign);
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -392,10 +397,6 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             tmem_ld_32x32(s_cols, reinterpret_cast<uint32_t(&)[32]>(s[0]));
             tmem_ld_32x32(s_cols + 32, reinterpret_cast<uint32_t(&)[32]>(s[32]));
             tmem_ld_wait();
-            if (p.scale_log2 < 0.0f) {
-#pragma unroll
-                for (int i = 0; i < 64; ++i) s[i] = -s[i];
-            }
             const int k0 = b * kTile;
             const bool masked = k0 < all_lo || k0 + kTile > all_hi;
             if (masked) {
@@ -453,7 +454,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             T* dst = static_cast<T*>(p.out) + (w.at.row0 + token) * p.ld_out + static_cast<long long>(head * p.group + index - token * p.group) * D + half * (D / 2);
             const long long part = static_cast<long long>(share) * p.tokens * p.heads + row;
             float* part_dst = part_out + part * D + half * (D / 2);
-#pragma unroll 1
+#pragma unroll (D == 64 ? 2 : 1)
             for (int c = 0; c < D / 2; c += 16) {
                 uint32_t o[16];
                 if (done > 0) {
