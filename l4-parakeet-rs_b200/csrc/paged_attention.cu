@@ -529,7 +529,7 @@ static int cache_map(CUtensorMap* map, const void* base, const pk100_paged_atten
 struct PagedPlan {
     int grid;                                            // blocks of the few-row kernel
     int pairs, shares;                                   // of the other one
-    long long counts, parts, part_out, share_ml, share_out, bytes;
+    long long counts, parts, part_out, share_count, share_ml, share_out, bytes;
 };
 
 static long long round256(long long n) { return (n + 255) / 256 * 256; }
@@ -545,7 +545,8 @@ static PagedPlan paged_plan_of(const pk100_paged_attention_args& a) {
     plan.counts = 0;
     plan.parts = round256(plan.grid * 4ll);
     plan.part_out = plan.parts + round256(2ll * plan.grid * static_cast<long long>(sizeof(RowsPart)));
-    plan.share_ml = plan.part_out + round256(2ll * plan.grid * kRows * a.head_dim * 4);
+    plan.share_count = plan.part_out + round256(2ll * plan.grid * kRows * a.head_dim * 4);
+    plan.share_ml = plan.share_count + 256;
     // Keys are shared out where the pairs of tiles leave SMs idle: few new tokens over a long cache.
     const long long rows = static_cast<long long>(a.tokens) * group, each = pair_rows(a.head_dim);
     const long long items = (rows + each - 1) / each * a.kv_heads;
@@ -657,14 +658,15 @@ extern "C" int pk100_paged_attention(void* stream_v, const pk100_paged_attention
         if (err != cudaSuccess) return static_cast<int>(err);
     }
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    int* share_count = reinterpret_cast<int*>(ws + plan.share_count);
     float2* share_ml = reinterpret_cast<float2*>(ws + plan.share_ml);
     float* share_out = reinterpret_cast<float*>(ws + plan.share_out);
-    if (many && (rc = paged_attention_chunks(a->type, a->head_dim, p, map_k, map_v, plan.pairs, plan.shares, share_ml, share_out, stream)) != PK100_OK) return rc;
+    if (many && (rc = paged_attention_chunks(a->type, a->head_dim, p, map_k, map_v, plan.pairs, plan.shares, share_count, share_ml, share_out, stream)) != PK100_OK) return rc;
     if (a->type == PK100_TYPE_F16)
         rc = a->head_dim == 128 ? launch_rows<__half, 128>(*a, p, plan, map_k, map_v, many, stream) : launch_rows<__half, 64>(*a, p, plan, map_k, map_v, many, stream);
     else
         rc = a->head_dim == 128 ? launch_rows<__nv_bfloat16, 128>(*a, p, plan, map_k, map_v, many, stream)
                                 : launch_rows<__nv_bfloat16, 64>(*a, p, plan, map_k, map_v, many, stream);
     if (rc != PK100_OK || !many || plan.shares == 1) return rc;
-    return paged_attention_join(a->type, a->head_dim, p, plan.shares, share_ml, share_out, stream);
+    return paged_attention_join(a->type, a->head_dim, p, share_count, share_ml, share_out, stream);
 }

@@ -55,12 +55,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 
 // The kernel for requests of more than p.few_rows rows (paged_attention_tcgen05.cu): `pairs` numbers of pairs of tiles
-// (tokens * group / pair_rows + requests), `shares` parts of a row's keys; part_ml [shares, tokens, heads] and
-// part_out [shares, tokens, heads, head_dim] where shares > 1.
+// (tokens * group / pair_rows + requests).  Where the pairs are few, a row's keys are shared out to up to `shares`; how many it came
+// to goes to share_count, their parts to part_ml [shares, tokens, heads] and part_out [shares, tokens, heads, head_dim], and
+// paged_attention_join adds them up (shares == 1: none of that).
 constexpr int pair_rows(int head_dim) { return head_dim == 128 ? 256 : 128; }
 int paged_attention_chunks(int type, int head_dim, const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares,
-                           float2* part_ml, float* part_out, cudaStream_t stream);
-// Adds the shares up.
-int paged_attention_join(int type, int head_dim, const PagedParams& p, int shares, const float2* part_ml, const float* part_out, cudaStream_t stream);
+                           int* share_count, float2* part_ml, float* part_out, cudaStream_t stream);
+int paged_attention_join(int type, int head_dim, const PagedParams& p, const int* share_count, const float2* part_ml, const float* part_out, cudaStream_t stream);
 
 }  // namespace pk100

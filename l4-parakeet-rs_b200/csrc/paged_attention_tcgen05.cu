@@ -1,4 +1,6 @@
 // Attention of many new tokens over a paged key-value cache on the tcgen05 tensor cores.
+#include <type_traits>
+
 #include "paged_attention.cuh"
 
 namespace pk100 {
@@ -25,9 +27,11 @@ struct Smem {
     uint8_t ring[ring_slots<D>()][D / 64][kAtom];          // key and value blocks in turn
     uint64_t full[ring_slots<D>()], empty[ring_slots<D>()];
     float top[kTiles][2][kTile];                           // row maxima of the halves; then sums
-    uint64_t q_ready, s_full[kTiles], p_full[kTiles], o_done[kTiles];
+    uint64_t q_ready[kTiles], s_full[kTiles], p_full[kTiles], o_done[kTiles];
     uint32_t tmem;
     int abort;
+    unsigned shares, items;                                // of the step
+    int row0[32], n[32], len[32], first[32], count[32];    // of up to 32 requests: geometry, their pairs of tiles
 };
 
 template <typename T> __host__ __device__ constexpr uint32_t type_bits() { return 0; }                                    // kind::f16 operands: fp16
@@ -57,7 +61,7 @@ __device__ __forceinline__ Pair exp2_fma(Pair x) {
 }
 
 // P = exp2(s * scale + shift) of 64 scores, stored as 16-bit pairs; the sum of the unrounded values.  ByFma: of 16 pairs
-// of scores, how many go to the FMA pipe (none where scores are masked: their -infinity has to give an exact zero).
+// of scores, how many go to the FMA pipe, where a masked score's -infinity gives 2^-126: nothing beside a sum of at least 1.
 template <typename T, int ByFma>
 __device__ __forceinline__ float weights_of_scores(const float (&s)[64], float scale, float shift, uint32_t p_cols) {
     const Pair scale2 = pair_of(scale, scale), shift2 = pair_of(shift, shift);
@@ -112,34 +116,83 @@ struct Work {
     }
 };
 
-// The pair of tiles with this number: its request and place there (pairs of one tile where D is 64); none: request < 0.
-// The pairs with the most keys come first, so that the last blocks to start are the short ones.
-struct Place { int request, pair; PagedRequest at; };
+// The step's pairs of tiles (pairs of one tile where D is 64) and where to find one.
+// Up to 32 requests: one warp orders them, the longest first, into shared memory; a request's last pairs, which see the most
+// keys, come first.  Up to 256: counted from the requests, in their order.  More: numbered over the batch with gaps, request r
+// from floor(first row / rows of a pair) + r on, which leaves room for its last, partial one.
+constexpr int kOrdered = 32, kCounted = 256;
+
 template <int kTiles>
-__device__ __forceinline__ Place place_of(const PagedParams& p, int number, int pairs) {
+__device__ __forceinline__ int pairs_of(const PagedParams& p, const PagedRequest& at) {
     constexpr int kRows = kTiles * kTile;
+    const int rows = at.n * p.group;
+    return rows > p.few_rows ? (rows + kRows - 1) / kRows : 0;
+}
+
+// All pairs, by a whole warp.
+template <int D>
+__device__ __forceinline__ int schedule(Smem<D>& sm, const PagedParams& p, int numbers) {
     const int lane = threadIdx.x % 32;
-    if (p.requests <= 32) {
-        // a request a lane, the longest first; a request's last pairs see the most keys
-        const bool there = lane < p.requests;
-        const PagedRequest at = there ? PagedRequest(p, lane) : PagedRequest(0, 0, 0, false);
-        const int rows = at.n * p.group, mine = rows > p.few_rows ? (rows + kRows - 1) / kRows : 0;
-        const int keys = there ? (p.window > 0 ? min(at.len, p.window) : at.len) : -1;
-        int before = 0;
-        for (int r = 0; r < p.requests; ++r) {
-            const int other = __shfl_sync(0xffffffffu, keys, r), count = __shfl_sync(0xffffffffu, mine, r);
-            if (other > keys || (other == keys && r < lane)) before += count;
-        }
-        const uint32_t has = __ballot_sync(0xffffffffu, there && number >= before && number < before + mine);
-        const int request = has == 0 ? 0 : __ffs(has) - 1;
-        const int pair = __shfl_sync(0xffffffffu, mine - 1 - (number - before), request);
-        return Place{has == 0 ? -1 : request, pair,
-                     PagedRequest(__shfl_sync(0xffffffffu, at.row0, request), __shfl_sync(0xffffffffu, at.n, request),
-                                  __shfl_sync(0xffffffffu, at.len, request), __shfl_sync(0xffffffffu, static_cast<int>(at.cut), request) != 0)};
+    if (p.requests > kCounted) return numbers;
+    if (p.requests > kOrdered) {
+        int sum = 0;
+        for (int r = lane; r < p.requests; r += 32) sum += pairs_of<tiles<D>()>(p, PagedRequest(p, r));
+        return __reduce_add_sync(0xffffffffu, sum);
     }
-    // More requests: numbered over the batch with gaps, request r from floor(first row / rows of a pair) + r on, which leaves room
-    // for its last, partial one; the last request that begins at or before the number, found 32 candidates at a time.
-    const int wanted = pairs - 1 - number;
+    const bool there = lane < p.requests;
+    const PagedRequest at = there ? PagedRequest(p, lane) : PagedRequest(0, 0, 0, false);
+    const int mine = pairs_of<tiles<D>()>(p, at), keys = there ? (p.window > 0 ? min(at.len, p.window) : at.len) : -1;
+    int before = 0;
+    for (int r = 0; r < p.requests; ++r) {
+        const int other = __shfl_sync(0xffffffffu, keys, r), count = __shfl_sync(0xffffffffu, mine, r);
+        if (other > keys || (other == keys && r < lane)) before += count;
+    }
+    sm.row0[lane] = at.row0;
+    sm.n[lane] = at.n;
+    sm.len[lane] = at.len | (at.cut ? static_cast<int>(0x80000000u) : 0);
+    sm.first[lane] = before;
+    sm.count[lane] = mine;
+    return __reduce_add_sync(0xffffffffu, mine);
+}
+
+// The pair with this number, by a whole warp: its request (none: < 0) and place there.
+struct Place { int request, pair; PagedRequest at; };
+template <int D>
+__device__ __forceinline__ Place place_of(const Smem<D>& sm, const PagedParams& p, int number, int numbers) {
+    constexpr int kTiles = tiles<D>(), kRows = kTiles * kTile;
+    const int lane = threadIdx.x % 32;
+    if (p.requests <= kOrdered) {
+        const int first = sm.first[lane], count = sm.count[lane];
+        const uint32_t has = __ballot_sync(0xffffffffu, number >= first && number < first + count);
+        const int request = has == 0 ? 0 : __ffs(has) - 1, len = sm.len[request];
+        return Place{has == 0 ? -1 : request, sm.count[request] - 1 - (number - sm.first[request]),
+                     PagedRequest(sm.row0[request], sm.n[request], len & 0x7fffffff, len < 0)};
+    }
+    if (p.requests <= kCounted) {
+        int before = 0;
+        for (int r0 = 0; r0 < p.requests; r0 += 32) {
+            const PagedRequest at = r0 + lane < p.requests ? PagedRequest(p, r0 + lane) : PagedRequest(0, 0, 0, false);
+            const int count = pairs_of<kTiles>(p, at);
+            int upto = count;
+#pragma unroll
+            for (int off = 1; off < 32; off *= 2) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, off);
+                if (lane >= off) upto += v;
+            }
+            const int first = before + upto - count;
+            const uint32_t has = __ballot_sync(0xffffffffu, number >= first && number < first + count);
+            if (has != 0) {
+                const int from = __ffs(has) - 1;
+                return Place{r0 + from, __shfl_sync(0xffffffffu, count - 1 - (number - first), from),
+                             PagedRequest(__shfl_sync(0xffffffffu, at.row0, from), __shfl_sync(0xffffffffu, at.n, from),
+                                          __shfl_sync(0xffffffffu, at.len, from), __shfl_sync(0xffffffffu, static_cast<int>(at.cut), from) != 0)};
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        return Place{-1, 0, PagedRequest(0, 0, 0, false)};
+    }
+    // the last request that begins at or before the number, found 32 candidates at a time
+    const int wanted = numbers - 1 - number;
     int lo = 0, hi = p.requests, begin = 0;      // begin(lo) <= wanted < begin(hi)
     while (hi - lo > 1) {
         const int step = (hi - lo + 31) / 32, r = lo + lane * step;
@@ -174,10 +227,11 @@ __device__ __forceinline__ Place place_of(const PagedParams& p, int number, int 
 // 2300.  Two prompts of 7.2 k tokens, 16 / 4 heads of 128: 425 to 440 us, 1 PFLOP/s (the few-row kernel in the same place: 4.6 ms);
 // 512 tokens over 32 000, 16 / 2 heads: 134 to 141 us, 1 PFLOP/s (764 us).  Nine chunks of 5 to 561 tokens, 16 heads of 64,
 // window 1024: 25 us, the latency of the longest block (32.8 with the requests in their own order).
-template <typename T, int D>
+template <typename T, int D, bool kLoop>
 __global__ void __launch_bounds__(threads<D>(), 3 - tiles<D>())
 paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p,
-                             const int pairs, const int shares, float2* __restrict__ part_ml, float* __restrict__ part_out) {
+                             const int pairs, const int most_shares, const unsigned slots, int* share_count, float2* __restrict__ part_ml,
+                             float* __restrict__ part_out) {
     extern __shared__ __align__(1024) uint8_t chunk_raw[];             // (the swizzled atoms need it)
     constexpr int kHalves = D / 64, kSlots = ring_slots<D>(), kSlotBytes = kHalves * kAtom, kTiles = tiles<D>(), kSoftmaxWarps = softmax_warps<D>();
     constexpr uint32_t kColumns = 256 * kTiles;                 // of tensor memory: S and O of the tiles
@@ -190,8 +244,8 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             mbar_init(&sm.full[s], 1);
             mbar_init(&sm.empty[s], 1);
         }
-        mbar_init(&sm.q_ready, kSoftmaxWarps);
         for (int t = 0; t < kTiles; ++t) {
+            mbar_init(&sm.q_ready[t], kTileWarps);
             mbar_init(&sm.s_full[t], 1);
             mbar_init(&sm.p_full[t], kTileWarps);
             mbar_init(&sm.o_done[t], 1);
@@ -204,35 +258,61 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         tmem_alloc(&sm.tmem, kColumns);
         tmem_relinquish();
     }
+    grid_dependency_wait();
+    grid_dependents_launch();                   // (only now: the few-row kernel behind this one does not wait for what is in front of it)
+    // Items of work: pair of tiles, key-value head and share of the keys, shared out where there are fewer pairs than blocks.
+    if (warp == 0) {
+        const int all = schedule(sm, p, pairs);
+        if (lane == 0) {
+            const unsigned columns = static_cast<unsigned>(all) * p.kv_heads;
+            sm.shares = max(min(static_cast<unsigned>(most_shares), slots / max(columns, 1u)), 1u);
+            sm.items = columns * sm.shares;
+            if (blockIdx.x == 0 && most_shares > 1) *share_count = sm.shares;
+        }
+    }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = sm.tmem;
-    grid_dependency_wait();
-    grid_dependents_launch();                   // (only now: the few-row kernel behind this one does not wait for what is in front of it)
-
-    const int head = blockIdx.x % p.kv_heads, share = blockIdx.x / p.kv_heads % shares;
-    const Place place = place_of<kTiles>(p, blockIdx.x / p.kv_heads / shares, pairs);
-    const int request = place.request;
-    Work<kTiles> w(p, place.at, request, head, place.pair);
-    const bool mine = request >= 0;
-    const int blocks = w.to - w.from;
-    // a share is two blocks of keys at least
-    const int parts = max(min(shares, blocks / 2), 1);
-    if (share >= parts) w.from = w.to;
-    else {
-        const int from = w.from;
-        w.from = from + static_cast<int>(static_cast<long long>(blocks) * share / parts);
-        w.to = from + static_cast<int>(static_cast<long long>(blocks) * (share + 1) / parts);
-    }
+    const unsigned shares = sm.shares;
+    // Every role goes through the block's items: f(work, request, head, share).  One item where the grid has a block for each that
+    // may exist, else the block's place in each pass over the grid, the passes forwards and backwards in turn, so that who has
+    // the longest of one has the shortest of the next.
+    auto one_item = [&](unsigned item, auto&& f) {
+        if (item >= sm.items) return;
+        // (shares of a column lie side by side: they read the same queries)
+        const unsigned column = item / shares;
+        const int share = static_cast<int>(item - column * shares), number = static_cast<int>(column / p.kv_heads), head = static_cast<int>(column - number * p.kv_heads);
+        const Place place = place_of(sm, p, number, pairs);
+        if (place.request < 0) return;
+        Work<kTiles> w(p, place.at, place.request, head, place.pair);
+        // a share is two blocks of keys at least
+        const int blocks = w.to - w.from, parts = max(min(static_cast<int>(shares), blocks / 2), 1), from = w.from;
+        if (share >= parts) w.from = w.to;
+        else {
+            w.from = from + static_cast<int>(static_cast<long long>(blocks) * share / parts);
+            w.to = from + static_cast<int>(static_cast<long long>(blocks) * (share + 1) / parts);
+        }
+        f(w, place.request, head, share);
+    };
+    auto each_item = [&](auto&& f) {
+        if constexpr (!kLoop) one_item(blockIdx.x, f);
+        else {
+#pragma unroll 1
+            for (unsigned base = 0, back = 0; base < sm.items; base += gridDim.x, back ^= 1)
+                one_item(base + (back ? gridDim.x - 1 - blockIdx.x : blockIdx.x), f);
+        }
+    };
     bool ok = true;
-    if (mine) {
     if (warp == kSoftmaxWarps) {
         // ------------------------------------------------------------ TMA
         const int box = min(kBox, 1 << p.page_shift), boxes = kTile / box;         // boxes: up to 8
+        int it = 0;
+        bool bad = false;
+        each_item([&](const Work<kTiles>& w, int request, int head, int) {
         const int* table = p.table + static_cast<long long>(request) * p.max_pages;
-        int it = 0, held = -32, id = 0;
-        bool bad = w.at.cut;
+        int held = -32, id = 0;
+        bad |= w.at.cut;
         for (int b = w.from; ok && b < w.to; ++b) {
             const int key = b * kTile + min(lane, boxes - 1) * box, page = key >> p.page_shift;
             if (((b * kTile + kTile - 1) >> p.page_shift) >= held + 32) {
@@ -261,6 +341,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 __syncwarp();
             }
         }
+        });
         if (bad && p.status != nullptr) atomicOr(p.status, PK100_STATUS_PAGE);
         // copies still in flight where a wait ran out: they must land before the block's memory is given away
         if (!ok || *abort_flag != 0) {
@@ -278,6 +359,11 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                                 (64ull << 32) | (1ull << 46) | (2ull << 61);
         auto k_offset = [](int ks) { return static_cast<uint32_t>((ks / 4) * (kAtom / 16) + 2 * (ks % 4)); };
         const bool leader = elect_one();
+        uint32_t phase[kTiles] = {};                         // parity of the tile's next block
+        uint32_t q_phase = 0;                                // of the next item with blocks
+        int it = 0;                                          // ring position of the block's keys; its values follow
+        each_item([&](const Work<kTiles>& w, int, int, int) {
+        if (!ok || w.from >= w.to) return;
         int tile_from[kTiles], tile_to[kTiles];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
@@ -292,18 +378,17 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                                     idesc_s, ks > 0);
             tc_commit_if(leader, &sm.s_full[t]);
         };
-        uint32_t phase[kTiles] = {};                     // parity of the tile's next block
         uint32_t filled[kTiles] = {};                    // O holds something
-        int it = 0;                                          // ring position of the block's keys; its values follow
         do {
-            if (w.from >= w.to) break;
-            CHUNK_WAIT(sm.q_ready, 0);
-            CHUNK_WAIT(sm.full[0], 0);
+            for (int t = 0; ok && t < kTiles; ++t) CHUNK_WAIT(sm.q_ready[t], q_phase);
+            if (!ok) break;
+            q_phase ^= 1;
+            CHUNK_WAIT(sm.full[it % kSlots], (it / kSlots) & 1);
             tc_fence_after_sync();
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
-                if (active(t, w.from)) scores(t, 0);
-            tc_commit_if(leader, &sm.empty[0]);
+                if (active(t, w.from)) scores(t, it % kSlots);
+            tc_commit_if(leader, &sm.empty[it % kSlots]);
 #pragma unroll 1
             for (int b = w.from; b < w.to; ++b, it += 2) {
                 const int v_slot = (it + 1) % kSlots, k_slot = (it + 2) % kSlots;
@@ -348,35 +433,41 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 tc_commit_if(leader, &sm.empty[v_slot]);
                 if (b + 1 < w.to) tc_commit_if(leader, &sm.empty[k_slot]);
             }
-            // the last arrival of the tensor cores comes before the block leaves
-            if (ok) CHUNK_WAIT(sm.empty[(it - 1) % kSlots], ((it - 1) / kSlots) & 1);
         } while (false);
+        });
+        // the last arrival of the tensor cores comes before the block leaves
+        if (ok && it > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sm.empty[(it - 1) % kSlots], ((it - 1) / kSlots) & 1, abort_flag)) != 0;
     } else {
         // ------------------------------------------------------------ softmax: half a row a thread
         const int t = warp / kTileWarps, half = (warp / 4) % 2, quad = warp % 4, tile_row = quad * 32 + lane;
-        {   // the queries of both tiles: 16 bytes a thread, rows that do not exist are zeros
-            constexpr int kChunks = D / 8, kEach = kTiles * kTile * kChunks / (kSoftmaxWarps * 32);
+        // the two warps of a quadrant of a tile
+        auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + quad) : "memory"); };
+        int before = 0;                                      // blocks of this tile in the items so far
+        each_item([&](const Work<kTiles>& w, int, int head, int share) {
+        if (w.from < w.to) {
+            // the tile's queries, 16 bytes a thread, rows that do not exist are zeros (the scores that the ones before were
+            // multiplied for have been read)
+            constexpr int kChunks = D / 8, kThreads = kTileWarps * 32, kEach = kTile * kChunks / kThreads;
+            const int thread = tid % kThreads;
             const uint32_t sign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;      // a negative scale turns the queries round
             uint4 v[kEach];                                  // (all requested before the first is stored)
 #pragma unroll
             for (int j = 0; j < kEach; ++j) {
-                const int r = (tid + j * kSoftmaxWarps * 32) / kChunks, index = w.row + r, token = index / p.group;
+                const int r = t * kTile + (thread + j * kThreads) / kChunks, index = w.row + r, token = index / p.group;
                 v[j] = r < w.rows ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.query) + (w.at.row0 + token) * p.ld_query +
-                                                                    static_cast<long long>(head * p.group + index - token * p.group) * D + tid % kChunks * 8)
+                                                                    static_cast<long long>(head * p.group + index - token * p.group) * D + thread % kChunks * 8)
                                   : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
             for (int j = 0; j < kEach; ++j) {
-                const int r = (tid + j * kSoftmaxWarps * 32) / kChunks, c = tid % kChunks, q_row = r % kTile;
-                *reinterpret_cast<uint4*>(sm.q[r / kTile][c / 8] + q_row * 128 + (((c % 8) ^ (q_row & 7)) << 4)) =
+                const int c = thread % kChunks, q_row = (thread + j * kThreads) / kChunks;
+                *reinterpret_cast<uint4*>(sm.q[t][c / 8] + q_row * 128 + (((c % 8) ^ (q_row & 7)) << 4)) =
                     make_uint4(v[j].x ^ sign, v[j].y ^ sign, v[j].z ^ sign, v[j].w ^ sign);
             }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.q_ready);
+            if (lane == 0) mbar_arrive(&sm.q_ready[t]);
         }
-        // the two warps of a quadrant of a tile
-        auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + quad) : "memory"); };
         const int index = w.row + t * kTile + tile_row, token = index / p.group;
         const bool live = t * kTile + tile_row < w.rows;
         const int row_lo = w.at.lo(p, token), row_hi = live ? w.at.hi(p, token) : 0;
@@ -391,7 +482,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         int done = 0;                                        // blocks of this tile
         // (a wait that ran out does not end the loop: the other warp of the pair would wait at the barrier for ever)
         for (int b = w.tile_from(p, t), end = w.tile_to(p, t); b < end; ++b, ++done) {
-            ok &= __all_sync(0xffffffffu, mbar_wait_bounded(&sm.s_full[t], done & 1, abort_flag)) != 0;
+            ok &= __all_sync(0xffffffffu, mbar_wait_bounded(&sm.s_full[t], (before + done) & 1, abort_flag)) != 0;
             tc_fence_after_sync();
             float s[64];
             tmem_ld_32x32(s_cols, reinterpret_cast<uint32_t(&)[32]>(s[0]));
@@ -419,7 +510,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 m = seen;
                 l *= factor;
                 if (done > 0) {
-                    ok &= __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], (done - 1) & 1, abort_flag)) != 0;
+                    ok &= __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], (before + done - 1) & 1, abort_flag)) != 0;
                     tc_fence_after_sync();
 #pragma unroll 1
                     for (int c = 0; c < D / 2; c += 16) {
@@ -433,21 +524,23 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 }
             }
             const float shift = m == -INFINITY ? 0.0f : -m * scale;
-            l += masked ? weights_of_scores<T, 0>(s, scale, shift, p_cols) : weights_of_scores<T, kByFma>(s, scale, shift, p_cols);
+            l += weights_of_scores<T, kByFma>(s, scale, shift, p_cols);
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.p_full[t]);
         }
         // ------------------------------------------------------------ output: half the features a thread
+        if (m == -INFINITY) l = 0.0f;                        // (nothing seen: masked scores count 2^-126 on the FMA pipe)
         pair_sync();
         sm.top[t][half][tile_row] = l;
         pair_sync();
         l += sm.top[t][half ^ 1][tile_row];
         if (ok && done > 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], (done - 1) & 1, abort_flag)) != 0;
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], (before + done - 1) & 1, abort_flag)) != 0;
             tc_fence_after_sync();
         }
+        before += done;
         if (ok && tile_rows > 0) {
             const long long row = static_cast<long long>(w.at.row0 + token) * p.heads + head * p.group + index - token * p.group;
             const float inverse = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
@@ -483,7 +576,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 else if (p.lse != nullptr) p.lse[row] = l > 0.0f ? (m * scale + log2f(l)) * kLn2 : (l == 0.0f ? -INFINITY : l);
             }
         }
-    }
+        });
     }
     if (!ok && lane == 0 && p.status != nullptr) atomicOr(p.status, 1);
     tc_fence_before_sync();
@@ -494,9 +587,11 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
 // out of the shares of a row's keys, in their order, a warp a row.
 template <typename T, int D>
 __global__ void __launch_bounds__(128)
-shares_join_kernel(const PagedParams p, const int shares, const float2* __restrict__ part_ml, const float* __restrict__ part_out) {
+shares_join_kernel(const PagedParams p, const int* share_count, const float2* __restrict__ part_ml, const float* __restrict__ part_out) {
     grid_dependents_launch();
     grid_dependency_wait();
+    const int shares = *share_count;
+    if (shares == 1) return;                     // (the rows are finished)
     const int token = blockIdx.x, lane = threadIdx.x % 32;
     // the request that has the token: the last one that starts at or before it (an empty one never is)
     int lo = 0, hi = p.requests;
@@ -536,40 +631,48 @@ shares_join_kernel(const PagedParams p, const int shares, const float2* __restri
 }
 
 template <typename T, int D>
-static int launch(const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares, float2* part_ml,
+static int launch(const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares, int* share_count, float2* part_ml,
                   float* part_out, cudaStream_t stream) {
-    constexpr auto kernel = paged_attention_chunk_kernel<T, D>;
     constexpr int bytes = sizeof(Smem<D>);
     static_assert(bytes <= 227 * 1024 / (3 - tiles<D>()) - (D == 64 ? 1024 : 0), "shared memory");
-    const cudaError_t granted = pk100_grant_smem<kernel>(bytes);
-    if (granted != cudaSuccess) return static_cast<int>(granted);
-    pk100_launch_chained(kernel, dim3(static_cast<unsigned>(pairs) * shares * p.kv_heads), dim3(threads<D>()), bytes, stream, map_k, map_v, p, pairs, shares,
-                         part_ml, part_out);
-    return pk100_launch_status();
+    const long long slots = pk100_sm_count() * (3 - tiles<D>()), columns = static_cast<long long>(pairs) * p.kv_heads;
+    // Up to 32 requests at most 32 pairs a head do not exist: a block for each that may.  With more, blocks that find nothing to
+    // do would cost more than the pass over the items (200 single tokens whose max_new is not known: 207 against 167 us).
+    auto run = [&](auto loop) -> int {
+        constexpr auto kernel = paged_attention_chunk_kernel<T, D, decltype(loop)::value>;
+        const cudaError_t granted = pk100_grant_smem<kernel>(bytes);
+        if (granted != cudaSuccess) return static_cast<int>(granted);
+        const long long most = columns * shares < slots ? columns * shares : slots, blocks = decltype(loop)::value || columns < most ? most : columns;
+        pk100_launch_chained(kernel, dim3(static_cast<unsigned>(blocks)), dim3(threads<D>()), bytes, stream, map_k, map_v, p, pairs, shares,
+                             static_cast<unsigned>(slots), share_count, part_ml, part_out);
+        return pk100_launch_status();
+    };
+    return p.requests <= kOrdered ? run(std::false_type()) : run(std::true_type());
 }
 
 template <typename T, int D>
-static int launch_join(const PagedParams& p, int shares, const float2* part_ml, const float* part_out, cudaStream_t stream) {
-    pk100_launch_chained(shares_join_kernel<T, D>, dim3(p.tokens, (p.heads + 3) / 4 < 8 ? (p.heads + 3) / 4 : 8), dim3(128), 0, stream, p, shares, part_ml, part_out);
+static int launch_join(const PagedParams& p, const int* share_count, const float2* part_ml, const float* part_out, cudaStream_t stream) {
+    pk100_launch_chained(shares_join_kernel<T, D>, dim3(p.tokens, (p.heads + 3) / 4 < 8 ? (p.heads + 3) / 4 : 8), dim3(128), 0, stream, p, share_count, part_ml,
+                         part_out);
     return pk100_launch_status();
 }
 
 }  // namespace chunk
 
 int paged_attention_chunks(int type, int head_dim, const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares,
-                           float2* part_ml, float* part_out, cudaStream_t stream) {
+                           int* share_count, float2* part_ml, float* part_out, cudaStream_t stream) {
     if (type == PK100_TYPE_F16)
-        return head_dim == 128 ? chunk::launch<__half, 128>(p, map_k, map_v, pairs, shares, part_ml, part_out, stream)
-                               : chunk::launch<__half, 64>(p, map_k, map_v, pairs, shares, part_ml, part_out, stream);
-    return head_dim == 128 ? chunk::launch<__nv_bfloat16, 128>(p, map_k, map_v, pairs, shares, part_ml, part_out, stream)
-                           : chunk::launch<__nv_bfloat16, 64>(p, map_k, map_v, pairs, shares, part_ml, part_out, stream);
+        return head_dim == 128 ? chunk::launch<__half, 128>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_out, stream)
+                               : chunk::launch<__half, 64>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_out, stream);
+    return head_dim == 128 ? chunk::launch<__nv_bfloat16, 128>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_out, stream)
+                           : chunk::launch<__nv_bfloat16, 64>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_out, stream);
 }
 
-int paged_attention_join(int type, int head_dim, const PagedParams& p, int shares, const float2* part_ml, const float* part_out, cudaStream_t stream) {
+int paged_attention_join(int type, int head_dim, const PagedParams& p, const int* share_count, const float2* part_ml, const float* part_out, cudaStream_t stream) {
     if (type == PK100_TYPE_F16)
-        return head_dim == 128 ? chunk::launch_join<__half, 128>(p, shares, part_ml, part_out, stream) : chunk::launch_join<__half, 64>(p, shares, part_ml, part_out, stream);
-    return head_dim == 128 ? chunk::launch_join<__nv_bfloat16, 128>(p, shares, part_ml, part_out, stream)
-                           : chunk::launch_join<__nv_bfloat16, 64>(p, shares, part_ml, part_out, stream);
+        return head_dim == 128 ? chunk::launch_join<__half, 128>(p, share_count, part_ml, part_out, stream) : chunk::launch_join<__half, 64>(p, share_count, part_ml, part_out, stream);
+    return head_dim == 128 ? chunk::launch_join<__nv_bfloat16, 128>(p, share_count, part_ml, part_out, stream)
+                           : chunk::launch_join<__nv_bfloat16, 64>(p, share_count, part_ml, part_out, stream);
 }
 
 }  // namespace pk100
