@@ -360,7 +360,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         auto k_offset = [](int ks) { return static_cast<uint32_t>((ks / 4) * (kAtom / 16) + 2 * (ks % 4)); };
         const bool leader = elect_one();
         uint32_t phase[kTiles] = {};                         // parity of the tile's next block
-        uint32_t q_phase = 0;                                // of the next item with blocks
+        uint32_t q_phase[kTiles] = {};                       // of the tile's next item with blocks
         int it = 0;                                          // ring position of the block's keys; its values follow
         each_item([&](const Work<kTiles>& w, int, int, int) {
         if (!ok || w.from >= w.to) return;
@@ -380,9 +380,13 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         };
         uint32_t filled[kTiles] = {};                    // O holds something
         do {
-            for (int t = 0; ok && t < kTiles; ++t) CHUNK_WAIT(sm.q_ready[t], q_phase);
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+                if (ok && tile_from[t] < tile_to[t]) {
+                    CHUNK_WAIT(sm.q_ready[t], q_phase[t]);
+                    q_phase[t] ^= 1;
+                }
             if (!ok) break;
-            q_phase ^= 1;
             CHUNK_WAIT(sm.full[it % kSlots], (it / kSlots) & 1);
             tc_fence_after_sync();
 #pragma unroll
@@ -444,7 +448,8 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + quad) : "memory"); };
         int before = 0;                                      // blocks of this tile in the items so far
         each_item([&](const Work<kTiles>& w, int, int head, int share) {
-        if (w.from < w.to) {
+        // (a tile without blocks brings no queries: its warps, which nothing holds back, would run ahead of the barrier's phases)
+        if (w.tile_from(p, t) < w.tile_to(p, t)) {
             // the tile's queries, 16 bytes a thread, rows that do not exist are zeros (the scores that the ones before were
             // multiplied for have been read)
             constexpr int kChunks = D / 8, kThreads = kTileWarps * 32, kEach = kTile * kChunks / kThreads;

@@ -533,6 +533,19 @@ def test_attention_of_a_mixed_step_captured(pk, cuda, dim):
         s.check(out)
 
 
+@pytest.mark.parametrize("dim,kv", [(128, 8), (64, 8)])
+@pytest.mark.parametrize("requests", [40, 300])
+def test_attention_of_more_chunks_than_blocks(pk, cuda, requests, dim, kv):
+    """More than 32 requests, each block of threads takes several; chunks that fill one tile of a pair, both, or neither."""
+    new = [(20, 130, 9, 20, 3, 64)[i % 6] for i in range(requests)]
+    cached = [(7 * i) % 200 for i in range(requests)]
+    s, status = Step(new, cached, 2 * kv, kv, dim, 16, F16, seed=requests), _int([0])
+    out = s.run(pk, status=status)
+    assert int(status) == 0
+    s.check(out)
+    assert torch.equal(s.run(pk), out)
+
+
 @pytest.mark.parametrize("dim,kv", [(128, 2), (64, 4)])
 def test_attention_of_single_tokens_beside_chunks(pk, cuda, dim, kv):
     """The kernels for single tokens and for chunks run side by side: the same bits every time, and what each request gets
