@@ -606,6 +606,25 @@ def test_calls_on_two_streams_at_once(pk, cuda):
     assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
 
 
+def test_kernels_of_all_kinds_on_streams_at_once(pk, cuda):
+    """Chunks of both head widths, single tokens, the wide INT4 product and the norm beside each other: tensor memory, shared
+    memory and workspaces are each call's own, the bits those of a call alone."""
+    codes, scales = _packed(20000, 1024, 1, cuda)
+    x, g, r = _normal(2, 5, 1024), _normal(3, 1024), _normal(4, 5, 1024)
+    a, b, c = Step([300, 5], [900, 3], 8, 2, 128, 32, F16, seed=1), Step([400], [0], 8, 8, 64, 16, BF16, seed=2), Step([1] * 9, [500] * 9, 8, 1, 128, 64, F16, seed=3)
+    calls = [lambda: a.run(pk), lambda: b.run(pk), lambda: c.run(pk), lambda: pk.ops.gemv_w4g128(x, codes, scales), lambda: pk.ops.add_rms_norm(x, g, residual=r)[0]]
+    want = [f().clone() for f in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    got = [[] for _ in calls]
+    for _ in range(15):
+        for i, (f, stream) in enumerate(zip(calls, streams)):
+            with torch.cuda.stream(stream):
+                got[i].append(f())
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(len(calls)) for o in got[i])
+
+
 def test_attention_refuses(pk, cuda):
     s = Step([1], [20], 8, 2, 128, 16, F16)
     with pytest.raises(ValueError):
