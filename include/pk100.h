@@ -683,7 +683,7 @@ int pk100_gemv_w4g128(void* stream, const pk100_gemm_args* args);
  * Rows t >= starts[requests] get slot and position -1.  Where the step does not fit (a negative length, more new
  * tokens than `tokens`, more pages than *free_count, free_capacity or max_pages) nothing is taken: PK100_STATUS_PLAN is set in
  * *status, starts and *used are 0, lengths = cached, every slot and position -1, block_table as it was.  At most
- * PK100_PLAN_MAX_REQUESTS requests (PK100_ERR_LIMIT).  Outputs overlap no input (lengths equal to cached or
+ * PK100_PLAN_MAX_REQUESTS requests and 2^30 tokens (PK100_ERR_LIMIT).  Outputs overlap no input (lengths equal to cached or
  * new_tokens is refused). */
 #define PK100_PLAN_MAX_REQUESTS 4096
 typedef struct pk100_paged_plan_args {

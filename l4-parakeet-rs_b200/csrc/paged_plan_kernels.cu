@@ -147,7 +147,7 @@ using namespace pk100;
 extern "C" int pk100_paged_plan(void* stream, const pk100_paged_plan_args* a) {
     if (a == nullptr) return PK100_ERR_NULL;
     if (a->requests < 0 || a->tokens < 0 || a->page_size <= 0 || a->max_pages <= 0 || a->free_capacity < 0) return PK100_ERR_SHAPE;
-    if (a->requests > PK100_PLAN_MAX_REQUESTS) return PK100_ERR_LIMIT;
+    if (a->requests > PK100_PLAN_MAX_REQUESTS || a->tokens > 1 << 30) return PK100_ERR_LIMIT;      // (rows are counted in 32 bits)
     if (a->starts == nullptr || a->used == nullptr || a->free_count == nullptr) return PK100_ERR_NULL;
     if (a->requests > 0 && (a->cached == nullptr || a->new_tokens == nullptr || a->block_table == nullptr || a->lengths == nullptr))
         return PK100_ERR_NULL;

@@ -67,6 +67,12 @@ def test_plan_refusals(pk):
     assert _plan(L, cached=258) == _plan(L, slots=5124) == _plan(L, status=2) == L.ERR_ALIGN
 
 
+def test_plan_refuses_more_rows_than_it_counts(pk):
+    # a warp's end of its run is at most the rows and 32 * 4 on top: in 32 bits up to 2^30 rows, not at the largest int
+    L = pk.lib
+    assert _plan(L, tokens=(1 << 30) + 1) == _plan(L, tokens=(1 << 31) - 1) == L.ERR_LIMIT
+
+
 def _attention(L, **changes):
     a = L.PagedAttentionArgs(type=L.TYPE_BF16, tokens=6, requests=2, heads=8, kv_heads=2, head_dim=64, pages=10, page_size=16, max_pages=4,
                              query=4096, ld_query=512, key_cache=8192, value_cache=16384, page_stride=2048, token_stride=128,
