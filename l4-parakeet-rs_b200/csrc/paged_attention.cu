@@ -600,10 +600,9 @@ extern "C" long long pk100_paged_attention_workspace_bytes(const pk100_paged_att
 extern "C" int pk100_paged_attention(void* stream_v, const pk100_paged_attention_args* a) {
     int rc = paged_check(a);
     if (rc != PK100_OK) return rc;
-    if (a->tokens == 0 || a->requests == 0) return PK100_OK;
-    if (a->query == nullptr || a->key_cache == nullptr || a->value_cache == nullptr || a->starts == nullptr || a->lengths == nullptr ||
-        a->block_table == nullptr || a->out == nullptr || a->workspace == nullptr)
-        return PK100_ERR_NULL;
+    if (a->tokens == 0 || (a->requests == 0 && a->key == nullptr)) return PK100_OK;      // (without requests new keys are written all the same)
+    if (a->query == nullptr || a->key_cache == nullptr || a->value_cache == nullptr || a->out == nullptr || a->workspace == nullptr) return PK100_ERR_NULL;
+    if (a->requests > 0 && (a->starts == nullptr || a->lengths == nullptr || a->block_table == nullptr)) return PK100_ERR_NULL;
     if (a->key != nullptr && (a->value == nullptr || a->slots == nullptr)) return PK100_ERR_NULL;
     const long long row = static_cast<long long>(a->heads) * a->head_dim, kv_row = static_cast<long long>(a->kv_heads) * a->head_dim;
     auto bad_ld = [&](long long ld, long long width) { return a->tokens > 1 && (ld < width || ld % 8 != 0); };     // (a single row has no distance)
@@ -652,7 +651,7 @@ extern "C" int pk100_paged_attention(void* stream_v, const pk100_paged_attention
         w.status = a->status;
         const long long work = a->tokens * (kv_row / 8), blocks = (work + 255) / 256, most = 8ll * pk100_sm_count();
         pk100_launch_chained(paged_append_kernel, dim3(static_cast<int>(blocks < most ? blocks : most)), dim3(256), 0, stream, w);
-        if ((rc = pk100_launch_status()) != PK100_OK) return rc;
+        if ((rc = pk100_launch_status()) != PK100_OK || a->requests == 0) return rc;
     } else {
         const cudaError_t err = cudaMemsetAsync(static_cast<uint8_t*>(a->workspace) + plan.counts, 0, plan.grid * 4ull, stream);
         if (err != cudaSuccess) return static_cast<int>(err);

@@ -391,6 +391,19 @@ def test_attention_writes_the_cache_and_nothing_else(pk, cuda):
     assert torch.equal(a, b)
 
 
+def test_attention_without_requests_writes_the_new_keys(pk, cuda):
+    key, value = _normal(90, 4, 2, 64), _normal(91, 4, 2, 64)
+    cache_k, cache_v = _normal(92, 3, 16, 2, 64), _normal(93, 3, 16, 2, 64)
+    want_k, want_v = cache_k.clone(), cache_v.clone()
+    want_k[1, 5], want_k[2, 15], want_v[1, 5], want_v[2, 15] = key[0], key[3], value[0], value[3]
+    empty = torch.zeros(0, dtype=torch.int32, device="cuda")
+    out = torch.full((4, 8, 64), 7.0, dtype=F16, device="cuda")
+    pk.ops.paged_attention(_normal(95, 4, 8, 64), cache_k, cache_v, empty.view(0, 5), torch.zeros(1, dtype=torch.int32, device="cuda"), empty, key=key,
+                           value=value, slots=torch.tensor([21, -1, -1, 47], device="cuda"), out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(cache_k, want_k) and torch.equal(cache_v, want_v) and bool((out == 7.0).all())
+
+
 def test_attention_rows_that_see_nothing(pk, cuda):
     """Lengths below the number of new tokens: the first rows stand before the first key.  No length at all."""
     s = Step([5, 200, 3], [20, 100, 0], 8, 2, 128, 16, F16)
