@@ -6,7 +6,6 @@ inside libpk100.so.  Tensors must be CUDA and contiguous where stated.
 from __future__ import annotations
 
 import functools
-import math
 import struct
 from collections import namedtuple
 
@@ -475,14 +474,14 @@ def paged_attention(query, key_cache, value_cache, block_table, starts, lengths,
     starts_at = _whole("starts", starts, (requests + 1,), i32, device)
     lengths_at = _whole("lengths", lengths, (requests,), i32, device)
     key_at = key_ld = value_at = value_ld = slots_at = 0
-    if key is not None:
-        if value is None or slots is None:
-            raise ValueError("key needs value and slots")
+    if key is not None or value is not None:
+        if key is None or value is None or slots is None:
+            raise ValueError("key, value and slots are given together")
         new_shape = (tokens, kv_heads, head_dim)
         key_at, key_ld = _heads("key", key, new_shape, dtype, device)
         value_at, value_ld = _heads("value", value, new_shape, dtype, device)
         slots_at = _whole("slots", slots, (tokens,), torch.int64, device)
-    if heads % kv_heads:
+    if not kv_heads or heads % kv_heads:
         raise ValueError(f"{heads} query heads do not share {kv_heads} key-value heads evenly")
     if out is None:
         out = torch.empty(shape, device=query.device, dtype=dtype)

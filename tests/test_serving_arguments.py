@@ -127,3 +127,31 @@ def test_wrappers_refuse_tensors_of_the_host(pk):
         ops.add_rms_norm(x.float(), x[0].float())
     with pytest.raises(ValueError):
         ops.add_rms_norm(x, x[0], mode=pk.lib.LN_S4_ROW)
+
+
+class _Placed(torch.Tensor):
+    """A tensor of the host that says it is on the current device: the wrapper's checks without a GPU."""
+    def get_device(self):
+        return 0
+
+
+def _attention_call(pk, monkeypatch, kv_heads=2, **changes):
+    placed = lambda *shape, dtype=torch.float16: torch.zeros(shape, dtype=dtype).as_subclass(_Placed)
+    monkeypatch.setattr(pk.ops, "_device", lambda t: 0)
+    args = dict(query=placed(3, 8, 64), key_cache=placed(5, 16, kv_heads, 64), value_cache=placed(5, 16, kv_heads, 64),
+                block_table=placed(1, 4, dtype=torch.int32), starts=placed(2, dtype=torch.int32), lengths=placed(1, dtype=torch.int32))
+    new = dict(key=placed(3, 2, 64), value=placed(3, 2, 64), slots=placed(3, dtype=torch.int64))
+    args.update({name: new[name] for name in changes.pop("new", ())}, **changes)
+    return pk.ops.paged_attention(**args)
+
+
+@pytest.mark.parametrize("new", [("value",), ("value", "slots"), ("key",), ("key", "value"), ("key", "slots")])
+def test_attention_wants_key_value_and_slots_together(pk, monkeypatch, new):
+    with pytest.raises(ValueError, match="together"):
+        _attention_call(pk, monkeypatch, new=new)
+
+
+@pytest.mark.parametrize("kv_heads", [0, 3])
+def test_attention_refuses_heads_that_do_not_divide(pk, monkeypatch, kv_heads):
+    with pytest.raises(ValueError, match="evenly"):
+        _attention_call(pk, monkeypatch, kv_heads=kv_heads)
