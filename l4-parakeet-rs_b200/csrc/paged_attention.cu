@@ -1,7 +1,5 @@
 // Attention of new tokens over a paged key-value cache: the copy of new keys and values into their slots, the kernel
 // for requests of few rows (single tokens), and the host side.
-#include <mutex>
-
 #include "paged_attention.cuh"
 
 namespace pk100 {
@@ -489,40 +487,15 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
 }
 
 // ------------------------------------------------------------- host
-// Tensor maps of caches, kept like those of pk100_tensor_map_2d.
-struct CacheMapKey {
-    const void* base; long long page_stride, token_stride, head_stride; int pages, page_size, kv_heads, head_dim, device;
-    bool operator==(const CacheMapKey& o) const {
-        return base == o.base && page_stride == o.page_stride && token_stride == o.token_stride && head_stride == o.head_stride &&
-               pages == o.pages && page_size == o.page_size && kv_heads == o.kv_heads && head_dim == o.head_dim && device == o.device;
-    }
-};
-struct CacheMapSlot { CacheMapKey key; CUtensorMap map; bool used; };
-
+// The tensor map of a cache: boxes of 64 features by a page or a block of keys.
 static int cache_map(CUtensorMap* map, const void* base, const pk100_paged_attention_args& a) {
-    static CacheMapSlot slots[256];
-    static std::mutex mutex;
-    int device = 0;
-    if (cudaGetDevice(&device) != cudaSuccess) device = -1;
-    const CacheMapKey key{base, a.page_stride, a.token_stride, a.head_stride, a.pages, a.page_size, a.kv_heads, a.head_dim, device};
-    const size_t hash = (reinterpret_cast<uintptr_t>(base) * 0x9E3779B97F4A7C15ull ^ (static_cast<uint64_t>(a.pages) << 20)) >> 48;
-    CacheMapSlot& slot = slots[hash % 256];
-    std::lock_guard<std::mutex> lock(mutex);
-    if (!slot.used || !(slot.key == key)) {
-        const unsigned long long dims[4] = {static_cast<unsigned long long>(a.head_dim), static_cast<unsigned long long>(a.page_size),
-                                            static_cast<unsigned long long>(a.kv_heads), static_cast<unsigned long long>(a.pages)};
-        // (an extent of one has no distance)
-        const unsigned long long strides[3] = {2ull * a.token_stride, 2ull * (a.kv_heads > 1 ? a.head_stride : a.token_stride),
-                                               2ull * (a.pages > 1 ? a.page_stride : a.token_stride)};
-        const unsigned box[4] = {64, static_cast<unsigned>(a.page_size < kBlock ? a.page_size : kBlock), 1, 1};
-        slot.used = false;
-        const int rc = pk100_tensor_map_4d(&slot.map, base, dims, strides, box);
-        if (rc != PK100_OK) return rc;
-        slot.key = key;
-        slot.used = true;
-    }
-    *map = slot.map;
-    return PK100_OK;
+    const unsigned long long dims[4] = {static_cast<unsigned long long>(a.head_dim), static_cast<unsigned long long>(a.page_size),
+                                        static_cast<unsigned long long>(a.kv_heads), static_cast<unsigned long long>(a.pages)};
+    // (an extent of one has no distance)
+    const unsigned long long strides[3] = {2ull * a.token_stride, 2ull * (a.kv_heads > 1 ? a.head_stride : a.token_stride),
+                                           2ull * (a.pages > 1 ? a.page_stride : a.token_stride)};
+    const unsigned box[4] = {64, static_cast<unsigned>(a.page_size < kBlock ? a.page_size : kBlock), 1, 1};
+    return pk100_tensor_map_4d(map, base, dims, strides, box);
 }
 
 // Where the workspace's arrays lie.
