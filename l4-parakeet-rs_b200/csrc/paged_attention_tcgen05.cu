@@ -37,31 +37,33 @@ struct Smem {
 template <typename T> __host__ __device__ constexpr uint32_t type_bits() { return 0; }                                    // kind::f16 operands: fp16
 template <> __host__ __device__ constexpr uint32_t type_bits<__nv_bfloat16>() { return (1u << 7) | (1u << 10); }
 
-__device__ __forceinline__ float max_of(float a, float b, float c) {
+__device__ __forceinline__ float max_of(float a, float b, float c) {          // (NaN where one of them is)
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 
-// 2^x for two values at most 9: n = rint(x), a polynomial of the remainder (minimax of the relative error, degree 3: 7.5e-5,
-// a sixth of half a step of an fp16 P), n into the exponent.  x below -126 counts as -126.  On the FMA pipe, where
-// ex2.approx (16 a clock and SM) would take as long as the tensor cores' products.
+// 2^x for two values at most 9: n = rint(x), a polynomial of the remainder (minimax of the relative error among those of
+// degree 3 that are 1 at 0: 1.01e-4, a fifth of half a step of an fp16 P), n into the exponent.  x below -127 counts as -127,
+// where 1 less 127 in the exponent is zero to the bit: a masked score has no weight at all (and between -127 and -126 no result
+// is below zero or above 2^-126).  NaN counts as -127, too.  On the FMA pipe, where ex2.approx (16 a clock and SM) would take as
+// long as the tensor cores' products.
 __device__ __forceinline__ Pair exp2_fma(Pair x) {
     const float2 v = halves_of(x);
-    x = pair_of(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
+    x = pair_of(fmaxf(v.x, -127.0f), fmaxf(v.y, -127.0f));
     const Pair magic = pair_of(12582912.0f, 12582912.0f), back = pair_of(-12582912.0f, -12582912.0f);       // 1.5 * 2^23
     const Pair n = pair_add(x, magic);
     const Pair r = pair_fma(pair_add(n, back), pair_of(-1.0f, -1.0f), x);
-    Pair y = pair_fma(r, pair_of(0.0551716685295105f, 0.0551716685295105f), pair_of(0.2426111251115799f, 0.2426111251115799f));
-    y = pair_fma(r, y, pair_of(0.6932609677314758f, 0.6932609677314758f));
-    y = pair_fma(r, y, pair_of(0.9999280571937561f, 0.9999280571937561f));
+    Pair y = pair_fma(r, pair_of(0.055009059607982635f, 0.055009059607982635f), pair_of(0.2422109693288803f, 0.2422109693288803f));
+    y = pair_fma(r, y, pair_of(0.6932829022407532f, 0.6932829022407532f));
+    y = pair_fma(r, y, pair_of(1.0f, 1.0f));
     const float2 whole = halves_of(n), part = halves_of(y);
     return pair_of(__uint_as_float(__float_as_uint(part.x) + (__float_as_uint(whole.x) << 23)),
                    __uint_as_float(__float_as_uint(part.y) + (__float_as_uint(whole.y) << 23)));
 }
 
 // P = exp2(s * scale + shift) of 64 scores, stored as 16-bit pairs; the sum of the unrounded values.  ByFma: of 16 pairs
-// of scores, how many go to the FMA pipe, where a masked score's -infinity gives 2^-126: nothing beside a sum of at least 1.
+// of scores, how many go to the FMA pipe.
 template <typename T, int ByFma>
 __device__ __forceinline__ float weights_of_scores(const float (&s)[64], float scale, float shift, uint32_t p_cols) {
     const Pair scale2 = pair_of(scale, scale), shift2 = pair_of(shift, shift);
@@ -505,7 +507,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             for (int i = 4; i < 60; i += 8)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) top[j] = max_of(top[j], s[i + 2 * j], s[i + 2 * j + 1]);
-            const float own = max_of(max_of(top[0], s[60], s[61]), max_of(top[1], s[62], s[63]), fmaxf(top[2], top[3]));
+            const float own = max_of(max_of(top[0], s[60], s[61]), max_of(top[1], s[62], s[63]), max_of(top[2], top[3], top[3]));
             sm.top[t][half][tile_row] = own;                 // (the partner has read the last one: S of this block came after its P)
             pair_sync();                                     // (also: both halves of S have been read, P may take their place)
             const float seen = fmaxf(m, fmaxf(own, sm.top[t][half ^ 1][tile_row]));
@@ -530,13 +532,13 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             }
             const float shift = m == -INFINITY ? 0.0f : -m * scale;
             l += weights_of_scores<T, kByFma>(s, scale, shift, p_cols);
+            if (!(own < INFINITY)) l = NAN;                  // (a score that is NaN or infinity makes the row NaN)
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.p_full[t]);
         }
         // ------------------------------------------------------------ output: half the features a thread
-        if (m == -INFINITY) l = 0.0f;                        // (nothing seen: masked scores count 2^-126 on the FMA pipe)
         pair_sync();
         sm.top[t][half][tile_row] = l;
         pair_sync();

@@ -572,6 +572,54 @@ def test_attention_of_single_tokens_beside_chunks(pk, cuda, dim, kv):
         assert torch.equal(s.run(pk), want)
 
 
+def _one_request(tokens, heads, dim, dtype, seed):
+    """Every head its own key-value head, pages of 64 in order, one request without a past."""
+    pages = -(-tokens // 64)
+    q, k, v = (_normal(seed + i, tokens, heads, dim, dtype=dtype) for i in range(3))
+    caches = [torch.zeros(pages, 64, heads, dim, dtype=dtype, device="cuda") for _ in range(2)]
+    rest = dict(block_table=_int([list(range(pages))]), starts=_int([0, tokens]), lengths=_int([tokens]),
+                slots=torch.arange(tokens, device="cuda"))
+    return q, k, v, lambda pk, k, v, **kw: pk.ops.paged_attention(q, *caches, key=k, value=v, **rest, **kw)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("tokens", [3, 150])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_keys_that_are_not_finite(pk, cuda, dim, tokens, dtype):
+    """A key of NaN at another place in each head: the rows that see it are no numbers, the others as they were."""
+    heads = 130 if tokens > 100 else tokens
+    q, k, v, run = _one_request(tokens, heads, dim, dtype, 300)
+    before = run(pk, k, v)
+    bad = k.clone()
+    for h in range(heads):
+        bad[h, h, 5] = math.nan
+    lse = torch.empty(tokens, heads, device="cuda")
+    out = run(pk, bad, v, lse=lse)
+    sees = torch.arange(tokens, device="cuda")[:, None] >= torch.arange(heads, device="cuda")[None]
+    assert bool(out[sees].isnan().all()) and bool(lse[sees].isnan().all())
+    assert torch.equal(out[~sees], before[~sees]) and bool(lse[~sees].isfinite().all())
+    # plus infinity where the query's sign agrees: no number either; minus infinity: a key of no weight
+    bad = k.clone()
+    for h in range(heads):
+        bad[h, h, 5] = math.inf
+    out = run(pk, bad, v)
+    up = sees & (q[:, :, 5] > 0)
+    assert not bool(out[up].isfinite().any())
+    assert bool(out[~up & (torch.arange(tokens, device="cuda")[:, None] > 0) & (torch.arange(heads, device="cuda")[None] > 0)].isfinite().all())
+
+
+@pytest.mark.parametrize("tokens", [3, 150])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_largest_values_that_a_row_does_not_see(pk, cuda, dim, tokens):
+    """A masked key has no weight, not a small one: the type's largest value behind a row changes nothing in it."""
+    q, k, v, run = _one_request(tokens, 2, dim, BF16, 310)
+    before = run(pk, k, v)
+    for first in range(1, tokens, 7 if tokens > 100 else 1):
+        large = v.clone()
+        large[first:] = torch.finfo(BF16).max
+        assert torch.equal(run(pk, k, large)[:first], before[:first]), first
+
+
 @pytest.mark.parametrize("n,k", [(1000, 1024), (20000, 1024)])
 def test_gemv_captured_and_under_a_cap(pk, cuda, n, k):
     codes, scales = _packed(n, k, 1, cuda)
