@@ -716,7 +716,8 @@ int pk100_paged_plan(void* stream, const pk100_paged_plan_args* args);
  * two tokens never share one); the caches are not written otherwise.
  * What is behind lengths[r] in a page, and pages behind it, may hold anything, infinities and NaN included; keys and
  * values in front of it are multiplied by zero weights too, so a value that is not finite reaches the rows of its
- * request that do not see it.  A page id outside [0, pages) reads as zeros, a slot outside the cache is not
+ * request that do not see it, and a key that is not finite makes the rows that see it NaN (unless it scores -infinity).
+ * A page id outside [0, pages) reads as zeros, a slot outside the cache is not
  * written, a length beyond max_pages pages is cut; each sets PK100_STATUS_PAGE.  Bit 0: a bounded wait expired.
  * max_new: no request has more new tokens than this (<= 0: not known).  It chooses kernels, no result but rounding
  * depends on it; requests beyond it are attended all the same.  Rounding depends on the lengths of the other requests,

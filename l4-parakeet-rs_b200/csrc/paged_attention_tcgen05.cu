@@ -15,8 +15,8 @@ template <int D> constexpr int softmax_warps() { return kTileWarps * tiles<D>();
 template <int D> constexpr int threads() { return softmax_warps<D>() * 32 + 64; }
 constexpr int kAtom = kTile * 128;              // 128 rows x 64 elements, 128-byte swizzle
 constexpr int kBox = 64;                        // most keys of a TMA box
-constexpr int kByFma = 5;                       // of 16 pairs of scores, whose exponentials the FMA pipe forms (two prompts: 3 453,
-                                                // 4 460, 5 407, 6 443 us: the order of the instructions moves with it)
+constexpr int kByFma = 5;                       // of 16 pairs of scores, whose exponentials the FMA pipe forms (two prompts: 4 472,
+                                                // 5 427, 6 454 us on one card: the order of the instructions moves with it)
 
 template <int D> constexpr int ring_slots() { return 5; }
 
@@ -37,20 +37,25 @@ struct Smem {
 template <typename T> __host__ __device__ constexpr uint32_t type_bits() { return 0; }                                    // kind::f16 operands: fp16
 template <> __host__ __device__ constexpr uint32_t type_bits<__nv_bfloat16>() { return (1u << 7) | (1u << 10); }
 
-__device__ __forceinline__ float max_of(float a, float b, float c) {          // (NaN where one of them is)
+__device__ __forceinline__ float max_of(float a, float b, float c) {
     float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
 
 // 2^x for two values at most 9: n = rint(x), a polynomial of the remainder (minimax of the relative error among those of
 // degree 3 that are 1 at 0: 1.01e-4, a fifth of half a step of an fp16 P), n into the exponent.  x below -127 counts as -127,
 // where 1 less 127 in the exponent is zero to the bit: a masked score has no weight at all (and between -127 and -126 no result
-// is below zero or above 2^-126).  NaN counts as -127, too.  On the FMA pipe, where ex2.approx (16 a clock and SM) would take as
-// long as the tensor cores' products.
+// is below zero or above 2^-126).  NaN (0x7fffffff) leaves as the largest number, 0x7f7fffff, which is infinity in 16 bits.
+// On the FMA pipe, where ex2.approx (16 a clock and SM) would take as long as the tensor cores' products.
 __device__ __forceinline__ Pair exp2_fma(Pair x) {
     const float2 v = halves_of(x);
-    x = pair_of(fmaxf(v.x, -127.0f), fmaxf(v.y, -127.0f));
+    x = pair_of(max_or_nan(v.x, -127.0f), max_or_nan(v.y, -127.0f));
     const Pair magic = pair_of(12582912.0f, 12582912.0f), back = pair_of(-12582912.0f, -12582912.0f);       // 1.5 * 2^23
     const Pair n = pair_add(x, magic);
     const Pair r = pair_fma(pair_add(n, back), pair_of(-1.0f, -1.0f), x);
@@ -61,6 +66,9 @@ __device__ __forceinline__ Pair exp2_fma(Pair x) {
     return pair_of(__uint_as_float(__float_as_uint(part.x) + (__float_as_uint(whole.x) << 23)),
                    __uint_as_float(__float_as_uint(part.y) + (__float_as_uint(whole.y) << 23)));
 }
+
+// A sum with such a number in it becomes NaN; others, below 2^39, stay as they are.
+__device__ __forceinline__ float nan_if_huge(float sum) { return fmaf(sum * 1e20f, 0.0f, sum); }
 
 // P = exp2(s * scale + shift) of 64 scores, stored as 16-bit pairs; the sum of the unrounded values.  ByFma: of 16 pairs
 // of scores, how many go to the FMA pipe.
@@ -507,7 +515,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             for (int i = 4; i < 60; i += 8)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) top[j] = max_of(top[j], s[i + 2 * j], s[i + 2 * j + 1]);
-            const float own = max_of(max_of(top[0], s[60], s[61]), max_of(top[1], s[62], s[63]), max_of(top[2], top[3], top[3]));
+            const float own = max_of(max_of(top[0], s[60], s[61]), max_of(top[1], s[62], s[63]), fmaxf(top[2], top[3]));
             sm.top[t][half][tile_row] = own;                 // (the partner has read the last one: S of this block came after its P)
             pair_sync();                                     // (also: both halves of S have been read, P may take their place)
             const float seen = fmaxf(m, fmaxf(own, sm.top[t][half ^ 1][tile_row]));
@@ -515,7 +523,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             if (__any_sync(0xffffffffu, (seen - m) * scale > 8.0f || (done == 0 && seen > m))) {
                 const float factor = exp2_approx((m - (seen == -INFINITY ? 0.0f : seen)) * scale);
                 m = seen;
-                l *= factor;
+                l = nan_if_huge(l) * factor;                 // (before the factor hides it)
                 if (done > 0) {
                     ok &= __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], (before + done - 1) & 1, abort_flag)) != 0;
                     tc_fence_after_sync();
@@ -532,7 +540,6 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             }
             const float shift = m == -INFINITY ? 0.0f : -m * scale;
             l += weights_of_scores<T, kByFma>(s, scale, shift, p_cols);
-            if (!(own < INFINITY)) l = NAN;                  // (a score that is NaN or infinity makes the row NaN)
             tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
@@ -543,6 +550,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         sm.top[t][half][tile_row] = l;
         pair_sync();
         l += sm.top[t][half ^ 1][tile_row];
+        l = nan_if_huge(l);
         if (ok && done > 0) {
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], (before + done - 1) & 1, abort_flag)) != 0;
             tc_fence_after_sync();
