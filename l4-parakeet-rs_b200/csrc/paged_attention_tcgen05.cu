@@ -234,9 +234,9 @@ __device__ __forceinline__ Place place_of(const Smem<D>& sm, const PagedParams& 
 // Scores, m, l and O are fp32; P is rounded to the type of V for the tensor cores, which costs what the rounding of the
 // output costs (the sum l is that of the unrounded P).
 // Bound by a tile's chain of scores, softmax and products: 3200 cycles per 128 keys of both tiles, of which the MMAs are
-// 2300.  Two prompts of 7.2 k tokens, 16 / 4 heads of 128: 407 to 428 us, 1 PFLOP/s (the few-row kernel in the same place: 4.6 ms);
-// 512 tokens over 32 000, 16 / 2 heads: 124 to 142 us, 1 PFLOP/s (764 us).  Nine chunks of 5 to 561 tokens, 16 heads of 64,
-// window 1024: 26 us, the latency of the longest block (32.8 with the requests in their own order).
+// 2300.  Two prompts of 7.2 k tokens, 16 / 4 heads of 128: 423 to 433 us, 1 PFLOP/s (the few-row kernel in the same place: 4.6 ms);
+// 512 tokens over 32 000, 16 / 2 heads: 140 to 145 us, 0.95 PFLOP/s (764 us).  Nine chunks of 5 to 561 tokens, 16 heads of 64,
+// window 1024: 27 us, the latency of the longest block (32.8 with the requests in their own order).
 template <typename T, int D, bool kLoop>
 __global__ void __launch_bounds__(threads<D>(), 3 - tiles<D>())
 paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p,
