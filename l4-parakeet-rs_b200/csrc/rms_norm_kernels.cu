@@ -1,6 +1,8 @@
 // Residual addition + root-mean-square norm with the output encodings of the 8-bit products.
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "element16.cuh"
 #include "pk100_internal.h"
 #include "ptx_sm100.cuh"
@@ -27,6 +29,14 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int column, int width,
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (column + i < width) row[column + i] = static_cast<uint8_t>((i < 4 ? v.x : v.y) >> (8 * (i % 4)));
+}
+
+// y / c rounded once, from the rounded reciprocal: the product is two roundings off, its remainder, which the multiply-add has
+// exactly, takes them back (P. Markstein, IBM J. Res. Dev. 34, 1990).  The product alone moved codes of values half-way
+// between two.  For finite y and quotients whose way stays among the normal numbers.
+__device__ __forceinline__ float quotient(float y, float c, float inverse) {
+    const float q = y * inverse;
+    return fmaf(fmaf(-q, c, y), inverse, q);
 }
 
 // A row belongs to a warp (8 rows a block) or to a whole block; every thread keeps Chunks x 8 of its elements, so
@@ -83,18 +93,18 @@ add_rms_norm_kernel(const RmsNormParams p) {
             sum = fmaf(x.y, x.y, sum);
             if constexpr (kRowScale) {
                 const float2 y = floats_of(b[i], T());
-                const float u = fabsf(x.x * y.x), v = fabsf(x.y * y.y);
-                if (u < INFINITY) top = fmaxf(top, u);              // what is a number
-                if (v < INFINITY) top = fmaxf(top, v);
+                top = fmaxf(top, fmaxf(fabsf(x.x * y.x), fabsf(x.y * y.y)));       // (NaN counts for nothing)
             }
         }
     }
+    // over the row, to all of its threads
+    auto reduce = [&] {
 #pragma unroll
-    for (int off = 16; off > 0; off /= 2) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if constexpr (kRowScale) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    }
-    if (p.threads > 32) {                               // the block is one row
+        for (int off = 16; off > 0; off /= 2) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            if constexpr (kRowScale) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        }
+        if (p.threads == 32) return;                    // (otherwise the block is one row)
         const int warps = p.threads / 32, warp = t / 32, lane = t % 32;
         if (lane == 0) {
             part_sum[warp] = sum;
@@ -108,50 +118,83 @@ add_rms_norm_kernel(const RmsNormParams p) {
             sum += __shfl_xor_sync(0xffffffffu, sum, off);
             if constexpr (kRowScale) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         }
-    }
+    };
+    reduce();
     const float rstd = rsqrtf(sum / p.width + p.eps);
+    bool finite = true;
+    if (kRowScale && top == INFINITY) {                 // (rare) the maximum over what is a number
+        finite = false;
+        top = 0.0f;
+#pragma unroll
+        for (int c = 0; c < Chunks; ++c) {
+            const uint32_t* a = reinterpret_cast<const uint32_t*>(&s[c]);
+            const uint4 g = load8(gamma, (c * p.threads + t) * 8, p.width, p.vec_gamma);
+            const uint32_t* b = reinterpret_cast<const uint32_t*>(&g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 x = floats_of(a[i], T()), y = floats_of(b[i], T());
+                const float u = fabsf(x.x * y.x), v = fabsf(x.y * y.y);
+                if (u < INFINITY) top = fmaxf(top, u);
+                if (v < INFINITY) top = fmaxf(top, v);
+            }
+        }
+        if (p.threads > 32) __syncthreads();            // (the parts have been read)
+        reduce();                                       // (the sum has done its work)
+    }
     float scale = 1.0f, inverse = p.inv_scale;
+    bool by_reciprocal = false;                         // the row's quotients: nothing on their way leaves the normal numbers
     if constexpr (kRowScale) {
         const float peak = top * rstd;
         if (peak > 0.0f && peak < INFINITY) scale = __fdiv_rn(peak, Mode == PK100_LN_E4M3_ROW ? 448.0f : 127.0f);
         inverse = __frcp_rn(scale);
+        by_reciprocal = finite && scale > 1e-18f && scale < 1e18f;
         if (t == 0) p.scales[row] = scale;
     }
+    auto write = [&](auto by_product) {
 #pragma unroll
-    for (int c = 0; c < Chunks; ++c) {
-        const int column = (c * p.threads + t) * 8;
-        const uint32_t* a = reinterpret_cast<const uint32_t*>(&s[c]);
-        const uint4 g = load8(gamma, column, p.width, p.vec_gamma);        // (again, from the L1: registers are blocks in flight)
-        const uint32_t* b = reinterpret_cast<const uint32_t*>(&g);
-        float y[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 x = floats_of(a[i], T()), w = floats_of(b[i], T());
-            y[2 * i] = x.x * rstd * w.x;
-            y[2 * i + 1] = x.y * rstd * w.y;
-        }
-        if constexpr (Mode == PK100_LN_F16) {
-            T* o = static_cast<T*>(p.output) + row * p.ld_out;
-            store8(o, column, p.width, p.vec_out, make_uint4(packed_of(y[0], y[1], T()), packed_of(y[2], y[3], T()),
-                                                             packed_of(y[4], y[5], T()), packed_of(y[6], y[7], T())));
-        } else {
-            uint32_t w[2] = {0, 0};
+        for (int c = 0; c < Chunks; ++c) {
+            const int column = (c * p.threads + t) * 8;
+            const uint32_t* a = reinterpret_cast<const uint32_t*>(&s[c]);
+            const uint4 g = load8(gamma, column, p.width, p.vec_gamma);        // (again, from the L1: registers are blocks in flight)
+            const uint32_t* b = reinterpret_cast<const uint32_t*>(&g);
+            float y[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                // a scale below the smallest normal number has no finite reciprocal: divide
-                const float lo = inverse < INFINITY ? y[2 * i] * inverse : y[2 * i] / scale;
-                const float hi = inverse < INFINITY ? y[2 * i + 1] * inverse : y[2 * i + 1] / scale;
-                if constexpr (Mode == PK100_LN_S8_ROW) {
-                    const int u = max(-127, min(127, __float2int_rn(lo))), v = max(-127, min(127, __float2int_rn(hi)));
-                    w[i / 2] |= static_cast<uint32_t>((u & 255) | ((v & 255) << 8)) << (16 * (i % 2));
-                } else {
-                    w[i / 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3))
-                                << (16 * (i % 2));
-                }
+                const float2 x = floats_of(a[i], T()), w = floats_of(b[i], T());
+                y[2 * i] = x.x * rstd * w.x;
+                y[2 * i + 1] = x.y * rstd * w.y;
             }
-            store_codes(static_cast<uint8_t*>(p.output) + row * p.ld_out, column, p.width, p.vec_out, make_uint2(w[0], w[1]));
+            if constexpr (Mode == PK100_LN_F16) {
+                T* o = static_cast<T*>(p.output) + row * p.ld_out;
+                store8(o, column, p.width, p.vec_out, make_uint4(packed_of(y[0], y[1], T()), packed_of(y[2], y[3], T()),
+                                                                 packed_of(y[4], y[5], T()), packed_of(y[6], y[7], T())));
+            } else {
+                uint32_t w[2] = {0, 0};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float lo, hi;
+                    if constexpr (!kRowScale) {
+                        lo = inverse < INFINITY ? y[2 * i] * inverse : y[2 * i] / scale;
+                        hi = inverse < INFINITY ? y[2 * i + 1] * inverse : y[2 * i + 1] / scale;
+                    } else {
+                        lo = decltype(by_product)::value ? quotient(y[2 * i], scale, inverse) : y[2 * i] / scale;
+                        hi = decltype(by_product)::value ? quotient(y[2 * i + 1], scale, inverse) : y[2 * i + 1] / scale;
+                    }
+                    if constexpr (Mode == PK100_LN_S8_ROW) {
+                        const int u = max(-127, min(127, __float2int_rn(lo))), v = max(-127, min(127, __float2int_rn(hi)));
+                        w[i / 2] |= static_cast<uint32_t>((u & 255) | ((v & 255) << 8)) << (16 * (i % 2));
+                    } else {
+                        w[i / 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3))
+                                    << (16 * (i % 2));
+                    }
+                }
+                store_codes(static_cast<uint8_t*>(p.output) + row * p.ld_out, column, p.width, p.vec_out, make_uint2(w[0], w[1]));
+            }
         }
-    }
+    };
+    // (a branch a row)
+    if (by_reciprocal) write(std::true_type());
+    else write(std::false_type());
 }
 
 template <typename T, int Mode>

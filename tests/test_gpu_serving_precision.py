@@ -1,0 +1,74 @@
+"""GPU tests of what the serving operators promise about single roundings: quotients of the norm's codes, small weights and
+sums of attention."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+# ------------------------------------------------------------- norm
+def _values_below(peak, dtype):
+    """Every number of the type between 0.05 and the peak, the peak among them."""
+    v = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    return v[(v.float() > 0.05) & (v.float() <= peak)]
+
+
+@pytest.mark.parametrize("mode,dtype,peak", [("e4m3", F16, 56.5), ("int8", F16, 14.8828125), ("e4m3", BF16, 24.5), ("int8", BF16, 53.75)])
+def test_norm_codes_are_those_of_the_quotient(pk, cuda, mode, dtype, peak):
+    """Rows of +1 and -1 have a mean square of 1, so y = s * gamma exactly, and the code is that of y / c, c = max |y| / top in
+    fp32: one rounding.  A product with the rounded reciprocal has two, and gives other codes for some of these y."""
+    L = pk.lib
+    gamma = _values_below(peak, dtype)
+    width, top = gamma.numel(), 448.0 if mode == "e4m3" else 127.0
+    x = torch.ones(3, width, dtype=dtype)
+    x[1] = -1
+    x[2, ::2] = -1
+    out, scales, _ = pk.ops.add_rms_norm(x.cuda(), gamma.cuda(), mode=L.LN_E4M3_ROW if mode == "e4m3" else L.LN_S8_ROW, eps=0.0)
+    y = x.float().numpy() * gamma.float().numpy()
+    c = np.float32(peak) / np.float32(top)
+    quotient, product = y / c, y * (np.float32(1) / c)
+    code = lambda q: torch.from_numpy(np.rint(q) if mode == "int8" else q).to(torch.int8 if mode == "int8" else torch.float8_e4m3fn).float()
+    assert not torch.equal(code(quotient), code(product))
+    assert (scales.cpu() == torch.from_numpy(np.array(c))).all()
+    got = (out if mode == "int8" else out.view(torch.float8_e4m3fn)).float().cpu()
+    assert torch.equal(got, code(quotient))
+
+
+@pytest.mark.parametrize("width", [40, 256, 4096, 20000])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_norm_products_beyond_the_largest_number_stay_out_of_the_maximum(pk, cuda, dtype, width):
+    """Rows beside each other, some of them with infinities: theirs have y = 0 or NaN and a scale of 1, the others their own codes
+    and scales to the bit."""
+    L = pk.lib
+    gen = torch.Generator().manual_seed(width)
+    x = torch.randn(40, width, generator=gen).to(dtype).cuda()
+    gamma = (torch.rand(width, generator=gen) + 0.5).to(dtype).cuda()
+    bad = x.clone()
+    bad[3, 7], bad[4, width - 1], bad[4, 0], bad[21, width // 2], bad[39, 5] = math.inf, -math.inf, math.inf, math.inf, math.nan
+    whole = torch.tensor([r not in (3, 4, 21, 39) for r in range(40)])
+    for mode in (L.LN_E4M3_ROW, L.LN_S8_ROW):
+        want, want_scales, _ = pk.ops.add_rms_norm(x, gamma, mode=mode)
+        out, scales, _ = pk.ops.add_rms_norm(bad, gamma, mode=mode)
+        assert torch.equal(out[whole], want[whole]) and torch.equal(scales[whole], want_scales[whole])
+        assert (scales[~whole] == 1.0).all()
+        codes = out.float() if mode == L.LN_S8_ROW else out.view(torch.float8_e4m3fn).float()
+        assert (codes[3][torch.isfinite(bad[3])] == 0).all() and (codes[21][torch.isfinite(bad[21])] == 0).all()
+        if mode == L.LN_E4M3_ROW:
+            assert torch.isnan(codes[3, 7]) and torch.isnan(codes[39]).all()
+
+
+def test_norm_products_beyond_the_largest_number_by_gamma_alone(pk, cuda):
+    """s * gamma beyond fp32 where s * rstd * gamma is not: such a y is clamped, the scale is that of the others."""
+    L = pk.lib
+    x = torch.full((2, 64), 1000.0, dtype=BF16, device="cuda")
+    gamma = torch.ones(64, dtype=BF16, device="cuda")
+    gamma[9] = 1e36
+    for mode, top in ((L.LN_E4M3_ROW, 448.0), (L.LN_S8_ROW, 127.0)):
+        out, scales, _ = pk.ops.add_rms_norm(x, gamma, mode=mode)
+        codes = out.float() if mode == L.LN_S8_ROW else out.view(torch.float8_e4m3fn).float()
+        assert (codes == top).all() and float((scales * top - 1).abs().max()) < 1e-5
