@@ -174,8 +174,8 @@ add_rms_norm_kernel(const RmsNormParams p) {
                 for (int i = 0; i < 4; ++i) {
                     float lo, hi;
                     if constexpr (!kRowScale) {
-                        lo = inverse < INFINITY ? y[2 * i] * inverse : y[2 * i] / scale;
-                        hi = inverse < INFINITY ? y[2 * i + 1] * inverse : y[2 * i + 1] / scale;
+                        lo = y[2 * i] * inverse;
+                        hi = y[2 * i + 1] * inverse;
                     } else {
                         lo = decltype(by_product)::value ? quotient(y[2 * i], scale, inverse) : y[2 * i] / scale;
                         hi = decltype(by_product)::value ? quotient(y[2 * i + 1], scale, inverse) : y[2 * i + 1] / scale;

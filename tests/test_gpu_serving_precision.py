@@ -72,3 +72,19 @@ def test_norm_products_beyond_the_largest_number_by_gamma_alone(pk, cuda):
         out, scales, _ = pk.ops.add_rms_norm(x, gamma, mode=mode)
         codes = out.float() if mode == L.LN_S8_ROW else out.view(torch.float8_e4m3fn).float()
         assert (codes == top).all() and float((scales * top - 1).abs().max()) < 1e-5
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_norm_with_a_fixed_scale_multiplies_by_whatever_it_is_given(pk, cuda, dtype):
+    """E4M3(y * inv_scale): an infinite factor saturates what is not zero and makes NaN of what is, NaN makes NaN."""
+    x = torch.randn(3, 100, generator=torch.Generator().manual_seed(1)).to(dtype)
+    x[1, ::3] = 0
+    gamma = torch.ones(100, dtype=dtype)
+    def codes(factor):
+        out, _, _ = pk.ops.add_rms_norm(x.cuda(), gamma.cuda(), mode=pk.lib.LN_E4M3_FIXED, inv_scale=factor)
+        return out.view(torch.float8_e4m3fn).float().cpu()
+    want = torch.where(x == 0, math.nan, 448.0 * torch.sign(x.float()))
+    assert torch.equal(codes(math.inf).nan_to_num(7.0), want.nan_to_num(7.0))
+    assert torch.equal(codes(-math.inf).nan_to_num(7.0), (-want).nan_to_num(7.0))
+    assert torch.isnan(codes(math.nan)).all()
+    assert (codes(0.0) == 0).all()
