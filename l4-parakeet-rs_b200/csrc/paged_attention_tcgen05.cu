@@ -519,8 +519,14 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             sm.top[t][half][tile_row] = own;                 // (the partner has read the last one: S of this block came after its P)
             pair_sync();                                     // (also: both halves of S have been read, P may take their place)
             const float seen = fmaxf(m, fmaxf(own, sm.top[t][half ^ 1][tile_row]));
+            // The exponents are s * scale - m * scale in one rounding, but m * scale has its own: of scores far from zero, where its half
+            // step would take P beyond every number (from 2^27 on), m is taken off the scores first.
+            const bool far = fabsf(seen * scale) >= 16384.0f && seen != -INFINITY;
             // (-inf - -inf is NaN: no growth)
-            if (__any_sync(0xffffffffu, (seen - m) * scale > 8.0f || (done == 0 && seen > m))) {
+            if (__any_sync(0xffffffffu, (seen - m) * scale > 8.0f || (done == 0 && seen > m) || far)) {
+                const float off = far ? seen : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 64; ++i) s[i] -= off;
                 const float factor = exp2_approx((m - (seen == -INFINITY ? 0.0f : seen)) * scale);
                 m = seen;
                 l = nan_if_huge(l) * factor;                 // (before the factor hides it)
@@ -538,7 +544,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                     }
                 }
             }
-            const float shift = m == -INFINITY ? 0.0f : -m * scale;
+            const float shift = far || m == -INFINITY ? 0.0f : -m * scale;
             l += weights_of_scores<T, kByFma>(s, scale, shift, p_cols);
             tmem_st_wait();
             tc_fence_before_sync();

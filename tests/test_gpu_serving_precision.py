@@ -88,3 +88,23 @@ def test_norm_with_a_fixed_scale_multiplies_by_whatever_it_is_given(pk, cuda, dt
     assert torch.equal(codes(-math.inf).nan_to_num(7.0), (-want).nan_to_num(7.0))
     assert torch.isnan(codes(math.nan)).all()
     assert (codes(0.0) == 0).all()
+
+
+# ------------------------------------------------------------- attention
+@pytest.mark.parametrize("tokens", [2, 300])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_scores_of_millions(pk, cuda, dim, tokens):
+    """fp16, the largest key of a row far above the others, scores up to 4e9: its value, but for the rounding of a weight and of
+    the output."""
+    k = torch.zeros(16, 32, 2, dim, dtype=F16, device="cuda")
+    v = torch.randn(16, 32, 2, dim, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").half()
+    flat = k.view(512, 2, dim)
+    flat[:, :, 0] = torch.arange(512, device="cuda").half()[:, None]
+    for large in (1.0, 300.0, 30000.0, 65504.0):
+        q = torch.zeros(tokens, 4, dim, dtype=F16, device="cuda")
+        q[:, :, 0] = large
+        for sign in (1.0, -1.0):
+            out = pk.ops.paged_attention(q, k, v, torch.arange(16, dtype=torch.int32, device="cuda")[None], torch.tensor([0, tokens], dtype=torch.int32, device="cuda"),
+                                         torch.tensor([512], dtype=torch.int32, device="cuda"), causal=False, scale=128.0 * sign)
+            want = v.view(512, 2, dim)[511 if sign > 0 else 0].repeat_interleave(2, 0)
+            assert bool(((out.double() - want.double()).abs() <= 2 * 2.0 ** -11 * want.double().abs() + 2.0 ** -25).all()), (large, sign)
