@@ -492,7 +492,8 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
         const uint32_t s_cols = tmem + lanes + t * kTile + half * 64, p_cols = tmem + lanes + t * kTile + half * 32;
         const uint32_t o_cols = tmem + lanes + kTiles * kTile + t * D + half * (D / 2);
-        const float scale = fmaxf(fabsf(p.scale_log2), 1e-37f);       // (-inf * 0 would be NaN; 1e-37 takes any score to 0)
+        // (-inf * 0 would be NaN; the smallest number takes any finite score to 0.  NaN stays.)
+        const float scale = fabsf(p.scale_log2) < 1e-45f ? 1e-45f : fabsf(p.scale_log2);
         float m = -INFINITY, l = 0.0f;                       // m: reference maximum of the raw scores; l: sum over this half of the keys
         int done = 0;                                        // blocks of this tile
         // (a wait that ran out does not end the loop: the other warp of the pair would wait at the barrier for ever)

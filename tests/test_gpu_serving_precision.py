@@ -108,3 +108,26 @@ def test_attention_of_scores_of_millions(pk, cuda, dim, tokens):
                                          torch.tensor([512], dtype=torch.int32, device="cuda"), causal=False, scale=128.0 * sign)
             want = v.view(512, 2, dim)[511 if sign > 0 else 0].repeat_interleave(2, 0)
             assert bool(((out.double() - want.double()).abs() <= 2 * 2.0 ** -11 * want.double().abs() + 2.0 ** -25).all()), (large, sign)
+
+
+@pytest.mark.parametrize("tokens", [2, 300])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_a_scale_of_zero_and_of_none(pk, cuda, dim, tokens):
+    """Scale 0 makes all keys alike, whatever they score (1e37 here); a scale that is no number makes rows that are none."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    v = torch.randn(12, 32, 2, dim, generator=gen, device="cuda").to(BF16)
+    k = torch.zeros_like(v)
+    k[..., 0] = torch.randn(12, 32, 2, generator=gen, device="cuda") * 1e18
+    q = torch.zeros(tokens, 4, dim, dtype=BF16, device="cuda")
+    q[..., 0] = 1e19
+    lse = torch.empty(tokens, 4, device="cuda")
+    rest = (k, v, torch.arange(12, dtype=torch.int32, device="cuda")[None], torch.tensor([0, tokens], dtype=torch.int32, device="cuda"),
+            torch.tensor([384], dtype=torch.int32, device="cuda"))
+    out = pk.ops.paged_attention(q, *rest, causal=False, scale=0.0, lse=lse)
+    flat = v.view(384, 2, dim).double()
+    want, spread = (t.mean(0).repeat_interleave(2, 0) for t in (flat, flat.abs()))
+    # half a step of each weight and of the output; 1e-4 for the exponentials
+    assert bool(((out.double() - want).abs() <= (2.0 ** -8 + 1e-4) * spread + 2.0 ** -8 * want.abs()).all())
+    assert float((lse.double() - math.log(384.0)).abs().max()) <= 1.1e-4
+    out = pk.ops.paged_attention(q, *rest, causal=False, scale=math.nan, lse=lse)
+    assert bool(out.isnan().all()) and bool(lse.isnan().all())
