@@ -79,6 +79,7 @@ __device__ __forceinline__ void mma_rows(float (&d)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+template <typename T> __device__ constexpr float weight_factor() { return static_cast<float>(1 << weight_bits<T>(0)); }     // (P is 1 at most)
 __device__ __forceinline__ void row_warps_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kRowWarps * 32) : "memory"); }
 
 // A request's work: tiles of 16 rows per key-value head, each over the key blocks that any row of the request sees
@@ -156,7 +157,7 @@ __device__ __forceinline__ void join_row(const PagedParams& p, const PagedReques
     }
 #pragma unroll
     for (int off = 16; off > 0; off /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    const float inverse = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+    const float inverse = sum > 0.0f ? 1.0f / (sum * weight_factor<T>()) : (sum == 0.0f ? 0.0f : sum);
     const int i = index / p.group;
     const long long h = head * p.group + index - i * p.group;
     T* dst = static_cast<T*>(p.out) + (at.row0 + i) * p.ld_out + h * D + lane * kWidth;
@@ -290,6 +291,7 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
         // ------------------------------------------------------------ products and softmax
         const int g = lane / 4, c = lane % 4;
         constexpr int kSteps = D / 16, kFeatureTiles = D / 32;          // k steps of Q.K; 8-feature tiles of a warp's quarter
+        constexpr float kFactor = weight_factor<T>();                   // of P and so of the output, not of the sums
         int it = 0;
         rows_walk(p, first_request, first_base, begin, end,
                   [&](const RowsShape& s, int request, int head, int tile, long long tile_first, int b0, int b1, bool whole) {
@@ -381,8 +383,8 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
                     l0 += x0 + x1;
                     l1 += y0 + y1;
                     const int chunk = 2 * warp + nt;
-                    *reinterpret_cast<uint32_t*>(&sm.p[buf][g * 128 + ((chunk ^ g) << 4) + 4 * c]) = packed_of(x0, x1, T());
-                    *reinterpret_cast<uint32_t*>(&sm.p[buf][(g + 8) * 128 + ((chunk ^ g) << 4) + 4 * c]) = packed_of(y0, y1, T());
+                    *reinterpret_cast<uint32_t*>(&sm.p[buf][g * 128 + ((chunk ^ g) << 4) + 4 * c]) = packed_of(x0 * kFactor, x1 * kFactor, T());
+                    *reinterpret_cast<uint32_t*>(&sm.p[buf][(g + 8) * 128 + ((chunk ^ g) << 4) + 4 * c]) = packed_of(y0 * kFactor, y1 * kFactor, T());
                 }
 #pragma unroll
                 for (int j = 0; j < kFeatureTiles; ++j) {
@@ -440,7 +442,7 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
                 l1 += sm.sum[w][g + 8];
             }
             if (whole) {
-                const float r0i = l0 > 0.0f ? 1.0f / l0 : (l0 == 0.0f ? 0.0f : l0), r1i = l1 > 0.0f ? 1.0f / l1 : (l1 == 0.0f ? 0.0f : l1);
+                const float r0i = l0 > 0.0f ? 1.0f / (l0 * kFactor) : (l0 == 0.0f ? 0.0f : l0), r1i = l1 > 0.0f ? 1.0f / (l1 * kFactor) : (l1 == 0.0f ? 0.0f : l1);
                 const long long h0 = head * p.group + tile * kRows + g - i0 * p.group, h1 = head * p.group + tile * kRows + g + 8 - i1 * p.group;
                 T* dst0 = static_cast<T*>(p.out) + (s.at.row0 + i0) * p.ld_out + h0 * D + warp * (D / 4) + 2 * c;
                 T* dst1 = static_cast<T*>(p.out) + (s.at.row0 + i1) * p.ld_out + h1 * D + warp * (D / 4) + 2 * c;

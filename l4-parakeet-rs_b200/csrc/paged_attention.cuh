@@ -54,6 +54,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
+// log2 of a factor that the weights P of a softmax get for the tensor cores: what fp16 has room for above the largest, so that
+// few of the small ones fall below its range.  Without it a key of 2^-25.5 had a weight in the sum but none in the output,
+// and 2^17 of them behind one dominating key took 3e-3 from a row.  bf16 reaches to 2^-133.
+template <typename T> __host__ __device__ constexpr int weight_bits(int largest) { return 0; }
+template <> __host__ __device__ constexpr int weight_bits<__half>(int largest) { return 14 - largest; }
+
 // The kernel for requests of more than p.few_rows rows (paged_attention_tcgen05.cu): `pairs` numbers of pairs of tiles
 // (tokens * group / pair_rows + requests).  Where the pairs are few, a row's keys are shared out to up to `shares`; how many it came
 // to goes to share_count, their parts to part_ml [shares, tokens, heads] and part_out [shares, tokens, heads, head_dim], and

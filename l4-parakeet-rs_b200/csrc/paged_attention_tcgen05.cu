@@ -48,7 +48,7 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
     return d;
 }
 
-// 2^x for two values at most 9: n = rint(x), a polynomial of the remainder (minimax of the relative error among those of
+// 2^x for two values at most 16: n = rint(x), a polynomial of the remainder (minimax of the relative error among those of
 // degree 3 that are 1 at 0: 1.01e-4, a fifth of half a step of an fp16 P), n into the exponent.  x below -127 counts as -127,
 // where 1 less 127 in the exponent is zero to the bit: a masked score has no weight at all (and between -127 and -126 no result
 // is below zero or above 2^-126).  NaN (0x7fffffff) leaves as the largest number, 0x7f7fffff, which is infinity in 16 bits.
@@ -67,7 +67,7 @@ __device__ __forceinline__ Pair exp2_fma(Pair x) {
                    __uint_as_float(__float_as_uint(part.y) + (__float_as_uint(whole.y) << 23)));
 }
 
-// A sum with such a number in it becomes NaN; others, below 2^39, stay as they are.
+// A sum with such a number in it becomes NaN; others, below 2^45, stay as they are.
 __device__ __forceinline__ float nan_if_huge(float sum) { return fmaf(sum * 1e20f, 0.0f, sum); }
 
 // P = exp2(s * scale + shift) of 64 scores, stored as 16-bit pairs; the sum of the unrounded values.  ByFma: of 16 pairs
@@ -230,7 +230,7 @@ __device__ __forceinline__ Place place_of(const Smem<D>& sm, const PagedParams& 
 //   O += P V   (A from tensor memory, V as it lies in the cache: MN-major), D TMEM columns.
 // While one tile's softmax runs, the tensor cores form the other's O and next S (heads of 64: the other block's of the
 // SM).  m follows the running maximum only when that has grown by more than 2^8 (then O and l are scaled down, which is
-// exact but for rounding): P stays below 2^8, within fp16's range, and the rescaling of O all but disappears.
+// exact but for rounding): P stays below 2^8 (fp16: 2^14, see weight_bits), and the rescaling of O all but disappears.
 // Scores, m, l and O are fp32; P is rounded to the type of V for the tensor cores, which costs what the rounding of the
 // output costs (the sum l is that of the unrounded P).
 // Bound by a tile's chain of scores, softmax and products: 3200 cycles per 128 keys of both tiles, of which the MMAs are
@@ -494,6 +494,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         const uint32_t o_cols = tmem + lanes + kTiles * kTile + t * D + half * (D / 2);
         // (-inf * 0 would be NaN; the smallest number takes any finite score to 0.  NaN stays.)
         const float scale = fabsf(p.scale_log2) < 1e-45f ? 1e-45f : fabsf(p.scale_log2);
+        constexpr float kBits = weight_bits<T>(8);
         float m = -INFINITY, l = 0.0f;                       // m: reference maximum of the raw scores; l: sum over this half of the keys
         int done = 0;                                        // blocks of this tile
         // (a wait that ran out does not end the loop: the other warp of the pair would wait at the barrier for ever)
@@ -545,7 +546,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                     }
                 }
             }
-            const float shift = far || m == -INFINITY ? 0.0f : -m * scale;
+            const float shift = far || m == -INFINITY ? kBits : fmaf(-m, scale, kBits);
             l += weights_of_scores<T, kByFma>(s, scale, shift, p_cols);
             tmem_st_wait();
             tc_fence_before_sync();
@@ -594,8 +595,9 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 }
             }
             if (live && half == 0) {
-                if (shares > 1) part_ml[part] = make_float2(m * scale, l);
-                else if (p.lse != nullptr) p.lse[row] = l > 0.0f ? (m * scale + log2f(l)) * kLn2 : (l == 0.0f ? -INFINITY : l);
+                const float base = fmaf(m, scale, -kBits);
+                if (shares > 1) part_ml[part] = make_float2(base, l);
+                else if (p.lse != nullptr) p.lse[row] = l > 0.0f ? (base + log2f(l)) * kLn2 : (l == 0.0f ? -INFINITY : l);
             }
         }
         });

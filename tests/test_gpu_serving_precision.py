@@ -91,6 +91,44 @@ def test_norm_with_a_fixed_scale_multiplies_by_whatever_it_is_given(pk, cuda, dt
 
 
 # ------------------------------------------------------------- attention
+def _one_key_and_many(kernel, dim, dtype, first, value, keys=1 << 17, far=25.5):
+    """A key that scores 0, the first or the last, and `keys` of -far (base 2): of this value, and of -1.  The arguments of a call in
+    which every row sees all of them, whole, and the rows' value and lse in 64 bits."""
+    kv, page = 8, 256
+    length = keys + 1
+    pages = -(-length // page)
+    k = torch.zeros(pages * page, kv, dim, dtype=dtype, device="cuda")
+    v = torch.full_like(k, -1.0)
+    k[:, :, 0] = -far
+    at = 0 if first else keys
+    k[at], v[at] = 0, value
+    # as many rows as leave no keys to be shared out: a part of the keys has another largest one
+    requests, new = (37, 1) if kernel == "rows" else (1, 4864)
+    q = torch.zeros(requests * new, kv, dim, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1
+    ids = torch.arange(pages, dtype=torch.int32, device="cuda")
+    args = dict(query=q, key_cache=k.view(pages, page, kv, dim), value_cache=v.view(pages, page, kv, dim), block_table=ids.expand(requests, -1).contiguous(),
+                starts=torch.arange(requests + 1, dtype=torch.int32, device="cuda") * new,
+                lengths=torch.full((requests,), length, dtype=torch.int32, device="cuda"), causal=False, scale=math.log(2.0), max_new=new)
+    rest = keys * 2.0 ** -far
+    return args, (value - rest) / (1 + rest), math.log1p(rest)
+
+
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("kernel,dim", [("rows", 64), ("rows", 128), ("chunk", 64), ("chunk", 128)])
+def test_attention_of_many_small_weights(pk, cuda, kernel, dim, dtype, first):
+    """2^17 keys of 2^-25.5, each less than half of fp16's smallest number, behind one whose value is 0: all of the row is theirs.
+    Tolerance: half a step of every weight and of the output, and in fp16 half the smallest number, 2^-25, of each weight, which
+    a factor of 2^6 at least has made smaller; 1e-5 for the exponentials, 1e-3 for what the tensor cores cut off their sums."""
+    half = 2.0 ** -11 if dtype is F16 else 2.0 ** -8
+    args, want, _ = _one_key_and_many(kernel, dim, dtype, first, 0.0)
+    out = pk.ops.paged_attention(**args)
+    tolerance = (2 * half + 1e-5 + 1e-3) * abs(want) + (2.0 ** 17 * 2.0 ** -31 if dtype is F16 else 0.0)
+    assert tolerance < 0.03 * abs(want)
+    assert float((out.double() - want).abs().max()) <= tolerance
+
+
 @pytest.mark.parametrize("tokens", [2, 300])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_attention_of_scores_of_millions(pk, cuda, dim, tokens):
