@@ -175,7 +175,9 @@ __device__ __forceinline__ void join_row(const PagedParams& p, const PagedReques
 // six of them in flight.  Q.K: each of four warps 16 keys; the row maxima are exchanged, so that all warps scale
 // alike; P in 16 bits through shared memory; P.V: each warp a quarter of the features.
 // Scores, maxima, sums and outputs are fp32; P is rounded to the type of V for the tensor cores, which costs what
-// the rounding of the output costs (the sum l is that of the unrounded P).
+// the rounding of the output costs (the sum l is that of the unrounded P).  The tensor cores cut off what falls below the last
+// bit of the sum that they add to: a block's products begin at zero and are added to the row's by the FMA pipe, which rounds.
+// (One sum over 2^19 keys was 4e-3 low.)  l is compensated: many small weights behind a large one are not lost in it.
 // One token of 48 requests over 320 to 12 000 keys, 32 / 8 heads of 128 (712 MB): 118 us, 6.0 TB/s.
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads, 2)
@@ -319,7 +321,7 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
             for (int j = 0; j < kFeatureTiles; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
-            float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+            float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, e0 = 0.0f, e1 = 0.0f;      // e: what l has too much
 
             const int from = max(s.block0 + b0, lo / kBlock), to = min(s.block0 + b1, (hi + kBlock - 1) / kBlock);
             for (int b = from; b < to; ++b, ++it) {
@@ -374,25 +376,20 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
                 const float a0 = exp2_approx(m0 - z0), a1 = exp2_approx(m1 - z1);
                 m0 = n0;
                 m1 = n1;
-                l0 *= a0;
-                l1 *= a1;
+                float b0 = 0.0f, b1 = 0.0f;                              // sums of the block
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt) {
                     const float x0 = exp2_approx(sc[nt][0] - z0), x1 = exp2_approx(sc[nt][1] - z0);
                     const float y0 = exp2_approx(sc[nt][2] - z1), y1 = exp2_approx(sc[nt][3] - z1);
-                    l0 += x0 + x1;
-                    l1 += y0 + y1;
+                    b0 += x0 + x1;
+                    b1 += y0 + y1;
                     const int chunk = 2 * warp + nt;
                     *reinterpret_cast<uint32_t*>(&sm.p[buf][g * 128 + ((chunk ^ g) << 4) + 4 * c]) = packed_of(x0 * kFactor, x1 * kFactor, T());
                     *reinterpret_cast<uint32_t*>(&sm.p[buf][(g + 8) * 128 + ((chunk ^ g) << 4) + 4 * c]) = packed_of(y0 * kFactor, y1 * kFactor, T());
                 }
-#pragma unroll
-                for (int j = 0; j < kFeatureTiles; ++j) {
-                    o[j][0] *= a0;
-                    o[j][1] *= a0;
-                    o[j][2] *= a1;
-                    o[j][3] *= a1;
-                }
+                add_compensated(l0, e0, a0, b0);
+                add_compensated(l1, e1, a1, b1);
+                float pv[kFeatureTiles][4] = {};
                 row_warps_sync();
                 const bool ragged = k0 < lo || k0 + kBlock > hi;         // keys that no row sees: their values may be anything
                 const int p_row = (((lane >> 3) & 1) << 3) + (lane & 7);
@@ -415,9 +412,16 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
                             vf[2] &= near;
                             vf[3] &= far;
                         }
-                        mma_rows(o[2 * j], pf, vf[0], vf[1], T());
-                        mma_rows(o[2 * j + 1], pf, vf[2], vf[3], T());
+                        mma_rows(pv[2 * j], pf, vf[0], vf[1], T());
+                        mma_rows(pv[2 * j + 1], pf, vf[2], vf[3], T());
                     }
+                }
+#pragma unroll
+                for (int j = 0; j < kFeatureTiles; ++j) {
+                    o[j][0] = fmaf(o[j][0], a0, pv[j][0]);
+                    o[j][1] = fmaf(o[j][1], a0, pv[j][1]);
+                    o[j][2] = fmaf(o[j][2], a1, pv[j][2]);
+                    o[j][3] = fmaf(o[j][3], a1, pv[j][3]);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.empty[stage]);
@@ -504,7 +508,7 @@ static int cache_map(CUtensorMap* map, const void* base, const pk100_paged_atten
 struct PagedPlan {
     int grid;                                            // blocks of the few-row kernel
     int pairs, shares;                                   // of the other one
-    long long counts, parts, part_out, share_count, share_ml, share_out, bytes;
+    long long counts, parts, part_out, share_count, share_ml, share_out, share_kept, bytes;
 };
 
 static long long round256(long long n) { return (n + 255) / 256 * 256; }
@@ -532,7 +536,9 @@ static PagedPlan paged_plan_of(const pk100_paged_attention_args& a) {
     plan.shares = shares < 1 ? 1 : static_cast<int>(shares);
     const long long share_rows = plan.shares > 1 ? static_cast<long long>(plan.shares) * a.tokens * a.heads : 0;
     plan.share_out = plan.share_ml + round256(share_rows * 8);
-    plan.bytes = plan.share_out + round256(share_rows * a.head_dim * 4);
+    const long long kept_rows = blocks * kBlock > kFoldKeys ? static_cast<long long>(plan.shares) * a.tokens * a.heads : 0;
+    plan.share_kept = plan.share_out + round256((kept_rows > share_rows ? kept_rows : share_rows) * a.head_dim * 4);
+    plan.bytes = plan.share_kept + round256(kept_rows * 16);
     return plan;
 }
 
@@ -635,7 +641,8 @@ extern "C" int pk100_paged_attention(void* stream_v, const pk100_paged_attention
     int* share_count = reinterpret_cast<int*>(ws + plan.share_count);
     float2* share_ml = reinterpret_cast<float2*>(ws + plan.share_ml);
     float* share_out = reinterpret_cast<float*>(ws + plan.share_out);
-    if (many && (rc = paged_attention_chunks(a->type, a->head_dim, p, map_k, map_v, plan.pairs, plan.shares, share_count, share_ml, share_out, stream)) != PK100_OK) return rc;
+    float2* share_kept = reinterpret_cast<float2*>(ws + plan.share_kept);
+    if (many && (rc = paged_attention_chunks(a->type, a->head_dim, p, map_k, map_v, plan.pairs, plan.shares, share_count, share_ml, share_kept, share_out, stream)) != PK100_OK) return rc;
     if (a->type == PK100_TYPE_F16)
         rc = a->head_dim == 128 ? launch_rows<__half, 128>(*a, p, plan, map_k, map_v, many, stream) : launch_rows<__half, 64>(*a, p, plan, map_k, map_v, many, stream);
     else

@@ -60,13 +60,24 @@ __device__ __forceinline__ float exp2_approx(float x) {
 template <typename T> __host__ __device__ constexpr int weight_bits(int largest) { return 0; }
 template <> __host__ __device__ constexpr int weight_bits<__half>(int largest) { return 14 - largest; }
 
+// sum = sum * factor + more, `excess` what the sum has too much from its roundings (W. Kahan, CACM 8, 1965)
+__device__ __forceinline__ void add_compensated(float& sum, float& excess, float factor, float more) {
+    const float before = sum * factor, part = fmaf(-excess, factor, more);
+    sum = before + part;
+    excess = (sum - before) - part;
+}
+
+// Keys that the chunk kernel adds up in tensor memory; the sums of more are kept in part_out and part_kept.
+constexpr int kFoldKeys = 8192;
+
 // The kernel for requests of more than p.few_rows rows (paged_attention_tcgen05.cu): `pairs` numbers of pairs of tiles
 // (tokens * group / pair_rows + requests).  Where the pairs are few, a row's keys are shared out to up to `shares`; how many it came
 // to goes to share_count, their parts to part_ml [shares, tokens, heads] and part_out [shares, tokens, heads, head_dim], and
-// paged_attention_join adds them up (shares == 1: none of that).
+// paged_attention_join adds them up (shares == 1: none of that).  Where max_pages hold more than kFoldKeys keys, part_kept [shares,
+// tokens, heads, 2] is there, and part_out of one share at least.
 constexpr int pair_rows(int head_dim) { return head_dim == 128 ? 256 : 128; }
 int paged_attention_chunks(int type, int head_dim, const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares,
-                           int* share_count, float2* part_ml, float* part_out, cudaStream_t stream);
+                           int* share_count, float2* part_ml, float2* part_kept, float* part_out, cudaStream_t stream);
 int paged_attention_join(int type, int head_dim, const PagedParams& p, const int* share_count, const float2* part_ml, const float* part_out, cudaStream_t stream);
 
 }  // namespace pk100

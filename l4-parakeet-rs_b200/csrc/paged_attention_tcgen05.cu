@@ -15,6 +15,9 @@ template <int D> constexpr int softmax_warps() { return kTileWarps * tiles<D>();
 template <int D> constexpr int threads() { return softmax_warps<D>() * 32 + 64; }
 constexpr int kAtom = kTile * 128;              // 128 rows x 64 elements, 128-byte swizzle
 constexpr int kBox = 64;                        // most keys of a TMA box
+// Key blocks after which O begins again at zero.  The tensor cores cut off what falls below the last bit of the sum that they
+// add to, up to 2^-23 of it for 16 keys: 6e-5 in 64 blocks (4e-3 over 2^19 keys in one sum).
+constexpr int kFold = kFoldKeys / kTile;
 constexpr int kByFma = 5;                       // of 16 pairs of scores, whose exponentials the FMA pipe forms (two prompts: 4 472,
                                                 // 5 427, 6 454 us on one card: the order of the instructions moves with it)
 
@@ -97,6 +100,18 @@ __device__ __forceinline__ float weights_of_scores(const float (&s)[64], float s
     }
     const float2 sums = halves_of(sum);
     return sums.x + sums.y;
+}
+
+// o = here * o + there * dst: 16 features of a row, which the thread alone has.
+__device__ __forceinline__ void add_kept(uint32_t (&o)[16], float here, const float* dst, float there) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(dst + i);
+        o[i] = __float_as_uint(fmaf(v.x, there, __uint_as_float(o[i]) * here));
+        o[i + 1] = __float_as_uint(fmaf(v.y, there, __uint_as_float(o[i + 1]) * here));
+        o[i + 2] = __float_as_uint(fmaf(v.z, there, __uint_as_float(o[i + 2]) * here));
+        o[i + 3] = __float_as_uint(fmaf(v.w, there, __uint_as_float(o[i + 3]) * here));
+    }
 }
 
 // What a block of threads works on: 256 rows of one request and key-value head, over a share of their keys.
@@ -240,8 +255,8 @@ __device__ __forceinline__ Place place_of(const Smem<D>& sm, const PagedParams& 
 template <typename T, int D, bool kLoop>
 __global__ void __launch_bounds__(threads<D>(), 3 - tiles<D>())
 paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p,
-                             const int pairs, const int most_shares, const unsigned slots, int* share_count, float2* __restrict__ part_ml,
-                             float* __restrict__ part_out) {
+                             const int pairs, const int most_shares, const unsigned slots, int* share_count, float2* part_ml,
+                             float2* part_kept, float* part_out) {
     extern __shared__ __align__(1024) uint8_t chunk_raw[];             // (the swizzled atoms need it)
     constexpr int kHalves = D / 64, kSlots = ring_slots<D>(), kSlotBytes = kHalves * kAtom, kTiles = tiles<D>(), kSoftmaxWarps = softmax_warps<D>();
     constexpr uint32_t kColumns = 256 * kTiles;                 // of tensor memory: S and O of the tiles
@@ -388,7 +403,6 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                                     idesc_s, ks > 0);
             tc_commit_if(leader, &sm.s_full[t]);
         };
-        uint32_t filled[kTiles] = {};                    // O holds something
         do {
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
@@ -429,8 +443,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
 #pragma unroll
                         for (int ks = 0; ks < kTile / 16; ++ks)
                             mma_from_tmem(leader, tmem + kTiles * kTile + t * D, tmem + t * kTile + ks * 8, desc_v + v_slot * (kSlotBytes / 16) + ks * 128u, idesc_o,
-                                          ks > 0 ? 1u : filled[t]);
-                        filled[t] = 1;
+                                          ks > 0 || (b - tile_from[t]) % kFold != 0);
                         tc_commit_if(leader, &sm.o_done[t]);
                     }
                     if (b + 1 < w.to && active(t, b + 1)) {
@@ -456,7 +469,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         const int t = warp / kTileWarps, half = (warp / 4) % 2, quad = warp % 4, tile_row = quad * 32 + lane;
         // the two warps of a quadrant of a tile
         auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + quad) : "memory"); };
-        int before = 0;                                      // blocks of this tile in the items so far
+        uint32_t phase = 0;                                  // parity of the tile's next block
         each_item([&](const Work<kTiles>& w, int, int head, int share) {
         // (a tile without blocks brings no queries: its warps, which nothing holds back, would run ahead of the barrier's phases)
         if (w.tile_from(p, t) < w.tile_to(p, t)) {
@@ -495,11 +508,20 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         // (-inf * 0 would be NaN; the smallest number takes any finite score to 0.  NaN stays.)
         const float scale = fabsf(p.scale_log2) < 1e-45f ? 1e-45f : fabsf(p.scale_log2);
         constexpr float kBits = weight_bits<T>(8);
-        float m = -INFINITY, l = 0.0f;                       // m: reference maximum of the raw scores; l: sum over this half of the keys
-        int done = 0;                                        // blocks of this tile
+        // the blocks of this tile, kFold at a time: what those before gave is kept in memory
+        int b = w.tile_from(p, t);
+        const int end = w.tile_to(p, t);
+        bool kept = false;
+#pragma unroll 1
+        do {
+        const int stop = min(b + kFold, end);
+        // m: reference maximum of the raw scores; l: sum over this half of the keys; limit: growth of the maximum (base 2) that m follows
+        float m = -INFINITY, l = 0.0f, limit = 8.0f;
+        const bool some = b < end;
+        bool first = true;
         // (a wait that ran out does not end the loop: the other warp of the pair would wait at the barrier for ever)
-        for (int b = w.tile_from(p, t), end = w.tile_to(p, t); b < end; ++b, ++done) {
-            ok &= __all_sync(0xffffffffu, mbar_wait_bounded(&sm.s_full[t], (before + done) & 1, abort_flag)) != 0;
+        for (; b < stop; ++b, phase ^= 1, first = false) {
+            ok &= __all_sync(0xffffffffu, mbar_wait_bounded(&sm.s_full[t], phase, abort_flag)) != 0;
             tc_fence_after_sync();
             float s[64];
             tmem_ld_32x32(s_cols, reinterpret_cast<uint32_t(&)[32]>(s[0]));
@@ -521,19 +543,19 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             sm.top[t][half][tile_row] = own;                 // (the partner has read the last one: S of this block came after its P)
             pair_sync();                                     // (also: both halves of S have been read, P may take their place)
             const float seen = fmaxf(m, fmaxf(own, sm.top[t][half ^ 1][tile_row]));
-            // The exponents are s * scale - m * scale in one rounding, but m * scale has its own: of scores far from zero, where its half
-            // step would take P beyond every number (from 2^27 on), m is taken off the scores first.
-            const bool far = fabsf(seen * scale) >= 16384.0f && seen != -INFINITY;
-            // (-inf - -inf is NaN: no growth)
-            if (__any_sync(0xffffffffu, (seen - m) * scale > 8.0f || (done == 0 && seen > m) || far)) {
-                const float off = far ? seen : 0.0f;
-#pragma unroll
-                for (int i = 0; i < 64; ++i) s[i] -= off;
+            // (-inf - -inf is NaN: no growth; the first number that a row sees is infinitely more than none)
+            if (__any_sync(0xffffffffu, (seen - m) * scale > limit)) {
                 const float factor = exp2_approx((m - (seen == -INFINITY ? 0.0f : seen)) * scale);
                 m = seen;
+                // The exponents are s * scale - m * scale in one rounding, but m * scale has its own: of scores far from zero, where its
+                // half step would take P beyond every number (from 2^27 on), m is taken off the scores first, in every block.
+                limit = fabsf(m * scale) >= 16384.0f && m != -INFINITY ? -1.0f : 8.0f;
+                const float off = limit < 0.0f ? m : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 64; ++i) s[i] -= off;
                 l = nan_if_huge(l) * factor;                 // (before the factor hides it)
-                if (done > 0) {
-                    ok &= __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], (before + done - 1) & 1, abort_flag)) != 0;
+                if (!first) {
+                    ok &= __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], phase ^ 1, abort_flag)) != 0;
                     tc_fence_after_sync();
 #pragma unroll 1
                     for (int c = 0; c < D / 2; c += 16) {
@@ -546,7 +568,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                     }
                 }
             }
-            const float shift = far || m == -INFINITY ? kBits : fmaf(-m, scale, kBits);
+            const float shift = limit < 0.0f || m == -INFINITY ? kBits : fmaf(-m, scale, kBits);
             l += weights_of_scores<T, kByFma>(s, scale, shift, p_cols);
             tmem_st_wait();
             tc_fence_before_sync();
@@ -554,26 +576,36 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             if (lane == 0) mbar_arrive(&sm.p_full[t]);
         }
         // ------------------------------------------------------------ output: half the features a thread
+        const bool last = b >= end;
         pair_sync();
         sm.top[t][half][tile_row] = l;
         pair_sync();
         l += sm.top[t][half ^ 1][tile_row];
         l = nan_if_huge(l);
-        if (ok && done > 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], (before + done - 1) & 1, abort_flag)) != 0;
+        if (!last) pair_sync();                              // (the next block's scores may be there already)
+        if (ok && some) {
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], phase ^ 1, abort_flag)) != 0;
             tc_fence_after_sync();
         }
-        before += done;
         if (ok && tile_rows > 0) {
             const long long row = static_cast<long long>(w.at.row0 + token) * p.heads + head * p.group + index - token * p.group;
-            const float inverse = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-            T* dst = static_cast<T*>(p.out) + (w.at.row0 + token) * p.ld_out + static_cast<long long>(head * p.group + index - token * p.group) * D + half * (D / 2);
             const long long part = static_cast<long long>(share) * p.tokens * p.heads + row;
             float* part_dst = part_out + part * D + half * (D / 2);
+            float base = fmaf(m, scale, -kBits), here = 1.0f, there = 0.0f;       // factors of O and of what is kept
+            if (kept && live) {
+                const float2 ml = part_kept[2 * part + half];
+                const float top = fmaxf(base, ml.x);
+                here = top == -INFINITY ? 0.0f : exp2_approx(base - top);
+                there = top == -INFINITY ? 0.0f : exp2_approx(ml.x - top);
+                base = top;
+                l = fmaf(ml.y, there, l * here);
+            }
+            const float inverse = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+            T* dst = static_cast<T*>(p.out) + (w.at.row0 + token) * p.ld_out + static_cast<long long>(head * p.group + index - token * p.group) * D + half * (D / 2);
 #pragma unroll (D == 64 ? 2 : 1)
             for (int c = 0; c < D / 2; c += 16) {
                 uint32_t o[16];
-                if (done > 0) {
+                if (some) {
                     tmem_ld_32x16(o_cols + c, o);
                     tmem_ld_wait();
                 } else {
@@ -581,8 +613,9 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                     for (int i = 0; i < 16; ++i) o[i] = 0;
                 }
                 if (!live) continue;
-                if (shares > 1) {
-                    if (done > 0) {
+                if (kept) add_kept(o, here, part_dst + c, there);
+                if (shares > 1 || !last) {
+                    if (some) {
 #pragma unroll
                         for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(part_dst + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                     }
@@ -594,12 +627,14 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                     *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(v[4], v[5], v[6], v[7]);
                 }
             }
-            if (live && half == 0) {
-                const float base = fmaf(m, scale, -kBits);
+            if (live && !last) part_kept[2 * part + half] = make_float2(base, l);
+            else if (live && half == 0) {
                 if (shares > 1) part_ml[part] = make_float2(base, l);
                 else if (p.lse != nullptr) p.lse[row] = l > 0.0f ? (base + log2f(l)) * kLn2 : (l == 0.0f ? -INFINITY : l);
             }
         }
+        kept = true;
+        } while (b < end);
         });
     }
     if (!ok && lane == 0 && p.status != nullptr) atomicOr(p.status, 1);
@@ -656,7 +691,7 @@ shares_join_kernel(const PagedParams p, const int* share_count, const float2* __
 
 template <typename T, int D>
 static int launch(const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares, int* share_count, float2* part_ml,
-                  float* part_out, cudaStream_t stream) {
+                  float2* part_kept, float* part_out, cudaStream_t stream) {
     constexpr int bytes = sizeof(Smem<D>);
     static_assert(bytes <= 227 * 1024 / (3 - tiles<D>()) - (D == 64 ? 1024 : 0), "shared memory");
     const long long slots = pk100_sm_count() * (3 - tiles<D>()), columns = static_cast<long long>(pairs) * p.kv_heads;
@@ -668,7 +703,7 @@ static int launch(const PagedParams& p, const CUtensorMap& map_k, const CUtensor
         if (granted != cudaSuccess) return static_cast<int>(granted);
         const long long most = columns * shares < slots ? columns * shares : slots, blocks = decltype(loop)::value || columns < most ? most : columns;
         pk100_launch_chained(kernel, dim3(static_cast<unsigned>(blocks)), dim3(threads<D>()), bytes, stream, map_k, map_v, p, pairs, shares,
-                             static_cast<unsigned>(slots), share_count, part_ml, part_out);
+                             static_cast<unsigned>(slots), share_count, part_ml, part_kept, part_out);
         return pk100_launch_status();
     };
     return p.requests <= kOrdered ? run(std::false_type()) : run(std::true_type());
@@ -684,12 +719,12 @@ static int launch_join(const PagedParams& p, const int* share_count, const float
 }  // namespace chunk
 
 int paged_attention_chunks(int type, int head_dim, const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares,
-                           int* share_count, float2* part_ml, float* part_out, cudaStream_t stream) {
+                           int* share_count, float2* part_ml, float2* part_kept, float* part_out, cudaStream_t stream) {
     if (type == PK100_TYPE_F16)
-        return head_dim == 128 ? chunk::launch<__half, 128>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_out, stream)
-                               : chunk::launch<__half, 64>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_out, stream);
-    return head_dim == 128 ? chunk::launch<__nv_bfloat16, 128>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_out, stream)
-                           : chunk::launch<__nv_bfloat16, 64>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_out, stream);
+        return head_dim == 128 ? chunk::launch<__half, 128>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_kept, part_out, stream)
+                               : chunk::launch<__half, 64>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_kept, part_out, stream);
+    return head_dim == 128 ? chunk::launch<__nv_bfloat16, 128>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_kept, part_out, stream)
+                           : chunk::launch<__nv_bfloat16, 64>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_kept, part_out, stream);
 }
 
 int paged_attention_join(int type, int head_dim, const PagedParams& p, const int* share_count, const float2* part_ml, const float* part_out, cudaStream_t stream) {

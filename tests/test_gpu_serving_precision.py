@@ -6,6 +6,8 @@ import numpy as np
 import pytest
 import torch
 
+from tests import serving_reference as R
+
 pytestmark = pytest.mark.gpu
 
 F16, BF16 = torch.float16, torch.bfloat16
@@ -169,3 +171,61 @@ def test_attention_of_a_scale_of_zero_and_of_none(pk, cuda, dim, tokens):
     assert float((lse.double() - math.log(384.0)).abs().max()) <= 1.1e-4
     out = pk.ops.paged_attention(q, *rest, causal=False, scale=math.nan, lse=lse)
     assert bool(out.isnan().all()) and bool(lse.isnan().all())
+
+
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("kernel,dim", [("rows", 64), ("rows", 128), ("chunk", 64), ("chunk", 128)])
+def test_attention_sums_of_small_weights_beside_a_large_one(pk, cuda, kernel, dim, first):
+    """The same rows with values of 1 and -1: sums that hold the large term have to take up the small ones.  Tolerance as above, and
+    what the tensor cores may lose of the 8192 keys that they add to one sum, 2.8e-3 / 16.  lse: the scores are exact; ln 2 and
+    log2(e) as factors of them, with their roundings, 26 * 2^-22, and the exponentials' 1.1e-4 of the small part; below 1e-5."""
+    args, want, want_lse = _one_key_and_many(kernel, dim, F16, first, 1.0)
+    lse = torch.empty(args["query"].shape[:2], device="cuda")
+    out = pk.ops.paged_attention(**args, lse=lse)
+    tolerance = 2.0 ** -11 * (1 + abs(want)) + 2.0 ** 17 * 2.0 ** -31 + 8192 * 2.0 ** -25.5 + 1e-5
+    assert tolerance < 0.5 * abs(1 / (1 + 2.0 ** -8.5) - want)                   # what a row without the small ones is off
+    assert float((out.double() - want).abs().max()) <= tolerance
+    assert float((lse.double() - want_lse).abs().max()) <= 1e-5
+
+
+def _repeated(keys, new, requests, dim, heads, kv, value, dtype=F16):
+    """Requests over 16 pages again and again: as many keys as wanted, all of score 0 and of this value."""
+    page, pages = 256, 16
+    table = (torch.arange(-(-keys // page), device="cuda", dtype=torch.int32) % pages).expand(requests, -1).contiguous()
+    return dict(query=torch.zeros(requests * new, heads, dim, dtype=dtype, device="cuda"), key_cache=torch.zeros(pages, page, kv, dim, dtype=dtype, device="cuda"),
+                value_cache=torch.full((pages, page, kv, dim), value, dtype=dtype, device="cuda"), block_table=table,
+                starts=torch.arange(requests + 1, dtype=torch.int32, device="cuda") * new,
+                lengths=torch.full((requests,), keys, dtype=torch.int32, device="cuda"), causal=False, max_new=new)
+
+
+@pytest.mark.parametrize("requests,new,heads", [(37, 1, 8), (1, 4864, 8)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_means_of_many_keys(pk, cuda, dim, requests, new, heads):
+    """The mean of 2^19 equal values is that value: the weights are exact, the tensor cores lose up to 2^-23 of a sum for 16 keys, 512 times
+    at most, and the output is rounded."""
+    for keys in (1 << 19, 70001, 8192, 8193):
+        args = _repeated(keys, new, requests, dim, heads, 8, 1.7)
+        value = float(args["value_cache"][0, 0, 0, 0])
+        lse = torch.empty(args["query"].shape[:2], device="cuda")
+        out = pk.ops.paged_attention(**args, lse=lse)
+        assert float((out.double() - value).abs().max()) <= value * (2.0 ** -11 + 512 * 2.0 ** -23 + 1e-6), keys
+        assert float((lse.double() - math.log(keys)).abs().max()) <= 2e-6 * math.log(keys)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_whose_maximum_grows_over_many_keys(pk, cuda, dim, dtype):
+    """Rows over 20 000 keys, two and a half sums in tensor memory, while the scores grow: what has left it is scaled down."""
+    kv, heads, tokens, page, keys = 8, 16, 2400, 64, 20000
+    pages = -(-keys // page)
+    normal = lambda seed, *shape: torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+    grow = torch.linspace(0.05, 3.0, pages * page, device="cuda")[:, None, None]
+    k = (normal(1, pages * page, kv, dim) * grow).to(dtype)
+    v, q = normal(2, pages * page, kv, dim).to(dtype), normal(3, tokens, heads, dim).to(dtype)
+    lse = torch.empty(tokens, heads, device="cuda")
+    out = pk.ops.paged_attention(q, k.view(pages, page, kv, dim), v.view(pages, page, kv, dim), torch.arange(pages, dtype=torch.int32, device="cuda")[None],
+                                 torch.tensor([0, tokens], dtype=torch.int32, device="cuda"), torch.tensor([keys], dtype=torch.int32, device="cuda"), lse=lse)
+    rows = torch.tensor([0, 1, 127, 128, 1000, 2271, 2399], device="cuda")
+    want, want_lse, spread, off = R.attention(q[rows], k[:keys], v[:keys], keys - tokens + rows, True, 0, 1 / math.sqrt(dim))
+    assert bool(((out[rows].double() - want).abs() <= R.attention_tolerance(want, spread, off, v, 1, dtype) + 1e-4 * spread).all())
+    assert float((lse[rows].double() - want_lse).abs().max()) <= 24 * 2.0 ** -22 * off + 1e-5 * (1 + off)
