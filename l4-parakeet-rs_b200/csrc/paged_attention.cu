@@ -508,7 +508,7 @@ static int cache_map(CUtensorMap* map, const void* base, const pk100_paged_atten
 struct PagedPlan {
     int grid;                                            // blocks of the few-row kernel
     int pairs, shares;                                   // of the other one
-    long long counts, parts, part_out, share_count, share_ml, share_out, share_kept, bytes;
+    long long counts, parts, part_out, share_count, share_ml, share_out, kept_ml, kept_out, bytes;
 };
 
 static long long round256(long long n) { return (n + 255) / 256 * 256; }
@@ -536,9 +536,10 @@ static PagedPlan paged_plan_of(const pk100_paged_attention_args& a) {
     plan.shares = shares < 1 ? 1 : static_cast<int>(shares);
     const long long share_rows = plan.shares > 1 ? static_cast<long long>(plan.shares) * a.tokens * a.heads : 0;
     plan.share_out = plan.share_ml + round256(share_rows * 8);
-    const long long kept_rows = blocks * kBlock > kFoldKeys ? static_cast<long long>(plan.shares) * a.tokens * a.heads : 0;
-    plan.share_kept = plan.share_out + round256((kept_rows > share_rows ? kept_rows : share_rows) * a.head_dim * 4);
-    plan.bytes = plan.share_kept + round256(kept_rows * 16);
+    const long long kept_rows = blocks * kBlock > kFoldKeys / 2 ? static_cast<long long>(plan.shares) * a.tokens * a.heads : 0;
+    plan.kept_ml = plan.share_out + round256(share_rows * a.head_dim * 4);
+    plan.kept_out = plan.kept_ml + round256(kept_rows * 16);
+    plan.bytes = plan.kept_out + round256(kept_rows * a.head_dim * 4);
     return plan;
 }
 
@@ -641,8 +642,10 @@ extern "C" int pk100_paged_attention(void* stream_v, const pk100_paged_attention
     int* share_count = reinterpret_cast<int*>(ws + plan.share_count);
     float2* share_ml = reinterpret_cast<float2*>(ws + plan.share_ml);
     float* share_out = reinterpret_cast<float*>(ws + plan.share_out);
-    float2* share_kept = reinterpret_cast<float2*>(ws + plan.share_kept);
-    if (many && (rc = paged_attention_chunks(a->type, a->head_dim, p, map_k, map_v, plan.pairs, plan.shares, share_count, share_ml, share_kept, share_out, stream)) != PK100_OK) return rc;
+    float2* kept_ml = reinterpret_cast<float2*>(ws + plan.kept_ml);
+    float* kept_out = reinterpret_cast<float*>(ws + plan.kept_out);
+    if (many && (rc = paged_attention_chunks(a->type, a->head_dim, p, map_k, map_v, plan.pairs, plan.shares, share_count, share_ml, share_out, kept_ml, kept_out, stream)) != PK100_OK)
+        return rc;
     if (a->type == PK100_TYPE_F16)
         rc = a->head_dim == 128 ? launch_rows<__half, 128>(*a, p, plan, map_k, map_v, many, stream) : launch_rows<__half, 64>(*a, p, plan, map_k, map_v, many, stream);
     else

@@ -67,17 +67,17 @@ __device__ __forceinline__ void add_compensated(float& sum, float& excess, float
     excess = (sum - before) - part;
 }
 
-// Keys that the chunk kernel adds up in tensor memory; the sums of more are kept in part_out and part_kept.
-constexpr int kFoldKeys = 8192;
+// Keys that the chunk kernel adds up in tensor memory; the sums of more are kept in kept_ml and kept_out.
+constexpr int kFoldKeys = 16384;
 
 // The kernel for requests of more than p.few_rows rows (paged_attention_tcgen05.cu): `pairs` numbers of pairs of tiles
 // (tokens * group / pair_rows + requests).  Where the pairs are few, a row's keys are shared out to up to `shares`; how many it came
 // to goes to share_count, their parts to part_ml [shares, tokens, heads] and part_out [shares, tokens, heads, head_dim], and
-// paged_attention_join adds them up (shares == 1: none of that).  Where max_pages hold more than kFoldKeys keys, part_kept [shares,
-// tokens, heads, 2] is there, and part_out of one share at least.
+// paged_attention_join adds them up (shares == 1: none of that).  Where max_pages hold more than half of kFoldKeys, kept_ml [shares,
+// tokens, heads, 2] and kept_out [shares, tokens, heads, head_dim] are there.
 constexpr int pair_rows(int head_dim) { return head_dim == 128 ? 256 : 128; }
 int paged_attention_chunks(int type, int head_dim, const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares,
-                           int* share_count, float2* part_ml, float2* part_kept, float* part_out, cudaStream_t stream);
+                           int* share_count, float2* part_ml, float* part_out, float2* kept_ml, float* kept_out, cudaStream_t stream);
 int paged_attention_join(int type, int head_dim, const PagedParams& p, const int* share_count, const float2* part_ml, const float* part_out, cudaStream_t stream);
 
 }  // namespace pk100

@@ -16,8 +16,10 @@ template <int D> constexpr int threads() { return softmax_warps<D>() * 32 + 64; 
 constexpr int kAtom = kTile * 128;              // 128 rows x 64 elements, 128-byte swizzle
 constexpr int kBox = 64;                        // most keys of a TMA box
 // Key blocks after which O begins again at zero.  The tensor cores cut off what falls below the last bit of the sum that they
-// add to, up to 2^-23 of it for 16 keys: 6e-5 in 64 blocks (4e-3 over 2^19 keys in one sum).
+// add to, up to 2^-23 of it for 16 keys: 1.2e-4 in 128 blocks (4e-3 over 2^19 keys in one sum).
 constexpr int kFold = kFoldKeys / kTile;
+// of the first time: the second tile of a pair has its turn under the first one's products
+__device__ __forceinline__ constexpr int first_fold(int tile) { return kFold - tile * (kFold / 2); }
 constexpr int kByFma = 5;                       // of 16 pairs of scores, whose exponentials the FMA pipe forms (two prompts: 4 472,
                                                 // 5 427, 6 454 us on one card: the order of the instructions moves with it)
 
@@ -100,18 +102,6 @@ __device__ __forceinline__ float weights_of_scores(const float (&s)[64], float s
     }
     const float2 sums = halves_of(sum);
     return sums.x + sums.y;
-}
-
-// o = here * o + there * dst: 16 features of a row, which the thread alone has.
-__device__ __forceinline__ void add_kept(uint32_t (&o)[16], float here, const float* dst, float there) {
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(dst + i);
-        o[i] = __float_as_uint(fmaf(v.x, there, __uint_as_float(o[i]) * here));
-        o[i + 1] = __float_as_uint(fmaf(v.y, there, __uint_as_float(o[i + 1]) * here));
-        o[i + 2] = __float_as_uint(fmaf(v.z, there, __uint_as_float(o[i + 2]) * here));
-        o[i + 3] = __float_as_uint(fmaf(v.w, there, __uint_as_float(o[i + 3]) * here));
-    }
 }
 
 // What a block of threads works on: 256 rows of one request and key-value head, over a share of their keys.
@@ -256,7 +246,7 @@ template <typename T, int D, bool kLoop>
 __global__ void __launch_bounds__(threads<D>(), 3 - tiles<D>())
 paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p,
                              const int pairs, const int most_shares, const unsigned slots, int* share_count, float2* part_ml,
-                             float2* part_kept, float* part_out) {
+                             float* part_out, float2* kept_ml, float* kept_out) {
     extern __shared__ __align__(1024) uint8_t chunk_raw[];             // (the swizzled atoms need it)
     constexpr int kHalves = D / 64, kSlots = ring_slots<D>(), kSlotBytes = kHalves * kAtom, kTiles = tiles<D>(), kSoftmaxWarps = softmax_warps<D>();
     constexpr uint32_t kColumns = 256 * kTiles;                 // of tensor memory: S and O of the tiles
@@ -443,7 +433,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
 #pragma unroll
                         for (int ks = 0; ks < kTile / 16; ++ks)
                             mma_from_tmem(leader, tmem + kTiles * kTile + t * D, tmem + t * kTile + ks * 8, desc_v + v_slot * (kSlotBytes / 16) + ks * 128u, idesc_o,
-                                          ks > 0 || (b - tile_from[t]) % kFold != 0);
+                                          ks > 0 || (b > tile_from[t] && (b - tile_from[t] - first_fold(t)) % kFold != 0));
                         tc_commit_if(leader, &sm.o_done[t]);
                     }
                     if (b + 1 < w.to && active(t, b + 1)) {
@@ -514,7 +504,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         bool kept = false;
 #pragma unroll 1
         do {
-        const int stop = min(b + kFold, end);
+        const int stop = min(b + (kept ? kFold : first_fold(t)), end);
         // m: reference maximum of the raw scores; l: sum over this half of the keys; limit: growth of the maximum (base 2) that m follows
         float m = -INFINITY, l = 0.0f, limit = 8.0f;
         const bool some = b < end;
@@ -591,46 +581,81 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             const long long row = static_cast<long long>(w.at.row0 + token) * p.heads + head * p.group + index - token * p.group;
             const long long part = static_cast<long long>(share) * p.tokens * p.heads + row;
             float* part_dst = part_out + part * D + half * (D / 2);
+            // Where the 4 features from 4 * i on of this thread's half are kept: nobody else reads them, so the 32 rows of a warp put
+            // theirs side by side into one row of the output's shape after the other (whose rows all exist where the tile is full).
+            auto kept_at = [&](int i) {
+                constexpr int kEach = D / 4, kRowsEach = 32 / kEach;                   // pieces of a row; rows that 32 of them take
+                const bool full = tile_rows >= kTile;
+                const int r = full ? quad * 32 + (half * (kEach / 2) + i) * kRowsEach + lane / kEach : tile_row;
+                const int at = w.row + t * kTile + r, tok = at / p.group;
+                const long long to = static_cast<long long>(share) * p.tokens * p.heads + static_cast<long long>(w.at.row0 + tok) * p.heads + head * p.group + at - tok * p.group;
+                return reinterpret_cast<float4*>(kept_out + to * D) + (full ? lane % kEach : half * (kEach / 2) + i);
+            };
             float base = fmaf(m, scale, -kBits), here = 1.0f, there = 0.0f;       // factors of O and of what is kept
             if (kept && live) {
-                const float2 ml = part_kept[2 * part + half];
+                const float2 ml = kept_ml[2 * part + half];
                 const float top = fmaxf(base, ml.x);
                 here = top == -INFINITY ? 0.0f : exp2_approx(base - top);
                 there = top == -INFINITY ? 0.0f : exp2_approx(ml.x - top);
                 base = top;
                 l = fmaf(ml.y, there, l * here);
             }
-            const float inverse = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-            T* dst = static_cast<T*>(p.out) + (w.at.row0 + token) * p.ld_out + static_cast<long long>(head * p.group + index - token * p.group) * D + half * (D / 2);
-#pragma unroll (D == 64 ? 2 : 1)
-            for (int c = 0; c < D / 2; c += 16) {
-                uint32_t o[16];
-                if (some) {
+            if (kept || !last) {                             // O and what is kept, to where it is kept or back to tensor memory
+#pragma unroll 1
+                for (int c = 0; c < D / 2; c += 16) {
+                    uint32_t o[16];
                     tmem_ld_32x16(o_cols + c, o);
                     tmem_ld_wait();
-                } else {
+                    if (live) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] = 0;
-                }
-                if (!live) continue;
-                if (kept) add_kept(o, here, part_dst + c, there);
-                if (shares > 1 || !last) {
-                    if (some) {
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(part_dst + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        for (int i = 0; i < 16; i += 4) {
+                            float4* at = kept_at((c + i) / 4);
+                            const float4 old = kept ? *at : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            const float4 v = make_float4(fmaf(old.x, there, __uint_as_float(o[i]) * here), fmaf(old.y, there, __uint_as_float(o[i + 1]) * here),
+                                                         fmaf(old.z, there, __uint_as_float(o[i + 2]) * here), fmaf(old.w, there, __uint_as_float(o[i + 3]) * here));
+                            if (!last) *at = v;
+                            o[i] = __float_as_uint(v.x);
+                            o[i + 1] = __float_as_uint(v.y);
+                            o[i + 2] = __float_as_uint(v.z);
+                            o[i + 3] = __float_as_uint(v.w);
+                        }
                     }
-                } else {
-                    uint32_t v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = packed_of(__uint_as_float(o[2 * i]) * inverse, __uint_as_float(o[2 * i + 1]) * inverse, T());
-                    *reinterpret_cast<uint4*>(dst + c) = make_uint4(v[0], v[1], v[2], v[3]);
-                    *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+                    if (last) tmem_st_32x16(o_cols + c, o);
                 }
+                if (last) tmem_st_wait();
+                else if (live) kept_ml[2 * part + half] = make_float2(base, l);
             }
-            if (live && !last) part_kept[2 * part + half] = make_float2(base, l);
-            else if (live && half == 0) {
-                if (shares > 1) part_ml[part] = make_float2(base, l);
-                else if (p.lse != nullptr) p.lse[row] = l > 0.0f ? (base + log2f(l)) * kLn2 : (l == 0.0f ? -INFINITY : l);
+            if (last) {
+                const float inverse = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+                T* dst = static_cast<T*>(p.out) + (w.at.row0 + token) * p.ld_out + static_cast<long long>(head * p.group + index - token * p.group) * D + half * (D / 2);
+#pragma unroll (D == 64 ? 2 : 1)
+                for (int c = 0; c < D / 2; c += 16) {
+                    uint32_t o[16];
+                    if (some) {
+                        tmem_ld_32x16(o_cols + c, o);
+                        tmem_ld_wait();
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = 0;
+                    }
+                    if (!live) continue;
+                    if (shares > 1) {
+                        if (some) {
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(part_dst + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        }
+                    } else {
+                        uint32_t v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = packed_of(__uint_as_float(o[2 * i]) * inverse, __uint_as_float(o[2 * i + 1]) * inverse, T());
+                        *reinterpret_cast<uint4*>(dst + c) = make_uint4(v[0], v[1], v[2], v[3]);
+                        *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+                    }
+                }
+                if (live && half == 0) {
+                    if (shares > 1) part_ml[part] = make_float2(base, l);
+                    else if (p.lse != nullptr) p.lse[row] = l > 0.0f ? (base + log2f(l)) * kLn2 : (l == 0.0f ? -INFINITY : l);
+                }
             }
         }
         kept = true;
@@ -691,7 +716,7 @@ shares_join_kernel(const PagedParams p, const int* share_count, const float2* __
 
 template <typename T, int D>
 static int launch(const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares, int* share_count, float2* part_ml,
-                  float2* part_kept, float* part_out, cudaStream_t stream) {
+                  float* part_out, float2* kept_ml, float* kept_out, cudaStream_t stream) {
     constexpr int bytes = sizeof(Smem<D>);
     static_assert(bytes <= 227 * 1024 / (3 - tiles<D>()) - (D == 64 ? 1024 : 0), "shared memory");
     const long long slots = pk100_sm_count() * (3 - tiles<D>()), columns = static_cast<long long>(pairs) * p.kv_heads;
@@ -703,7 +728,7 @@ static int launch(const PagedParams& p, const CUtensorMap& map_k, const CUtensor
         if (granted != cudaSuccess) return static_cast<int>(granted);
         const long long most = columns * shares < slots ? columns * shares : slots, blocks = decltype(loop)::value || columns < most ? most : columns;
         pk100_launch_chained(kernel, dim3(static_cast<unsigned>(blocks)), dim3(threads<D>()), bytes, stream, map_k, map_v, p, pairs, shares,
-                             static_cast<unsigned>(slots), share_count, part_ml, part_kept, part_out);
+                             static_cast<unsigned>(slots), share_count, part_ml, part_out, kept_ml, kept_out);
         return pk100_launch_status();
     };
     return p.requests <= kOrdered ? run(std::false_type()) : run(std::true_type());
@@ -719,12 +744,12 @@ static int launch_join(const PagedParams& p, const int* share_count, const float
 }  // namespace chunk
 
 int paged_attention_chunks(int type, int head_dim, const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int pairs, int shares,
-                           int* share_count, float2* part_ml, float2* part_kept, float* part_out, cudaStream_t stream) {
+                           int* share_count, float2* part_ml, float* part_out, float2* kept_ml, float* kept_out, cudaStream_t stream) {
     if (type == PK100_TYPE_F16)
-        return head_dim == 128 ? chunk::launch<__half, 128>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_kept, part_out, stream)
-                               : chunk::launch<__half, 64>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_kept, part_out, stream);
-    return head_dim == 128 ? chunk::launch<__nv_bfloat16, 128>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_kept, part_out, stream)
-                           : chunk::launch<__nv_bfloat16, 64>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_kept, part_out, stream);
+        return head_dim == 128 ? chunk::launch<__half, 128>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_out, kept_ml, kept_out, stream)
+                               : chunk::launch<__half, 64>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_out, kept_ml, kept_out, stream);
+    return head_dim == 128 ? chunk::launch<__nv_bfloat16, 128>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_out, kept_ml, kept_out, stream)
+                           : chunk::launch<__nv_bfloat16, 64>(p, map_k, map_v, pairs, shares, share_count, part_ml, part_out, kept_ml, kept_out, stream);
 }
 
 int paged_attention_join(int type, int head_dim, const PagedParams& p, const int* share_count, const float2* part_ml, const float* part_out, cudaStream_t stream) {
