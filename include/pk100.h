@@ -706,7 +706,8 @@ int pk100_paged_plan(void* stream, const pk100_paged_plan_args* args);
  * out; its keys are the first lengths[r] positions of its pages, the new tokens' own among them, and its i-th new
  * token stands at position p = lengths[r] - new + i:
  *   out = softmax_j(scale * q . k_j) . v_j over the positions j < lengths[r], j <= p when causal, j > p - window when
- *   window > 0;  lse (fp32 [tokens, heads], may be NULL) = log sum_j exp(scale * q . k_j).
+ *   window > 0;  lse (fp32 [tokens, heads], may be NULL) = log sum_j exp(scale * q . k_j), to 1e-5 beside the rounding of the
+ *   fp32 scores.
  * A row that sees nothing gets zeros and lse -infinity.  Rows behind starts[requests] are not touched.
  * Query head h reads key-value head h / (heads / kv_heads).  head_dim 64 or 128; page_size 16, 32, 64, 128 or 256.
  * Element (page, token, head, d) of both caches is at page * page_stride + token * token_stride + head * head_stride

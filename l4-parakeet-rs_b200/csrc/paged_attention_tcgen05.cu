@@ -20,8 +20,8 @@ constexpr int kBox = 64;                        // most keys of a TMA box
 constexpr int kFold = kFoldKeys / kTile;
 // of the first time: the second tile of a pair has its turn under the first one's products
 __device__ __forceinline__ constexpr int first_fold(int tile) { return kFold - tile * (kFold / 2); }
-constexpr int kByFma = 5;                       // of 16 pairs of scores, whose exponentials the FMA pipe forms (two prompts: 4 472,
-                                                // 5 427, 6 454 us on one card: the order of the instructions moves with it)
+constexpr int kByFma = 5;                       // of 16 pairs of scores, whose exponentials the FMA pipe forms (two prompts: 4 426,
+                                                // 5 423, 6 435 us on one card: the order of the instructions moves with it)
 
 template <int D> constexpr int ring_slots() { return 5; }
 
@@ -54,7 +54,7 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
 }
 
 // 2^x for two values at most 16: n = rint(x), a polynomial of the remainder (minimax of the relative error among those of
-// degree 3 that are 1 at 0: 1.01e-4, a fifth of half a step of an fp16 P), n into the exponent.  x below -127 counts as -127,
+// degree 4 that are 1 at 0: 2.9e-6; of degree 3 the 1.01e-4 showed in the lse of rows that such a weight dominates), n into the exponent.  x below -127 counts as -127,
 // where 1 less 127 in the exponent is zero to the bit: a masked score has no weight at all (and between -127 and -126 no result
 // is below zero or above 2^-126).  NaN (0x7fffffff) leaves as the largest number, 0x7f7fffff, which is infinity in 16 bits.
 // On the FMA pipe, where ex2.approx (16 a clock and SM) would take as long as the tensor cores' products.
@@ -64,8 +64,9 @@ __device__ __forceinline__ Pair exp2_fma(Pair x) {
     const Pair magic = pair_of(12582912.0f, 12582912.0f), back = pair_of(-12582912.0f, -12582912.0f);       // 1.5 * 2^23
     const Pair n = pair_add(x, magic);
     const Pair r = pair_fma(pair_add(n, back), pair_of(-1.0f, -1.0f), x);
-    Pair y = pair_fma(r, pair_of(0.055009059607982635f, 0.055009059607982635f), pair_of(0.2422109693288803f, 0.2422109693288803f));
-    y = pair_fma(r, y, pair_of(0.6932829022407532f, 0.6932829022407532f));
+    Pair y = pair_fma(r, pair_of(0.009582852944731712f, 0.009582852944731712f), pair_of(0.055906426161527634f, 0.055906426161527634f));
+    y = pair_fma(r, y, pair_of(0.24024099111557007f, 0.24024099111557007f));
+    y = pair_fma(r, y, pair_of(0.6931241750717163f, 0.6931241750717163f));
     y = pair_fma(r, y, pair_of(1.0f, 1.0f));
     const float2 whole = halves_of(n), part = halves_of(y);
     return pair_of(__uint_as_float(__float_as_uint(part.x) + (__float_as_uint(whole.x) << 23)),

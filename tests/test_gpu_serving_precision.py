@@ -229,3 +229,33 @@ def test_attention_whose_maximum_grows_over_many_keys(pk, cuda, dim, dtype):
     want, want_lse, spread, off = R.attention(q[rows], k[:keys], v[:keys], keys - tokens + rows, True, 0, 1 / math.sqrt(dim))
     assert bool(((out[rows].double() - want).abs() <= R.attention_tolerance(want, spread, off, v, 1, dtype) + 1e-4 * spread).all())
     assert float((lse[rows].double() - want_lse).abs().max()) <= 24 * 2.0 ** -22 * off + 1e-5 * (1 + off)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_lse_of_a_row_that_one_key_dominates(pk, cuda, dim, dtype):
+    """In the second block of keys, in each of its places (one a head), a key a little less than 2^8 above the first one's largest, so
+    that the kernel's reference stays behind: the row's lse is that key's score and the sum's logarithm.  The exponentials are good
+    to 2.9e-6, their argument and the sum to some units of 2^-22 of at most 16, the result to 2^-23 of at most 6."""
+    heads, tokens, keys = 128, 40, 256
+    q = torch.zeros(tokens, heads, dim, dtype=dtype, device="cuda")
+    q[..., 0] = 1
+    v = torch.randn(4, 64, heads, dim, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda").to(dtype)
+    for large in (7.25, 7.3125, 6.625, 5.6875, 4.5):
+        k = torch.zeros(4, 64, heads, dim, dtype=dtype, device="cuda")
+        flat = k.view(keys, heads, dim)
+        flat[:, :, 0] = -40.0
+        flat[0, :, 0] = 0.0
+        for h in range(heads):
+            flat[128 + h, h, 0] = large
+        lse = torch.empty(tokens, heads, device="cuda")
+        out = pk.ops.paged_attention(q, k, v, torch.arange(4, dtype=torch.int32, device="cuda")[None], torch.tensor([0, tokens], dtype=torch.int32, device="cuda"),
+                                     torch.tensor([keys], dtype=torch.int32, device="cuda"), causal=False, scale=math.log(2.0), lse=lse)
+        total = 1 + 2.0 ** large + 254 * 2.0 ** -40
+        assert float((lse.double() - math.log(total)).abs().max()) <= 2.9e-6 + 16 * 2.0 ** -22 + 6 * 2.0 ** -23, large
+        flat_v = v.view(keys, heads, dim).double()
+        picked = torch.stack([flat_v[128 + h, h] for h in range(heads)])
+        want = (flat_v[0] + 2.0 ** large * picked + 2.0 ** -40 * (flat_v.sum(0) - flat_v[0] - picked)) / total
+        half = 2.0 ** -11 if dtype is F16 else 2.0 ** -8
+        bound = (half + 1e-5) * (flat_v[0].abs() + 2.0 ** large * picked.abs()) / total + half * want.abs() + 1e-6
+        assert bool(((out.double() - want).abs() <= bound).all())
