@@ -749,6 +749,12 @@ typedef struct pk100_paged_attention_args {
 long long pk100_paged_attention_workspace_bytes(const pk100_paged_attention_args* args);
 int pk100_paged_attention(void* stream, const pk100_paged_attention_args* args);
 
+/* How long a wait inside the kernels of pk100_gemv_w4g128 and pk100_paged_attention may take from now on (a captured launch keeps
+ * what was set at its capture): negative, the default, is 2 s, far beyond any legal one.  A kernel whose wait runs out sets bit 0
+ * of its status, leaves its output undefined and returns when nothing of its own is in flight.  0 gives up on all that is not there at the
+ * first look: for tests of a host's error path. */
+int pk100_set_wait_limit(long long nanoseconds);
+
 #ifdef __cplusplus
 }
 #endif

@@ -280,6 +280,16 @@ int pk100_tensor_map_4d(void* map, const void* base, const unsigned long long (&
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? PK100_OK : PK100_ERR_DRIVER;
 }
 
+static std::atomic<long long> g_wait_limit{-1};
+extern "C" int pk100_set_wait_limit(long long nanoseconds) {
+    g_wait_limit.store(nanoseconds < 0 ? -1 : nanoseconds);
+    return PK100_OK;
+}
+unsigned long long pk100_wait_limit() {
+    const long long limit = g_wait_limit.load(std::memory_order_relaxed);
+    return limit < 0 ? pk100::kWaitBudgetNs : static_cast<unsigned long long>(limit);
+}
+
 int pk100_cta_budget() { return pk100::shared_budget(); }
 
 bool pk100_dependent_launch_enabled() { return pk100::g_dependent_launch.load(std::memory_order_relaxed) != 0; }

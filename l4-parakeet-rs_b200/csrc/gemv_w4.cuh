@@ -24,6 +24,7 @@ struct GemvParams {
     float alpha; int valid_rows;
     void* out; long long ld_out; int out_type;
     int* status;                      // of the wide kernel's waits
+    unsigned long long wait_ns;       // their limit
 };
 
 // 8 codes of a word -> 4 pairs of weights f16(code * scale), pair i = codes (i, i + 4).  With its sign bit flipped a code

@@ -233,6 +233,7 @@ extern "C" int pk100_gemv_w4g128(void* stream_v, const pk100_gemm_args* a) {
     p.out = a->out; p.ld_out = a->ld_out; p.out_type = a->out_type;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
     p.status = a->status;
+    p.wait_ns = pk100_wait_limit();
     // From 16 384 weight rows on (three and a half tiles a cluster) the wide kernel: 13 rows by 28 672 x 8192 in 36 us against 50, x 1024
     // in 10.7 against 14.9; one row about the same; 8192 x 4096 9.7 against 9.4, 4096 x 14 336 17.5 against 15.0.
     if (a->n >= kWideRows && a->k <= gemv_wide_limit()) {

@@ -18,14 +18,16 @@ constexpr int kMostGroups = 32;                 // of a block: 4 KB of activatio
 struct Smem {
     uint8_t x[kMostGroups][2][16 * 128];        // activations in the codes' order, 64 k an atom, 128-byte swizzle
     uint8_t ring[kStages][kStageBytes];         // codes, 128-byte swizzle; at the end of a round the block's sums
-    uint64_t full[kStages], empty[kStages], a_full[kBuffers], a_empty[kBuffers], done, x_ready;
+    uint64_t full[kStages], empty[kStages], a_full[kBuffers], a_empty[kBuffers], done, x_ready, drained;
     uint32_t tmem;
     int abort;
 };
 static_assert(kStages * kStageBytes >= kTiles / 2 * kTile * 16 * 4, "the sums of half a round fit the ring");
 
 #define WIDE_WAIT(bar, parity) \
-    if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&(bar), (parity), abort_flag)) != 0)) break
+    if (!(ok = __all_sync(0xffffffffu, mbar_wait_within(&(bar), (parity), abort_flag, p.wait_ns)) != 0)) break
+#define WIDE_LOOK(bar, parity) \
+    if (!(ok = __all_sync(0xffffffffu, mbar_look_within(&(bar), (parity), abort_flag, p.wait_ns)) != 0)) break
 
 __device__ __forceinline__ float4 load_from_cluster(uint32_t addr) {
     float4 v;
@@ -63,6 +65,7 @@ gemv_w4g128_wide_kernel(const __grid_constant__ CUtensorMap map_codes, const Gem
             mbar_init(&sm.a_empty[b], 1);
         }
         mbar_init(&sm.done, 1);
+        mbar_init(&sm.drained, 1);
         mbar_init(&sm.x_ready, kWarps);
         fence_barrier_init();
         prefetch_tensormap(&map_codes);
@@ -101,21 +104,16 @@ gemv_w4g128_wide_kernel(const __grid_constant__ CUtensorMap map_codes, const Gem
             for (int t = 0; ok && t < tiles; ++t)
                 for (int pair = 0; pair < pairs; ++pair, ++it) {
                     const uint32_t s = it % kStages;
-                    WIDE_WAIT(sm.empty[s], (it / kStages + 1) & 1);
+                    WIDE_LOOK(sm.empty[s], (it / kStages + 1) & 1);
                     mbar_arrive_expect_tx_if(leader, &sm.full[s], kStageBytes);
                     tma_load_2d_if(leader, sm.ring[s], &map_codes, &sm.full[s], (pair0 + pair) * kGroup, (first + t) * kTile);
                 }
-            if (!ok || *abort_flag != 0) {       // copies still in flight where a wait ran out
-                const uint64_t start = global_timer_ns();
-                for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i)
-                    while (!mbar_try_wait(&sm.full[i % kStages], (i / kStages) & 1) && global_timer_ns() - start < 100000000ull) {}
-            }
         } else if (warp == kWarps + 1) {
             // ------------------------------------------------------------ MMA
             constexpr uint32_t idesc = make_instr_desc<KIND_F16>(kTile, 16);
             const uint64_t desc_x = make_smem_desc<128>(smem_u32(sm.x));
             const bool leader = elect_one();
-            ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&sm.x_ready, 0, abort_flag)) != 0;
+            ok = ok && __all_sync(0xffffffffu, mbar_look_within(&sm.x_ready, 0, abort_flag, p.wait_ns)) != 0;
             for (int t = 0; ok && t < tiles; ++t)
                 for (int group = 0; group < count; ++group, ++it) {
                     const uint32_t b = it % kBuffers;
@@ -177,7 +175,7 @@ gemv_w4g128_wide_kernel(const __grid_constant__ CUtensorMap map_codes, const Gem
             float* sums = reinterpret_cast<float*>(sm.ring);
             if (warp < kWarps) {
                 if (from == 0 && count > 0) {
-                    ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&sm.done, rounds & 1, abort_flag)) != 0;
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait_within(&sm.done, rounds & 1, abort_flag, p.wait_ns)) != 0;
                     tc_fence_after_sync();
                 }
                 const int quad = warp % 4, row = quad * 32 + lane;
@@ -223,6 +221,15 @@ gemv_w4g128_wide_kernel(const __grid_constant__ CUtensorMap map_codes, const Gem
     if (!ok && lane == 0 && p.status != nullptr) atomicOr(p.status, 1);
     tc_fence_before_sync();
     __syncthreads();
+    // where a wait ran out, whoever's: copies and products must end before the block's memory is given away
+    if (*abort_flag != 0) {
+        if (warp == kWarps) {
+            for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i) mbar_drain(&sm.full[i % kStages], (i / kStages) & 1);
+        } else if (warp == kWarps + 1) {
+            tc_commit_if(elect_one(), &sm.drained);           // (the same lane every time)
+            mbar_drain(&sm.drained, 0);
+        }
+    }
     if (warp == kWarps + 1) tmem_dealloc(tmem, 512);
 }
 

@@ -236,12 +236,13 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
     const int first_request = sm.request;
     const long long first_base = sm.base;
     volatile int* abort_flag = &sm.abort;
+    int it = 0;                                          // stages of this role so far
+    bool ok = true;
 
     if (warp == kRowWarps) {
         // ------------------------------------------------------------ loads
         const int box = min(kBlock, 1 << p.page_shift), boxes = kBlock / box;
-        int it = 0;
-        bool bad = false, ok = true;
+        bool bad = false;
         rows_walk(p, first_request, first_base, begin, end, [&](const RowsShape& s, int request, int head, int tile, long long, int b0, int b1, bool) {
             const int row_first = tile * kRows / p.group, row_last = min((tile * kRows + kRows - 1) / p.group, s.at.n - 1);
             const int lo = s.at.lo(p, row_first), hi = s.at.hi(p, row_last);
@@ -251,7 +252,7 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
             int held = -32, id = 0;                         // pages [held, held + 32): one a lane
             for (int b = from; ok && b < to; ++b, ++it) {
                 const int stage = it % kStages;
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sm.empty[stage], (it / kStages + 1) & 1, abort_flag)) != 0;
+                ok = __all_sync(0xffffffffu, mbar_look_within(&sm.empty[stage], (it / kStages + 1) & 1, abort_flag, p.wait_ns)) != 0;
                 if (!ok) break;
                 const int key = b * kBlock + min(lane, boxes - 1) * box, page = key >> p.page_shift;
                 const int last = (b * kBlock + kBlock - 1) >> p.page_shift;
@@ -279,22 +280,12 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
                 __syncwarp();
             }
         });
-        if (p.status != nullptr) {
-            if (bad) atomicOr(p.status, PK100_STATUS_PAGE);
-            if (!ok && lane == 0) atomicOr(p.status, 1);
-        }
-        // copies still in flight where a wait ran out: they must land before the block's memory is given away
-        if (!ok || *abort_flag != 0) {
-            const uint64_t start = global_timer_ns();
-            for (int i = max(it - kStages, 0); i < it; ++i)
-                while (!mbar_try_wait(&sm.full[i % kStages], (i / kStages) & 1) && global_timer_ns() - start < 100000000ull) {}
-        }
+        if (bad && p.status != nullptr) atomicOr(p.status, PK100_STATUS_PAGE);
     } else {
         // ------------------------------------------------------------ products and softmax
         const int g = lane / 4, c = lane % 4;
         constexpr int kSteps = D / 16, kFeatureTiles = D / 32;          // k steps of Q.K; 8-feature tiles of a warp's quarter
         constexpr float kFactor = weight_factor<T>();                   // of P and so of the output, not of the sums
-        int it = 0;
         rows_walk(p, first_request, first_base, begin, end,
                   [&](const RowsShape& s, int request, int head, int tile, long long tile_first, int b0, int b1, bool whole) {
             const int rows = s.at.n * p.group - tile * kRows;           // rows of the tile that exist (or more)
@@ -326,7 +317,8 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
             const int from = max(s.block0 + b0, lo / kBlock), to = min(s.block0 + b1, (hi + kBlock - 1) / kBlock);
             for (int b = from; b < to; ++b, ++it) {
                 const int stage = it % kStages, buf = it & 1;
-                mbar_wait_bounded(&sm.full[stage], (it / kStages) & 1, abort_flag);
+                // (one that ran out does not end the loop: the other warps would wait at the barriers for ever)
+                ok &= mbar_look_within(&sm.full[stage], (it / kStages) & 1, abort_flag, p.wait_ns);
                 __syncwarp();
                 float sc[2][4] = {};
                 const int key_row = 16 * warp + ((lane >> 4) << 3) + (lane & 7);
@@ -489,6 +481,12 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
             }
         });
     }
+    // A wait that ran out, the loader's or a reader's, is reported, and its warp stays until the copies have landed: the block's
+    // memory is given away when all its warps have left.
+    if (__any_sync(0xffffffffu, !ok)) {
+        if (lane == 0 && p.status != nullptr) atomicOr(p.status, 1);
+        for (int i = max(it - kStages, 0); i < it; ++i) mbar_drain(&sm.full[i % kStages], (i / kStages) & 1);
+    }
     if (beside) grid_dependency_wait();
 }
 
@@ -616,6 +614,7 @@ extern "C" int pk100_paged_attention(void* stream_v, const pk100_paged_attention
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.few_rows = kRows;
     p.status = a->status;
+    p.wait_ns = pk100_wait_limit();
     // Where no request has more rows than the few-row kernel takes, it takes them all; the hint may be wrong, so it does then, too.
     const int most_new = a->max_new > 0 && a->max_new < a->tokens ? a->max_new : a->tokens;
     const bool many = static_cast<long long>(most_new) * p.group > kRows;

@@ -19,6 +19,7 @@ struct PagedParams {
     float scale_log2;                                  // scale * log2(e)
     int few_rows;                                      // requests of up to this many (token, head) rows belong to the few-row kernel
     int* status;
+    unsigned long long wait_ns;                        // limit of a wait
 };
 
 constexpr float kLn2 = 0.6931471805599453f;

@@ -32,7 +32,7 @@ struct Smem {
     uint8_t ring[ring_slots<D>()][D / 64][kAtom];          // key and value blocks in turn
     uint64_t full[ring_slots<D>()], empty[ring_slots<D>()];
     float top[kTiles][2][kTile];                           // row maxima of the halves; then sums
-    uint64_t q_ready[kTiles], s_full[kTiles], p_full[kTiles], o_done[kTiles];
+    uint64_t q_ready[kTiles], s_full[kTiles], p_full[kTiles], o_done[kTiles], drained;
     uint32_t tmem;
     int abort;
     unsigned shares, items;                                // of the step
@@ -226,7 +226,9 @@ __device__ __forceinline__ Place place_of(const Smem<D>& sm, const PagedParams& 
 }
 
 #define CHUNK_WAIT(bar, parity) \
-    if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&(bar), (parity), abort_flag)) != 0)) break
+    if (!(ok = __all_sync(0xffffffffu, mbar_wait_within(&(bar), (parity), abort_flag, p.wait_ns)) != 0)) break
+#define CHUNK_LOOK(bar, parity) \
+    if (!(ok = __all_sync(0xffffffffu, mbar_look_within(&(bar), (parity), abort_flag, p.wait_ns)) != 0)) break
 
 // The query heads of a key-value head are rows of one tile (row = token * group + head), so a chunk of few tokens fills
 // its tiles and keys are read once for all of them.  A tile of 128 rows has eight softmax warps (half a row a thread, the
@@ -266,6 +268,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
             mbar_init(&sm.p_full[t], kTileWarps);
             mbar_init(&sm.o_done[t], 1);
         }
+        mbar_init(&sm.drained, 1);
         fence_barrier_init();
         prefetch_tensormap(&map_k);
         prefetch_tensormap(&map_v);
@@ -320,10 +323,10 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         }
     };
     bool ok = true;
+    int it = 0;                                          // ring position of the role
     if (warp == kSoftmaxWarps) {
         // ------------------------------------------------------------ TMA
         const int box = min(kBox, 1 << p.page_shift), boxes = kTile / box;         // boxes: up to 8
-        int it = 0;
         bool bad = false;
         each_item([&](const Work<kTiles>& w, int request, int head, int) {
         const int* table = p.table + static_cast<long long>(request) * p.max_pages;
@@ -346,7 +349,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv, ++it) {
                 const int slot = it % kSlots;
-                CHUNK_WAIT(sm.empty[slot], (it / kSlots + 1) & 1);
+                CHUNK_LOOK(sm.empty[slot], (it / kSlots + 1) & 1);
                 if (lane == 0) mbar_arrive_expect_tx(&sm.full[slot], count * box * 128 * kHalves);
                 __syncwarp();
                 if (need) {
@@ -359,12 +362,6 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         }
         });
         if (bad && p.status != nullptr) atomicOr(p.status, PK100_STATUS_PAGE);
-        // copies still in flight where a wait ran out: they must land before the block's memory is given away
-        if (!ok || *abort_flag != 0) {
-            const uint64_t start = global_timer_ns();
-            for (int i = max(it - kSlots, 0); i < it; ++i)
-                while (!mbar_try_wait(&sm.full[i % kSlots], (i / kSlots) & 1) && global_timer_ns() - start < 100000000ull) {}
-        }
     } else if (warp == kSoftmaxWarps + 1) {
         // ------------------------------------------------------------ MMA
         constexpr uint32_t idesc_s = make_instr_desc<KIND_F16>(kTile, kTile) | type_bits<T>();
@@ -377,7 +374,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         const bool leader = elect_one();
         uint32_t phase[kTiles] = {};                         // parity of the tile's next block
         uint32_t q_phase[kTiles] = {};                       // of the tile's next item with blocks
-        int it = 0;                                          // ring position of the block's keys; its values follow
+        // (it: of the block's keys; its values follow)
         each_item([&](const Work<kTiles>& w, int, int, int) {
         if (!ok || w.from >= w.to) return;
         int tile_from[kTiles], tile_to[kTiles];
@@ -398,7 +395,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
                 if (ok && tile_from[t] < tile_to[t]) {
-                    CHUNK_WAIT(sm.q_ready[t], q_phase[t]);
+                    CHUNK_LOOK(sm.q_ready[t], q_phase[t]);
                     q_phase[t] ^= 1;
                 }
             if (!ok) break;
@@ -454,7 +451,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         } while (false);
         });
         // the last arrival of the tensor cores comes before the block leaves
-        if (ok && it > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sm.empty[(it - 1) % kSlots], ((it - 1) / kSlots) & 1, abort_flag)) != 0;
+        if (ok && it > 0) ok = __all_sync(0xffffffffu, mbar_wait_within(&sm.empty[(it - 1) % kSlots], ((it - 1) / kSlots) & 1, abort_flag, p.wait_ns)) != 0;
     } else {
         // ------------------------------------------------------------ softmax: half a row a thread
         const int t = warp / kTileWarps, half = (warp / 4) % 2, quad = warp % 4, tile_row = quad * 32 + lane;
@@ -512,7 +509,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         bool first = true;
         // (a wait that ran out does not end the loop: the other warp of the pair would wait at the barrier for ever)
         for (; b < stop; ++b, phase ^= 1, first = false) {
-            ok &= __all_sync(0xffffffffu, mbar_wait_bounded(&sm.s_full[t], phase, abort_flag)) != 0;
+            ok &= __all_sync(0xffffffffu, mbar_wait_within(&sm.s_full[t], phase, abort_flag, p.wait_ns)) != 0;
             tc_fence_after_sync();
             float s[64];
             tmem_ld_32x32(s_cols, reinterpret_cast<uint32_t(&)[32]>(s[0]));
@@ -546,7 +543,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 for (int i = 0; i < 64; ++i) s[i] -= off;
                 l = nan_if_huge(l) * factor;                 // (before the factor hides it)
                 if (!first) {
-                    ok &= __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], phase ^ 1, abort_flag)) != 0;
+                    ok &= __all_sync(0xffffffffu, mbar_wait_within(&sm.o_done[t], phase ^ 1, abort_flag, p.wait_ns)) != 0;
                     tc_fence_after_sync();
 #pragma unroll 1
                     for (int c = 0; c < D / 2; c += 16) {
@@ -575,7 +572,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
         l = nan_if_huge(l);
         if (!last) pair_sync();                              // (the next block's scores may be there already)
         if (ok && some) {
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sm.o_done[t], phase ^ 1, abort_flag)) != 0;
+            ok = __all_sync(0xffffffffu, mbar_wait_within(&sm.o_done[t], phase ^ 1, abort_flag, p.wait_ns)) != 0;
             tc_fence_after_sync();
         }
         if (ok && tile_rows > 0) {
@@ -666,6 +663,15 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
     if (!ok && lane == 0 && p.status != nullptr) atomicOr(p.status, 1);
     tc_fence_before_sync();
     __syncthreads();
+    // where a wait ran out, whoever's: copies and products must end before the block's memory is given away
+    if (*abort_flag != 0) {
+        if (warp == kSoftmaxWarps) {
+            for (int i = max(it - kSlots, 0); i < it; ++i) mbar_drain(&sm.full[i % kSlots], (i / kSlots) & 1);
+        } else if (warp == kSoftmaxWarps + 1) {
+            tc_commit_if(elect_one(), &sm.drained);           // (the same lane every time)
+            mbar_drain(&sm.drained, 0);
+        }
+    }
     if (warp == kSoftmaxWarps + 1) tmem_dealloc(tmem, kColumns);
 }
 

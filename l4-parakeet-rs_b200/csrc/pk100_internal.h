@@ -123,6 +123,9 @@ int pk100_gemm_chained(void* stream, const pk100_gemm_args* args, bool b_settled
 // SMs a launch may count on: all of them, or the cap set by pk100_set_gemm_cta_cap.
 int pk100_cta_budget();
 
+// Nanoseconds that a wait of a serving operator's kernel may take (pk100_set_wait_limit).
+unsigned long long pk100_wait_limit();
+
 // 2-D TMA descriptor of a row-major matrix [rows, cols] (`ld` elements between rows) with a box of
 // [box_rows, swizzle_bytes / elem_bytes] elements; served from the library's descriptor cache
 // (gemm_host.cu).  `map` points to a CUtensorMap.

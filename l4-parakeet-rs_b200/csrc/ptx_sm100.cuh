@@ -133,6 +133,51 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
     }
 }
 
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
+// The same with the host's limit (pk100_set_wait_limit).
+__device__ __forceinline__ bool mbar_wait_within(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t start = global_timer_ns();
+    uint32_t polls = 0;
+    while (true) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((++polls & 63u) == 0u || limit_ns == 0) {
+            if (*abort_flag != 0) return false;
+            if (global_timer_ns() - start >= limit_ns) {
+                *abort_flag = 1;
+                return false;
+            }
+        }
+    }
+}
+
+// The same; a limit of 0 gives up where the first look, which does not sleep, finds the phase incomplete.
+__device__ __forceinline__ bool mbar_look_within(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns) {
+    if (limit_ns != 0) return mbar_wait_within(bar, parity, abort_flag, limit_ns);
+    if (mbar_test_wait(bar, parity)) return true;
+    *abort_flag = 1;
+    return false;
+}
+
+// Where a block gave up: waits (0.1 s at most) for a phase of something still in flight, which must not end behind the block.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+    const uint64_t start = global_timer_ns();
+    while (!mbar_try_wait(bar, parity) && global_timer_ns() - start < 100000000ull) {}
+}
+
 // --------------------------------------------------------------------- TMA
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");

@@ -131,6 +131,7 @@ SIGNATURES = {
     "pk100_paged_plan": [vp, C.POINTER(PagedPlanArgs)],
     "pk100_paged_attention": [vp, C.POINTER(PagedAttentionArgs)],
     "pk100_paged_attention_workspace_bytes": [C.POINTER(PagedAttentionArgs)],
+    "pk100_set_wait_limit": [i64],
 }
 
 for _name, _argtypes in SIGNATURES.items():
