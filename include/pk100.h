@@ -670,7 +670,7 @@ int pk100_add_rms_norm(void* stream, const pk100_rms_norm_args* args);
  * weights' bytes and pk100_gemm's tiles are mostly padding: the same arguments, weights W = f16(code * scale) and
  * epilogue algebra, fp32 sums (in another order than pk100_gemm's).  Any n; k % 128 == 0; a and b 16-byte
  * aligned, lda % 8 == 0; out and residual of any leading dimension; PK100_EPI_LINEAR; out_type PK100_OUT_F16 or
- * _F32.  More than 16 rows: PK100_ERR_LIMIT.  A row's bits depend on its own values, n and k alone.  tau, keep_*,
+ * _F32.  More than 16 rows or 2^30 columns: PK100_ERR_LIMIT.  A row's bits depend on its own values, n and k alone.  tau, keep_*,
  * stats_out and max_ctas are not read. */
 int pk100_gemv_w4g128(void* stream, const pk100_gemm_args* args);
 

@@ -57,7 +57,7 @@ gemv_w4g128_kernel(const GemvParams p) {
     const int last = static_cast<int>(static_cast<long long>(all) * (blockIdx.x + 1) / gridDim.x);
     // chunks of nearly equal size
     const int chunks = (last - first + kGemvTiles - 1) / kGemvTiles;
-    auto chunk_at = [&](int chunk) { return first + (last - first) * chunk / chunks; };
+    auto chunk_at = [&](int chunk) { return first + static_cast<int>(static_cast<long long>(last - first) * chunk / chunks); };
     grid_dependents_launch();
     grid_dependency_wait();
 
@@ -212,7 +212,7 @@ extern "C" int pk100_gemv_w4g128(void* stream_v, const pk100_gemm_args* a) {
     if (a->act < PK100_ACT_NONE || a->act > PK100_ACT_RELU) return PK100_ERR_UNSUPPORTED;
     if (a->out_type != PK100_OUT_F16 && a->out_type != PK100_OUT_F32) return PK100_ERR_UNSUPPORTED;
     if (a->m < 0 || a->n <= 0 || a->k <= 0 || a->k % kGroup != 0) return PK100_ERR_SHAPE;
-    if (a->m > 16) return PK100_ERR_LIMIT;
+    if (a->m > 16 || a->n > 1 << 30) return PK100_ERR_LIMIT;             // (rows of weights are counted in 32 bits, whole tiles of them)
     if (a->m == 0) return PK100_OK;
     if (a->a == nullptr || a->b == nullptr || a->out == nullptr || a->b_group_scales == nullptr) return PK100_ERR_NULL;
     // (a single row has no distance)

@@ -259,3 +259,27 @@ def test_attention_lse_of_a_row_that_one_key_dominates(pk, cuda, dim, dtype):
         half = 2.0 ** -11 if dtype is F16 else 2.0 ** -8
         bound = (half + 1e-5) * (flat_v[0].abs() + 2.0 ** large * picked.abs()) / total + half * want.abs() + 1e-6
         assert bool(((out.double() - want).abs() <= bound).all())
+
+
+# ------------------------------------------------------------- few-row products
+def test_gemv_of_more_columns_than_a_block_counts_in_32_bits(pk, cuda):
+    """One block takes 1.5 M columns (12 GB of codes): its tiles times its chunks pass 2^31.  The bits are those of all blocks."""
+    n, k = 1500000, 16512
+    codes = torch.empty(n, k // 2, dtype=torch.uint8, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for part in codes.split(100000):
+        part.copy_(torch.randint(0, 256, part.shape, generator=gen, device="cuda", dtype=torch.uint8))
+    scales = (torch.rand(k // 128, n, generator=gen, device="cuda") * 0.02 + 1e-4).half()
+    x = torch.randn(2, k, generator=gen, device="cuda").half()
+    want = pk.ops.gemv_w4g128(x, codes, scales, out_type=pk.lib.OUT_F32)
+    out = torch.full_like(want, 7.0)
+    try:
+        pk.lib.lib.pk100_set_gemm_cta_cap(1)
+        pk.ops.gemv_w4g128(x, codes, scales, out=out, out_type=pk.lib.OUT_F32)
+    finally:
+        pk.lib.lib.pk100_set_gemm_cta_cap(0)
+    assert torch.equal(out, want)
+    rows = torch.tensor([0, 1, 63, 64, 749999, 1372096, 1372097, 1499999], device="cuda")
+    w = R.w4_weights(codes[rows], scales[:, rows])
+    ref = x.double() @ w.t()
+    assert bool(((out[:, rows].double() - ref).abs() <= R.gemv_tolerance(x, w, ref, torch.float32)).all())
