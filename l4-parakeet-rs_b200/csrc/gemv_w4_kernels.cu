@@ -55,9 +55,9 @@ gemv_w4g128_kernel(const GemvParams p) {
     const int groups = p.k / kGroup, all = (p.n + 15) / 16;
     const int first = static_cast<int>(static_cast<long long>(all) * blockIdx.x / gridDim.x);
     const int last = static_cast<int>(static_cast<long long>(all) * (blockIdx.x + 1) / gridDim.x);
-    // chunks of nearly equal size
-    const int chunks = (last - first + kGemvTiles - 1) / kGemvTiles;
-    auto chunk_at = [&](int chunk) { return first + static_cast<int>(static_cast<long long>(last - first) * chunk / chunks); };
+    // chunks of nearly equal size, the larger ones first
+    const int chunks = (last - first + kGemvTiles - 1) / kGemvTiles, each = (last - first) / chunks, larger = last - first - each * chunks;
+    auto chunk_at = [&](int chunk) { return first + chunk * each + min(chunk, larger); };
     grid_dependents_launch();
     grid_dependency_wait();
 
