@@ -110,18 +110,19 @@ gemv_w4g128_kernel(const GemvParams p) {
         for (int i = 0; i < 2 * kGemvTiles; ++i) scale_next[i] = __half();
         const __half* x_src = p.a + g * p.lda + warp * kGroup + 32 * c;
         const __half* scale_src = p.group_scales + static_cast<long long>(warp) * p.n + at * 16 + g;
-        auto request = [&](int group) {                                // activations and scales, a group ahead
+        // activations and scales, a group ahead (plain loads: the kernel in front may still be writing them when this one starts)
+        auto request = [&](int group) {
             if (group >= groups) return;
 #pragma unroll
             for (int j = 0; j < RowTiles; ++j)
                 if (8 * j + g < p.m) {
                     const uint4* src = reinterpret_cast<const uint4*>(x_src + 8 * j * p.lda);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x_next[j][i] = __ldg(src + i);
+                    for (int i = 0; i < 4; ++i) x_next[j][i] = src[i];
                 }
 #pragma unroll
             for (int i = 0; i < 2 * kGemvTiles; ++i)
-                if (8 * i < limit) scale_next[i] = __ldg(scale_src + 8 * i);
+                if (8 * i < limit) scale_next[i] = scale_src[8 * i];
             x_src += kGemvWarps * kGroup;
             scale_src += static_cast<long long>(kGemvWarps) * p.n;
         };

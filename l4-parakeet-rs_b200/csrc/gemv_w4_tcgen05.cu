@@ -136,7 +136,7 @@ gemv_w4g128_wide_kernel(const __grid_constant__ CUtensorMap map_codes, const Gem
             auto settle = [&] { while (group >= count && t < tiles) { group -= count; ++t; } };
             auto scale_of = [&] {
                 const int n = (first + t) * kTile + static_cast<int>(row);
-                return t < tiles && n < p.n && g0 + group < groups ? __ldg(p.group_scales + static_cast<long long>(g0 + group) * p.n + n) : __half();
+                return t < tiles && n < p.n && g0 + group < groups ? p.group_scales[static_cast<long long>(g0 + group) * p.n + n] : __half();
             };
             if (count > 0) settle();
             __half scale = scale_of();

@@ -678,7 +678,7 @@ paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __
 // out of the shares of a row's keys, in their order, a warp a row.
 template <typename T, int D>
 __global__ void __launch_bounds__(128)
-shares_join_kernel(const PagedParams p, const int* share_count, const float2* __restrict__ part_ml, const float* __restrict__ part_out) {
+shares_join_kernel(const PagedParams p, const int* share_count, const float2* part_ml, const float* part_out) {
     grid_dependents_launch();
     grid_dependency_wait();
     const int shares = *share_count;
