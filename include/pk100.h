@@ -707,7 +707,8 @@ int pk100_paged_plan(void* stream, const pk100_paged_plan_args* args);
  * token stands at position p = lengths[r] - new + i:
  *   out = softmax_j(scale * q . k_j) . v_j over the positions j < lengths[r], j <= p when causal, j > p - window when
  *   window > 0;  lse (fp32 [tokens, heads], may be NULL) = log sum_j exp(scale * q . k_j), to 1e-5 beside the rounding of the
- *   fp32 scores.
+ *   fp32 scores.  Weights of the softmax are multiplied in the type of the caches: requests of few (token, head) rows with
+ *   what that rounding left, others without.
  * A row that sees nothing gets zeros and lse -infinity.  Rows behind starts[requests] are not touched.
  * Query head h reads key-value head h / (heads / kv_heads).  head_dim 64 or 128; page_size 16, 32, 64, 128 or 256.
  * Element (page, token, head, d) of both caches is at page * page_stride + token * token_stride + head * head_stride

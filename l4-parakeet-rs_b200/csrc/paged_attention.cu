@@ -56,7 +56,7 @@ template <int D>
 struct RowsSmem {
     uint8_t k[rows_stages<D>()][D / 64][kBlock * 128];
     uint8_t v[rows_stages<D>()][D / 64][kBlock * 128];
-    uint8_t p[2][kRows * 128];
+    uint8_t p[2][2][kRows * 128];              // weights and what their rounding left
     float top[2][kRowWarps][kRows];
     float sum[kRowWarps][kRows];
     long long scan[kRowThreads / 32];
@@ -173,9 +173,10 @@ __device__ __forceinline__ void join_row(const PagedParams& p, const PagedReques
 // keys and values are read once for all of them.
 // A warp requests 64-key stages by TMA (a page or part of one a box, 128-byte swizzle), two blocks an SM keep up to
 // six of them in flight.  Q.K: each of four warps 16 keys; the row maxima are exchanged, so that all warps scale
-// alike; P in 16 bits through shared memory; P.V: each warp a quarter of the features.
-// Scores, maxima, sums and outputs are fp32; P is rounded to the type of V for the tensor cores, which costs what
-// the rounding of the output costs (the sum l is that of the unrounded P).  The tensor cores cut off what falls below the last
+// alike; P through shared memory; P.V: each warp a quarter of the features.
+// Scores, maxima, sums and outputs are fp32; P goes to the tensor cores in two numbers of the type of V, the rounded weight and
+// the rounded rest: one alone had cost what the rounding of the output costs, two cost 2 us of 128, as long as the cache's bytes
+// decide.  The tensor cores cut off what falls below the last
 // bit of the sum that they add to: a block's products begin at zero and are added to the row's by the FMA pipe, which rounds.
 // (One sum over 2^19 keys was 4e-3 low.)  l is compensated: many small weights behind a large one are not lost in it.
 // One token of 48 requests over 320 to 12 000 keys, 32 / 8 heads of 128 (712 MB): 118 us, 6.0 TB/s.
@@ -376,8 +377,15 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
                     b0 += x0 + x1;
                     b1 += y0 + y1;
                     const int chunk = 2 * warp + nt;
-                    *reinterpret_cast<uint32_t*>(&sm.p[buf][g * 128 + ((chunk ^ g) << 4) + 4 * c]) = packed_of(x0 * kFactor, x1 * kFactor, T());
-                    *reinterpret_cast<uint32_t*>(&sm.p[buf][(g + 8) * 128 + ((chunk ^ g) << 4) + 4 * c]) = packed_of(y0 * kFactor, y1 * kFactor, T());
+                    auto put = [&](float u, float v, int row) {
+                        const uint32_t near = packed_of(u, v, T());
+                        const float2 r = floats_of(near, T());
+                        const int at = row * 128 + ((chunk ^ g) << 4) + 4 * c;
+                        *reinterpret_cast<uint32_t*>(&sm.p[buf][0][at]) = near;
+                        *reinterpret_cast<uint32_t*>(&sm.p[buf][1][at]) = packed_of(u - r.x, v - r.y, T());
+                    };
+                    put(x0 * kFactor, x1 * kFactor, g);
+                    put(y0 * kFactor, y1 * kFactor, g + 8);
                 }
                 add_compensated(l0, e0, a0, b0);
                 add_compensated(l1, e1, a1, b1);
@@ -387,8 +395,10 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
                 const int p_row = (((lane >> 3) & 1) << 3) + (lane & 7);
 #pragma unroll
                 for (int ks = 0; ks < kBlock / 16; ++ks) {
-                    uint32_t pf[4];
-                    ldmatrix_x4(pf, smem_u32(sm.p[buf]) + p_row * 128 + (((ks * 2 + (lane >> 4)) ^ (p_row & 7)) << 4));
+                    uint32_t pf[4], rest[4];
+                    const uint32_t p_at = smem_u32(sm.p[buf][0]) + p_row * 128 + (((ks * 2 + (lane >> 4)) ^ (p_row & 7)) << 4);
+                    ldmatrix_x4(pf, p_at);
+                    ldmatrix_x4(rest, p_at + kRows * 128);
                     const int v_row = ks * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
 #pragma unroll
                     for (int j = 0; j < kFeatureTiles / 2; ++j) {
@@ -406,6 +416,8 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
                         }
                         mma_rows(pv[2 * j], pf, vf[0], vf[1], T());
                         mma_rows(pv[2 * j + 1], pf, vf[2], vf[3], T());
+                        mma_rows(pv[2 * j], rest, vf[0], vf[1], T());
+                        mma_rows(pv[2 * j + 1], rest, vf[2], vf[3], T());
                     }
                 }
 #pragma unroll

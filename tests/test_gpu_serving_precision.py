@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from tests import serving_reference as R
+from tests.test_gpu_serving import Step
 
 pytestmark = pytest.mark.gpu
 
@@ -259,6 +260,23 @@ def test_attention_lse_of_a_row_that_one_key_dominates(pk, cuda, dim, dtype):
         half = 2.0 ** -11 if dtype is F16 else 2.0 ** -8
         bound = (half + 1e-5) * (flat_v[0].abs() + 2.0 ** large * picked.abs()) / total + half * want.abs() + 1e-6
         assert bool(((out.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 8, 128), (16, 2, 64), (20, 4, 128)])
+def test_attention_of_single_tokens_rounds_no_weight(pk, cuda, heads, kv, dim, dtype):
+    """Where values cancel, a rounding of the weights would show beside the small output: there is none but the output's.  The
+    weights' second numbers leave a half step of a half step."""
+    s = Step([1] * 8, [0, 1, 20, 63, 64, 500, 3000, 9000], heads, kv, dim, 32, dtype, seed=11)
+    s.q.mul_(0.2)
+    out, at, half = s.run(pk, max_new=1), 0, R.HALF[dtype]
+    for r, (n, c) in enumerate(zip(s.new, s.cached)):
+        k, v = (R.paged(cache, s.table[r], c + n) for cache in (s.k_cache, s.v_cache))
+        want, _, spread, off = R.attention(s.q[at:at + n], k, v, torch.arange(c, c + n, device="cuda"), True, 0, dim ** -0.5)
+        score = 24 * 2.0 ** -22 * off + 1e-6                           # of an exponent: see attention_tolerance
+        bound = half * want.abs() + (half * half + 2 * score) * spread + R.TINY[dtype]
+        assert bool(((out[at:at + n].double() - want).abs() <= bound).all()), r
+        at += n
 
 
 # ------------------------------------------------------------- few-row products
