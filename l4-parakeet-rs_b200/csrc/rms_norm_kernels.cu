@@ -31,12 +31,44 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int column, int width,
         if (column + i < width) row[column + i] = static_cast<uint8_t>((i < 4 ? v.x : v.y) >> (8 * (i % 4)));
 }
 
-// y / c rounded once, from the rounded reciprocal: the product is two roundings off, its remainder, which the multiply-add has
-// exactly, takes them back (P. Markstein, IBM J. Res. Dev. 34, 1990).  The product alone moved codes of values half-way
-// between two.  For finite y and quotients whose way stays among the normal numbers.
-__device__ __forceinline__ float quotient(float y, float c, float inverse) {
-    const float q = y * inverse;
-    return fmaf(fmaf(-q, c, y), inverse, q);
+// y / c = s * gamma * (limit / max |s * gamma|): the root cancels, the product of two 16-bit numbers is exact in fp32, and the
+// row's factor comes in two numbers, high + low.  One rounding is left of the quotient; five, with y and c rounded in between,
+// moved codes of values half-way between two.
+__device__ __forceinline__ float quotient(float product, float high, float low) { return fmaf(product, high, product * low); }
+
+__device__ __forceinline__ float widest_or_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(fabsf(b)));
+    return d;
+}
+
+// The nearest integers (ties to even) of limit * product / top as bytes, 0 of NaN.  Where a rounded quotient is half-way, which
+// side the exact one lies on is decided in 64 bits.
+__device__ __forceinline__ uint2 nearest_bytes(const float (&product)[8], float high, float low, float top, float limit) {
+    constexpr float kMagic = 12582912.0f;               // 1.5 * 2^23: a quotient is 127 at most
+    float n[8], off = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float q = quotient(product[i], high, low);
+        n[i] = q + kMagic;
+        off = widest_or_nan(off, q - (n[i] - kMagic));
+    }
+    if (!(off < 0.5f)) {                                // (one of a million)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float q = quotient(product[i], high, low);
+            if (fabsf(q - (n[i] - kMagic)) < 0.5f) continue;
+            const double beyond = static_cast<double>(limit) * product[i] - static_cast<double>(q) * top;
+            if (beyond != 0.0) n[i] = (q + (beyond > 0.0 ? 0.5f : -0.5f)) + kMagic;
+            if (q != q) n[i] = kMagic;
+        }
+    }
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        w[i] = __byte_perm(__byte_perm(__float_as_uint(n[4 * i]), __float_as_uint(n[4 * i + 1]), 0x0040),
+                           __byte_perm(__float_as_uint(n[4 * i + 2]), __float_as_uint(n[4 * i + 3]), 0x0040), 0x5410);
+    return make_uint2(w[0], w[1]);
 }
 
 // A row belongs to a warp (8 rows a block) or to a whole block; every thread keeps Chunks x 8 of its elements, so
@@ -141,60 +173,77 @@ add_rms_norm_kernel(const RmsNormParams p) {
         if (p.threads > 32) __syncthreads();            // (the parts have been read)
         reduce();                                       // (the sum has done its work)
     }
-    float scale = 1.0f, inverse = p.inv_scale;
-    bool by_reciprocal = false;                         // the row's quotients: nothing on their way leaves the normal numbers
+    constexpr float kLimit = Mode == PK100_LN_E4M3_ROW ? 448.0f : 127.0f;
+    float scale = 1.0f, high = 0.0f, low = 0.0f;
+    bool by_products = false;                           // the row's codes: all of it is numbers, within range
     if constexpr (kRowScale) {
         const float peak = top * rstd;
-        if (peak > 0.0f && peak < INFINITY) scale = __fdiv_rn(peak, Mode == PK100_LN_E4M3_ROW ? 448.0f : 127.0f);
-        inverse = __frcp_rn(scale);
-        by_reciprocal = finite && scale > 1e-18f && scale < 1e18f;
+        if (peak > 0.0f && peak < INFINITY) {
+            scale = __fdiv_rn(peak, kLimit);
+            by_products = finite && top > 1e-30f && top < 1e30f;
+        }
+        high = __fdiv_rn(kLimit, top);
+        low = __fdiv_rn(fmaf(-high, top, kLimit), top);
         if (t == 0) p.scales[row] = scale;
     }
-    auto write = [&](auto by_product) {
+    auto write = [&](auto products) {
 #pragma unroll
         for (int c = 0; c < Chunks; ++c) {
             const int column = (c * p.threads + t) * 8;
             const uint32_t* a = reinterpret_cast<const uint32_t*>(&s[c]);
             const uint4 g = load8(gamma, column, p.width, p.vec_gamma);        // (again, from the L1: registers are blocks in flight)
             const uint32_t* b = reinterpret_cast<const uint32_t*>(&g);
-            float y[8];
+            float y[8];                                  // or s * gamma
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float2 x = floats_of(a[i], T()), w = floats_of(b[i], T());
-                y[2 * i] = x.x * rstd * w.x;
-                y[2 * i + 1] = x.y * rstd * w.y;
+                y[2 * i] = decltype(products)::value ? x.x * w.x : x.x * rstd * w.x;
+                y[2 * i + 1] = decltype(products)::value ? x.y * w.y : x.y * rstd * w.y;
             }
             if constexpr (Mode == PK100_LN_F16) {
                 T* o = static_cast<T*>(p.output) + row * p.ld_out;
                 store8(o, column, p.width, p.vec_out, make_uint4(packed_of(y[0], y[1], T()), packed_of(y[2], y[3], T()),
                                                                  packed_of(y[4], y[5], T()), packed_of(y[6], y[7], T())));
             } else {
-                uint32_t w[2] = {0, 0};
+                uint2 codes;
+                if constexpr (Mode == PK100_LN_S8_ROW && decltype(products)::value) {
+                    codes = nearest_bytes(y, high, low, top, kLimit);
+                } else {
+                    uint32_t w[2] = {0, 0};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float lo, hi;
-                    if constexpr (!kRowScale) {
-                        lo = y[2 * i] * inverse;
-                        hi = y[2 * i + 1] * inverse;
-                    } else {
-                        lo = decltype(by_product)::value ? quotient(y[2 * i], scale, inverse) : y[2 * i] / scale;
-                        hi = decltype(by_product)::value ? quotient(y[2 * i + 1], scale, inverse) : y[2 * i + 1] / scale;
+                    for (int i = 0; i < 8; i += 2) {
+                        float lo, hi;
+                        if constexpr (decltype(products)::value) {
+                            lo = quotient(y[i], high, low);
+                            hi = quotient(y[i + 1], high, low);
+                        } else if constexpr (kRowScale) {
+                            lo = y[i] / scale;
+                            hi = y[i + 1] / scale;
+                        } else {
+                            lo = y[i] * p.inv_scale;
+                            hi = y[i + 1] * p.inv_scale;
+                        }
+                        uint32_t pair;
+                        if constexpr (Mode == PK100_LN_S8_ROW) {
+                            const int u = max(-127, min(127, __float2int_rn(lo))), v = max(-127, min(127, __float2int_rn(hi)));
+                            pair = static_cast<uint32_t>((u & 255) | ((v & 255) << 8));
+                        } else {
+                            pair = __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+                        }
+                        w[i / 4] |= pair << (8 * (i % 4));
                     }
-                    if constexpr (Mode == PK100_LN_S8_ROW) {
-                        const int u = max(-127, min(127, __float2int_rn(lo))), v = max(-127, min(127, __float2int_rn(hi)));
-                        w[i / 2] |= static_cast<uint32_t>((u & 255) | ((v & 255) << 8)) << (16 * (i % 2));
-                    } else {
-                        w[i / 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3))
-                                    << (16 * (i % 2));
-                    }
+                    codes = make_uint2(w[0], w[1]);
                 }
-                store_codes(static_cast<uint8_t*>(p.output) + row * p.ld_out, column, p.width, p.vec_out, make_uint2(w[0], w[1]));
+                store_codes(static_cast<uint8_t*>(p.output) + row * p.ld_out, column, p.width, p.vec_out, codes);
             }
         }
     };
-    // (a branch a row)
-    if (by_reciprocal) write(std::true_type());
-    else write(std::false_type());
+    if constexpr (kRowScale) {                          // (a branch a row)
+        if (by_products) write(std::true_type());
+        else write(std::false_type());
+    } else {
+        write(std::false_type());
+    }
 }
 
 template <typename T, int Mode>

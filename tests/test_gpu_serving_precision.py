@@ -21,10 +21,12 @@ def _values_below(peak, dtype):
     return v[(v.float() > 0.05) & (v.float() <= peak)]
 
 
-@pytest.mark.parametrize("mode,dtype,peak", [("e4m3", F16, 56.5), ("int8", F16, 14.8828125), ("e4m3", BF16, 24.5), ("int8", BF16, 53.75)])
+@pytest.mark.parametrize("mode,dtype,peak", [("e4m3", F16, 56.5), ("int8", F16, 14.8828125), ("e4m3", BF16, 24.5), ("int8", BF16, 53.75),
+                                             ("int8", F16, 63.5), ("int8", BF16, 63.5), ("e4m3", F16, 56.0)])
 def test_norm_codes_are_those_of_the_quotient(pk, cuda, mode, dtype, peak):
-    """Rows of +1 and -1 have a mean square of 1, so y = s * gamma exactly, and the code is that of y / c, c = max |y| / top in
-    fp32: one rounding.  A product with the rounded reciprocal has two, and gives other codes for some of these y."""
+    """Rows of +1 and -1 have a mean square of 1, so y = s * gamma exactly, and y / c = y * top / max |y|: the code is the nearest of
+    that, ties to even.  A product with the rounded reciprocal of c gives other codes for some of the first four rows' values.  In
+    64 bits the quotient of these numbers is half-way where the exact one is, and only there; E4M3 codes are those of its fp32 value."""
     L = pk.lib
     gamma = _values_below(peak, dtype)
     width, top = gamma.numel(), 448.0 if mode == "e4m3" else 127.0
@@ -32,14 +34,37 @@ def test_norm_codes_are_those_of_the_quotient(pk, cuda, mode, dtype, peak):
     x[1] = -1
     x[2, ::2] = -1
     out, scales, _ = pk.ops.add_rms_norm(x.cuda(), gamma.cuda(), mode=L.LN_E4M3_ROW if mode == "e4m3" else L.LN_S8_ROW, eps=0.0)
-    y = x.float().numpy() * gamma.float().numpy()
+    y = x.double().numpy() * gamma.double().numpy()
     c = np.float32(peak) / np.float32(top)
-    quotient, product = y / c, y * (np.float32(1) / c)
-    code = lambda q: torch.from_numpy(np.rint(q) if mode == "int8" else q).to(torch.int8 if mode == "int8" else torch.float8_e4m3fn).float()
-    assert not torch.equal(code(quotient), code(product))
+    product = y.astype(np.float32) * (np.float32(1) / c)
+    code = lambda q: torch.from_numpy(np.rint(q) if mode == "int8" else q.astype(np.float32)).to(torch.int8 if mode == "int8" else torch.float8_e4m3fn).float()
+    want = code(y * top / peak)
+    assert peak in (56.0, 63.5) or not torch.equal(want, code(product))
     assert (scales.cpu() == torch.from_numpy(np.array(c))).all()
     got = (out if mode == "int8" else out.view(torch.float8_e4m3fn)).float().cpu()
-    assert torch.equal(got, code(quotient))
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,width", [(777, 2560), (2000, 4096), (40, 96)])
+def test_norm_int8_codes_are_the_nearest(pk, cuda, dtype, rows, width):
+    """Rows as a model has them: every code is the nearest integer of limit * s * gamma / max |s * gamma|, which 64 bits hold."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    x, r = (torch.randn(rows, width, generator=gen, device="cuda").to(dtype) for _ in range(2))
+    gamma = (torch.randn(width, generator=gen, device="cuda") * 0.1 + 1.0).to(dtype)
+    out, _, s = pk.ops.add_rms_norm(x, gamma, residual=r, mode=pk.lib.LN_S8_ROW)
+    y = s.double() * gamma.double()
+    assert torch.equal(out.double(), torch.round(y * 127.0 / y.abs().amax(1, keepdim=True)))
+
+
+def test_norm_int8_codes_beside_a_gamma_that_is_none(pk, cuda):
+    x = torch.randn(5, 300, generator=torch.Generator().manual_seed(1)).half().cuda()
+    gamma = torch.ones(300, dtype=F16, device="cuda")
+    want, want_scales, _ = pk.ops.add_rms_norm(x[:, :299].contiguous(), gamma[:299], mode=pk.lib.LN_S8_ROW)
+    gamma[299] = math.nan
+    x[:, 299] = 0.5
+    out, scales, _ = pk.ops.add_rms_norm(x, gamma, mode=pk.lib.LN_S8_ROW)
+    assert bool((out[:, 299] == 0).all()) and torch.equal(out[:, :299], want)
 
 
 @pytest.mark.parametrize("width", [40, 256, 4096, 20000])
