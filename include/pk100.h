@@ -746,7 +746,9 @@ typedef struct pk100_paged_attention_args {
     int* status;                                  /* may be NULL */
 } pk100_paged_attention_args;
 
-/* Depends on tokens, requests, heads, kv_heads, head_dim and max_pages * page_size alone; 0 where the arguments are refused. */
+/* Depends on tokens, requests, heads, kv_heads, head_dim, max_pages * page_size and the number of SMs of the current device; 0 where the
+ * arguments are refused.  Where max_pages hold more than 8192 keys it has room for an fp32 copy of out: sums over more keys than the
+ * tensor cores can add up without loss are kept there. */
 long long pk100_paged_attention_workspace_bytes(const pk100_paged_attention_args* args);
 int pk100_paged_attention(void* stream, const pk100_paged_attention_args* args);
 

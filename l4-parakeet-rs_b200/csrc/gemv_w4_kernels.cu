@@ -42,7 +42,7 @@ struct GemvSmem {
 // come by asynchronous copies, up to 96 KB of them in flight, into a ring in which every thread reads what it has
 // copied itself: no barrier in the loop, and the next chunk is on its way while this one is joined.  Activations and
 // scales of the next group are requested a group ahead.
-// One row by 8192 x 4096 (17 MB): 6.8 us; 1024 x 4096: 3.9 us.  Bound by the conversion and by mma.sync, whose ten issue
+// One row by 8192 x 4096 (17 MB): 6.8 us; 1024 x 4096: 4.0 us.  Bound by the conversion and by mma.sync, whose ten issue
 // cycles nothing else fills; small products by their chain of load, conversion and join.
 template <int RowTiles>
 __global__ void __launch_bounds__(kGemvThreads, 1)
@@ -235,8 +235,9 @@ extern "C" int pk100_gemv_w4g128(void* stream_v, const pk100_gemm_args* a) {
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
     p.status = a->status;
     p.wait_ns = pk100_wait_limit();
-    // From 16 384 weight rows on (three and a half tiles a cluster) the wide kernel: 13 rows by 28 672 x 8192 in 36 us against 50, x 1024
-    // in 10.7 against 14.9; one row about the same; 8192 x 4096 9.7 against 9.4, 4096 x 14 336 17.5 against 15.0.
+    // From 16 384 weight rows on (almost four tiles a cluster) the wide kernel: 13 rows by 28 672 x 8192 in 36 us against 50, x 1024
+    // in 11.2 against 15.0, 16 384 x 4096 in 15.2 against 18.0; one row by 28 672 x 8192 in 33.5 against 36.4.  Below, one row by 8192 x 4096 takes
+    // 9.3 us there against 6.8 here, 13 rows 9.8 against 9.4 (4096 x 14 336 14.5 against 15.2, 12 288 x 4096 12.1 against 15.6).
     if (a->n >= kWideRows && a->k <= gemv_wide_limit()) {
         const int rc = launch_gemv_wide(p, stream);
         if (rc != PK100_ERR_UNSUPPORTED) return rc;                    // (the device holds no such cluster)

@@ -135,7 +135,9 @@ struct Work {
 // The step's pairs of tiles (pairs of one tile where D is 64) and where to find one.
 // Up to 32 requests: one warp orders them, the longest first, into shared memory; a request's last pairs, which see the most
 // keys, come first.  Up to 256: counted from the requests, in their order.  More: numbered over the batch with gaps, request r
-// from floor(first row / rows of a pair) + r on, which leaves room for its last, partial one.
+// from floor(first row / rows of a pair) + r on, which leaves room for its last, partial one.  Counting: 256 requests of 10 to 60 tokens
+// 110 us against 125 with numbers, 200 101 against 107, 100 56.6 against 57.7; numbers: 500 197 against 210, 1000 368 against 459, 300 the same.
+// (A warp orders as many as it has lanes; what ordering brings stands at the kernel, what the pass over the items costs few requests at its launch.)
 constexpr int kOrdered = 32, kCounted = 256;
 
 template <int kTiles>
@@ -243,9 +245,9 @@ __device__ __forceinline__ Place place_of(const Smem<D>& sm, const PagedParams& 
 // output costs (the sum l is that of the unrounded P): bf16 outputs are 2.3e-3 off instead of 1.7e-3, fp16 2.5e-4 instead of 2.0e-4,
 // relative to their norm.  The rest of the rounding in a second product, as in the few-row kernel, took two prompts from 440 to 556 us.
 // Bound by a tile's chain of scores, softmax and products: 3200 cycles per 128 keys of both tiles, of which the MMAs are
-// 2300.  Two prompts of 7.2 k tokens, 16 / 4 heads of 128: 423 to 433 us, 1 PFLOP/s (the few-row kernel in the same place: 4.6 ms);
-// 512 tokens over 32 000, 16 / 2 heads: 140 to 145 us, 0.95 PFLOP/s (764 us).  Nine chunks of 5 to 561 tokens, 16 heads of 64,
-// window 1024: 27 us, the latency of the longest block (32.8 with the requests in their own order).
+// 2300.  Two prompts of 7.2 k tokens, 16 / 4 heads of 128: 423 to 437 us, 1 PFLOP/s (the few-row kernel in the same place: 4.6 ms);
+// 512 tokens over 32 000, 16 / 2 heads: 138 to 146 us, 0.95 PFLOP/s (764 us); 4096 over 32 000 981 us (967 with one sum of all keys).  Nine
+// chunks of 5 to 561 tokens, 16 heads of 64, window 1024: 26.6 us, the latency of the longest block (6 us more in their own order).
 template <typename T, int D, bool kLoop>
 __global__ void __launch_bounds__(threads<D>(), 3 - tiles<D>())
 paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PagedParams p,
@@ -729,7 +731,8 @@ static int launch(const PagedParams& p, const CUtensorMap& map_k, const CUtensor
     static_assert(bytes <= 227 * 1024 / (3 - tiles<D>()) - (D == 64 ? 1024 : 0), "shared memory");
     const long long slots = pk100_sm_count() * (3 - tiles<D>()), columns = static_cast<long long>(pairs) * p.kv_heads;
     // Up to 32 requests at most 32 pairs a head do not exist: a block for each that may.  With more, blocks that find nothing to
-    // do would cost more than the pass over the items (200 single tokens whose max_new is not known: 207 against 167 us).
+    // do would cost more than the pass over the items (200 single tokens whose max_new is not known: 207 against 167 us; the pass
+    // over the items costs few requests 11 us of two prompts and 3 of nine ragged chunks).
     auto run = [&](auto loop) -> int {
         constexpr auto kernel = paged_attention_chunk_kernel<T, D, decltype(loop)::value>;
         const cudaError_t granted = pk100_grant_smem<kernel>(bytes);

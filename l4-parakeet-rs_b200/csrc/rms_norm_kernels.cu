@@ -74,7 +74,7 @@ __device__ __forceinline__ uint2 nearest_bytes(const float (&product)[8], float 
 // A row belongs to a warp (8 rows a block) or to a whole block; every thread keeps Chunks x 8 of its elements, so
 // the row is read once.  Mean square and max |s * gamma| leave in ONE reduction: max |y| = rstd * max |s * gamma|.
 // Sums are fp32 in a fixed order.  The codes are formed from the fp32 y: rounding it to 16 bits first would cost
-// bf16 rows a bit of their 7-bit codes.  Bound by HBM for many rows (16 384 x 4096 bf16 to E4M3, 470 MB: 79 us, 5.9 TB/s),
+// bf16 rows a bit of their 7-bit codes.  Bound by HBM for many rows (16 384 x 4096 bf16 to E4M3, 470 MB: 75 to 82 us, 5.7 to 6.2 TB/s),
 // by the latency of load, reduction and store for a few.
 template <typename T, int Mode, int Chunks, int Block>
 __global__ void __launch_bounds__(Block, 1024 / Block)
@@ -299,8 +299,8 @@ extern "C" int pk100_add_rms_norm(void* stream, const pk100_rms_norm_args* a) {
     p.vec_res_out = vec(a->residual_out, a->ld_res_out, 16);
     p.vec_gamma = vec(a->gamma, 8, 16);
     p.vec_out = vec(a->output, a->ld_out, a->mode == PK100_LN_F16 ? 16 : 8);
-    // As few chunks a thread as have all rows resident at once, the shortest chain (777 x 2560: 5.1 us with two, 7.3 with four);
-    // more rows: four in flight a thread (16 384 x 4096 in 79 us; two: 91 to 128, eight: 117).  A row that 32 threads hold
+    // As few chunks a thread as have all rows resident at once, the shortest chain (777 x 2560: 4.5 us with two, 5.4
+    // with one, 6.6 with four); more rows: four in flight a thread (16 384 x 4096 to E4M3 in 75 us; two: 86, one: 124).  A row that 32 threads hold
     // goes to a warp, without the exchange through shared memory.
     const int need = (a->width + 7) / 8;
     int chunks = 1;
