@@ -20,6 +20,18 @@ __device__ __forceinline__ uint32_t packed_of(float lo, float hi, __nv_bfloat16)
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// The same, rounded towards zero.
+__device__ __forceinline__ uint32_t packed_below(float lo, float hi, __half) {
+    uint32_t r;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t packed_below(float lo, float hi, __nv_bfloat16) {
+    uint32_t r;
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
 // 8 elements of a row from `column` on, packed; those at or behind `width` read as zero.  vec: 16-byte aligned and whole.
 template <typename T>
 __device__ __forceinline__ uint4 load8(const T* row, int column, int width, bool vec) {

@@ -174,7 +174,7 @@ __device__ __forceinline__ void join_row(const PagedParams& p, const PagedReques
 // A warp requests 64-key stages by TMA (a page or part of one a box, 128-byte swizzle), two blocks an SM keep up to
 // six of them in flight.  Q.K: each of four warps 16 keys; the row maxima are exchanged, so that all warps scale
 // alike; P through shared memory; P.V: each warp a quarter of the features.
-// Scores, maxima, sums and outputs are fp32; P goes to the tensor cores in two numbers of the type of V, the rounded weight and
+// Scores, maxima, sums and outputs are fp32; P goes to the tensor cores in two numbers of the type of V, the weight cut off and
 // the rounded rest: one alone had cost what the rounding of the output costs, two cost 2 us of 128, as long as the cache's bytes
 // decide.  The tensor cores cut off what falls below the last
 // bit of the sum that they add to: a block's products begin at zero and are added to the row's by the FMA pipe, which rounds.
@@ -378,11 +378,13 @@ paged_attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __g
                     b1 += y0 + y1;
                     const int chunk = 2 * warp + nt;
                     auto put = [&](float u, float v, int row) {
-                        const uint32_t near = packed_of(u, v, T());
+                        // cut off, so that the rest has no other sign, and the rest of what is not zero not zero: an infinite
+                        // value times the two is infinite (its last bit is set where the weight's halves, plus 0x7fff, reach the sign)
+                        const uint32_t near = packed_below(u, v, T());
                         const float2 r = floats_of(near, T());
                         const int at = row * 128 + ((chunk ^ g) << 4) + 4 * c;
                         *reinterpret_cast<uint32_t*>(&sm.p[buf][0][at]) = near;
-                        *reinterpret_cast<uint32_t*>(&sm.p[buf][1][at]) = packed_of(u - r.x, v - r.y, T());
+                        *reinterpret_cast<uint32_t*>(&sm.p[buf][1][at]) = packed_of(u - r.x, v - r.y, T()) | (((near + 0x7fff7fffu) >> 15) & 0x00010001u);
                     };
                     put(x0 * kFactor, x1 * kFactor, g);
                     put(y0 * kFactor, y1 * kFactor, g + 8);
