@@ -56,7 +56,7 @@ template <int D>
 struct RowsSmem {
     uint8_t k[rows_stages<D>()][D / 64][kBlock * 128];
     uint8_t v[rows_stages<D>()][D / 64][kBlock * 128];
-    uint8_t p[2][2][kRows * 128];              // weights and what their rounding left
+    uint8_t p[2][2][kRows * 128];              // weights cut off, and their rests
     float top[2][kRowWarps][kRows];
     float sum[kRowWarps][kRows];
     long long scan[kRowThreads / 32];
